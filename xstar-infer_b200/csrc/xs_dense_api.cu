@@ -1,0 +1,509 @@
+// C ABI of include/xs_moe_dense.h: argument checks, workspace plans and launches.  No exception leaves this file.
+#include "xs_moe_dense.h"
+
+#include "xs_api_common.cuh"
+#include "xs_norm_residual.cuh"
+#include "xs_w4_rows.cuh"
+
+using namespace xs_api;
+
+namespace {
+
+// A pointer the kernels may follow: device (or managed) memory of the current device.
+int check_on_device(const void *p, int device, const char *name)
+{
+    cudaPointerAttributes at;
+    if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+        cudaGetLastError();
+        return fail(XS_MOE_ERR_INVALID_ARG, "device mismatch: %s is not device memory", name);
+    }
+    if (at.type == cudaMemoryTypeManaged)
+        return 0;
+    if (at.type != cudaMemoryTypeDevice)
+        return fail(XS_MOE_ERR_INVALID_ARG, "device mismatch: %s is not device memory", name);
+    if (at.device != device)
+        return fail(XS_MOE_ERR_INVALID_ARG, "device mismatch: %s is on device %d, the current device is %d", name, at.device, device);
+    return 0;
+}
+
+int current_device(int *dev)
+{
+    XS_CUDA(cudaGetDevice(dev));
+    return 0;
+}
+
+bool overlap(const void *a, size_t an, const void *b, size_t bn)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && an && bn && x < y + bn && y < x + an;
+}
+
+bool misaligned(const void *p, uintptr_t n)
+{
+    return reinterpret_cast<uintptr_t>(p) % n != 0;
+}
+
+// shapes only: what the workspace queries need
+int check_w4_shape(const XsMoeW4 *w, int32_t tokens)
+{
+    if (!w)
+        return fail(XS_MOE_ERR_INVALID_ARG, "weight is null");
+    if (w->reserved != 0)
+        return fail(XS_MOE_ERR_INVALID_ARG, "reserved fields must be zero");
+    if (tokens < 0 || w->rows <= 0 || w->cols <= 0)
+        return fail(XS_MOE_ERR_INVALID_ARG, "shape mismatch: non-positive dimension");
+    if (w->group != 32 && w->group != 64 && w->group != 128)
+        return fail(XS_MOE_ERR_UNSUPPORTED, "group must be 32, 64 or 128");
+    if (w->cols % w->group != 0)
+        return fail(XS_MOE_ERR_INVALID_ARG, "shape mismatch: columns must be a multiple of the group");
+    return 0;
+}
+
+int check_gated_shape(const XsMoeW4 *w, int32_t activation, int32_t tokens)
+{
+    if (int rc = check_w4_shape(w, tokens))
+        return rc;
+    if (w->rows % 2 != 0)
+        return fail(XS_MOE_ERR_INVALID_ARG, "gate_up out must be even");
+    if (activation != XS_MOE_SILU && activation != XS_MOE_GELU_TANH)
+        return fail(XS_MOE_ERR_UNSUPPORTED, "unknown activation");
+    return 0;
+}
+
+int check_mlp_shape(const XsMoeW4 *gu, const XsMoeW4 *dn, int32_t activation, int32_t tokens)
+{
+    if (int rc = check_gated_shape(gu, activation, tokens))
+        return rc;
+    if (int rc = check_w4_shape(dn, tokens))
+        return rc;
+    if (dn->cols != gu->rows / 2 || dn->rows != gu->cols)
+        return fail(XS_MOE_ERR_INVALID_ARG, "shape mismatch: down must be (hidden, intermediate)");
+    return 0;
+}
+
+int check_w4_data(const XsMoeW4 *w, int dev)
+{
+    if (!w->codes_dev || !w->scales_dev)
+        return fail(XS_MOE_ERR_INVALID_ARG, "null tensor pointer");
+    if (misaligned(w->codes_dev, 16) || misaligned(w->scales_dev, 2))
+        return fail(XS_MOE_ERR_INVALID_ARG, "tensors must be 16-byte aligned (scales 2-byte)");
+    if (int rc = check_on_device(w->codes_dev, dev, "codes"))
+        return rc;
+    if (int rc = check_on_device(w->scales_dev, dev, "scales"))
+        return rc;
+    return w->zeros_dev ? check_on_device(w->zeros_dev, dev, "zeros") : 0;
+}
+
+// in_place: the caller may write the result over x itself (same address)
+int check_io(const void *x, size_t x_elems, void *out, size_t out_elems, const void *ws, size_t ws_bytes, int dev, bool in_place = false)
+{
+    if (!x || !out)
+        return fail(XS_MOE_ERR_INVALID_ARG, "null tensor pointer");
+    if (misaligned(x, 16) || misaligned(out, 2))
+        return fail(XS_MOE_ERR_INVALID_ARG, "x must be 16-byte aligned, out 2-byte");
+    if ((!(in_place && x == out) && overlap(x, x_elems * 2, out, out_elems * 2)) || overlap(x, x_elems * 2, ws, ws_bytes) || overlap(out, out_elems * 2, ws, ws_bytes))
+        return fail(XS_MOE_ERR_INVALID_ARG, "x, out and the workspace must not overlap");
+    if (int rc = check_on_device(x, dev, "x"))
+        return rc;
+    if (int rc = check_on_device(out, dev, "out"))
+        return rc;
+    return check_on_device(ws, dev, "workspace");
+}
+
+size_t bf16_bytes(size_t rows, size_t cols)
+{
+    return align_up(rows * cols * 2, 256);
+}
+
+xs::W4Matrix matrix_of(const XsMoeW4 *w)
+{
+    return {static_cast<const uint8_t *>(w->codes_dev), static_cast<const __nv_bfloat16 *>(w->scales_dev), w->zeros_dev};
+}
+
+int launch_w4(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void *out, cudaStream_t st)
+{
+    const int n_out = gated ? w->rows / 2 : w->rows;
+    const dim3 grid((n_out + 7) / 8, (T + 7) / 8);
+    const __nv_bfloat16 *xb = static_cast<const __nv_bfloat16 *>(x);
+    __nv_bfloat16 *ob = static_cast<__nv_bfloat16 *>(out);
+    if (gated)
+        XS_CUDA(launch_pdl(xs::w4_rows_kernel<true>, grid, 256, 0, st, matrix_of(w), xb, ob, n_out, T, w->cols, w->group, act));
+    else
+        XS_CUDA(launch_pdl(xs::w4_rows_kernel<false>, grid, 256, 0, st, matrix_of(w), xb, ob, n_out, T, w->cols, w->group, act));
+    note_launch();
+    return 0;
+}
+
+int launch_norm_residual(const xs::NormResidualArgs &a, cudaStream_t st)
+{
+    const size_t smem = static_cast<size_t>(a.H) * 4;
+    if (smem > 48 * 1024)
+        XS_CUDA(cudaFuncSetAttribute(xs::norm_residual_loop_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    XS_CUDA(launch_pdl(xs::norm_residual_loop_kernel, a.rows, xs::kNrLoopThreads, smem, st, a));
+    note_launch();
+    return 0;
+}
+
+constexpr int kNormMaxHidden = 56 * 1024; // a row in shared memory as f32
+
+int check_norm_shape(int gate_kind, const void *gate, int32_t rows, int32_t hidden)
+{
+    if (gate_kind < XS_MOE_GATE_NONE || gate_kind > XS_MOE_GATE_FULL)
+        return fail(XS_MOE_ERR_INVALID_ARG, "unknown gate kind");
+    if ((gate != nullptr) != (gate_kind != XS_MOE_GATE_NONE))
+        return fail(XS_MOE_ERR_INVALID_ARG, "gate and gate kind disagree");
+    if (rows < 0 || hidden <= 0)
+        return fail(XS_MOE_ERR_INVALID_ARG, "shape mismatch: non-positive dimension");
+    if (hidden > kNormMaxHidden)
+        return fail(XS_MOE_ERR_UNSUPPORTED, "hidden must be at most %d", kNormMaxHidden);
+    return 0;
+}
+
+size_t gate_elems(int kind, size_t rows, size_t hidden)
+{
+    return kind == XS_MOE_GATE_CHANNEL ? hidden : kind == XS_MOE_GATE_ROW ? rows : kind == XS_MOE_GATE_FULL ? rows * hidden : 0;
+}
+
+int check_norm(const XsMoeNormResidual *a)
+{
+    if (!a)
+        return fail(XS_MOE_ERR_INVALID_ARG, "arguments are null");
+    if (a->reserved[0] || a->reserved[1])
+        return fail(XS_MOE_ERR_INVALID_ARG, "reserved fields must be zero");
+    if (int rc = check_norm_shape(a->gate_kind, a->gate_dev, a->rows, a->hidden))
+        return rc;
+    if (!a->residual_dev)
+        return fail(XS_MOE_ERR_INVALID_ARG, "null tensor pointer");
+    if ((a->next_weight_dev != nullptr) != (a->next_out_dev != nullptr))
+        return fail(XS_MOE_ERR_INVALID_ARG, "next weight and next output go together");
+    if (a->y_dev ? !a->residual_out_dev : (a->residual_out_dev || a->post_weight_dev || a->gate_dev || !a->next_out_dev))
+        return fail(XS_MOE_ERR_INVALID_ARG, "y and residual_out go together; without y there is only the next norm");
+    if (a->rows == 0)
+        return 0;
+    const void *ptr[] = {a->y_dev, a->residual_dev, a->post_weight_dev, a->gate_dev, a->next_weight_dev, a->residual_out_dev, a->next_out_dev};
+    const char *name[] = {"y", "residual", "post weight", "gate", "next weight", "residual_out", "next_out"};
+    const size_t full = static_cast<size_t>(a->rows) * a->hidden, h = a->hidden;
+    const size_t elems[] = {full, full, h, gate_elems(a->gate_kind, a->rows, a->hidden), h, full, full};
+    int dev = 0;
+    if (int rc = current_device(&dev))
+        return rc;
+    for (int i = 0; i < 7; i++) {
+        if (!ptr[i])
+            continue;
+        if (misaligned(ptr[i], 2))
+            return fail(XS_MOE_ERR_INVALID_ARG, "tensors must be 2-byte aligned");
+        if (int rc = check_on_device(ptr[i], dev, name[i]))
+            return rc;
+    }
+    for (int o = 5; o < 7; o++)
+        for (int i = 0; i < 7; i++) {
+            // every element of y and residual is read by the thread that writes it, before it does: the same address is fine
+            const bool in_place = i < 2 && ptr[i] == ptr[o];
+            if (i != o && !in_place && overlap(ptr[o], elems[o] * 2, ptr[i], elems[i] * 2))
+                return fail(XS_MOE_ERR_INVALID_ARG, "%s overlaps %s", name[o], name[i]);
+        }
+    return 0;
+}
+
+int run_norm(const XsMoeNormResidual *a, cudaStream_t st)
+{
+    if (a->rows == 0)
+        return 0;
+    xs::NormResidualArgs k;
+    k.y = static_cast<const __nv_bfloat16 *>(a->y_dev);
+    k.r = static_cast<const __nv_bfloat16 *>(a->residual_dev);
+    k.w_post = static_cast<const __nv_bfloat16 *>(a->post_weight_dev);
+    k.gate = static_cast<const __nv_bfloat16 *>(a->gate_dev);
+    k.w_next = static_cast<const __nv_bfloat16 *>(a->next_weight_dev);
+    k.r_out = static_cast<__nv_bfloat16 *>(a->residual_out_dev);
+    k.n_out = static_cast<__nv_bfloat16 *>(a->next_out_dev);
+    k.gate_kind = a->gate_kind;
+    k.rows = a->rows;
+    k.H = a->hidden;
+    k.eps = a->eps;
+    k.c = a->residual_scale;
+    k.offset = a->weight_offset;
+    return launch_norm_residual(k, st);
+}
+
+int check_block_norms(const XsMoeBlockNorms *n, int32_t rows, int32_t hidden, int dev)
+{
+    if (!n)
+        return fail(XS_MOE_ERR_INVALID_ARG, "norms are null");
+    if (n->reserved[0] || n->reserved[1])
+        return fail(XS_MOE_ERR_INVALID_ARG, "reserved fields must be zero");
+    if (int rc = check_norm_shape(n->gate_kind, n->gate_dev, rows, hidden))
+        return rc;
+    if (!n->pre_weight_dev)
+        return fail(XS_MOE_ERR_INVALID_ARG, "null tensor pointer");
+    const void *ptr[] = {n->pre_weight_dev, n->post_weight_dev, n->gate_dev};
+    const char *name[] = {"pre weight", "post weight", "gate"};
+    for (int i = 0; i < 3; i++) {
+        if (!ptr[i])
+            continue;
+        if (misaligned(ptr[i], 2))
+            return fail(XS_MOE_ERR_INVALID_ARG, "tensors must be 2-byte aligned");
+        if (int rc = check_on_device(ptr[i], dev, name[i]))
+            return rc;
+    }
+    return 0;
+}
+
+// what the norms of a block write must not be what they read later
+int check_block_overlap(const XsMoeBlockNorms *n, int32_t rows, int32_t hidden, const void *out, const void *ws, size_t ws_bytes)
+{
+    const size_t h = static_cast<size_t>(hidden) * 2, full = h * rows, g = gate_elems(n->gate_kind, rows, hidden) * 2;
+    const void *ptr[] = {n->pre_weight_dev, n->post_weight_dev, n->gate_dev};
+    const size_t len[] = {h, h, g};
+    for (int i = 0; i < 3; i++)
+        if (overlap(ptr[i], len[i], out, full) || overlap(ptr[i], len[i], ws, ws_bytes))
+            return fail(XS_MOE_ERR_INVALID_ARG, "a norm weight or the gate overlaps out or the workspace");
+    return 0;
+}
+
+XsMoeNormResidual pre_norm(const XsMoeBlockNorms *n, const void *x, void *xn, int32_t rows, int32_t hidden)
+{
+    XsMoeNormResidual a{};
+    a.residual_dev = x;
+    a.next_weight_dev = n->pre_weight_dev;
+    a.next_out_dev = xn;
+    a.rows = rows;
+    a.hidden = hidden;
+    a.eps = n->eps;
+    a.residual_scale = 1.0f;
+    a.weight_offset = n->weight_offset;
+    return a;
+}
+
+XsMoeNormResidual block_tail(const XsMoeBlockNorms *n, const void *y, const void *x, void *out, int32_t rows, int32_t hidden)
+{
+    XsMoeNormResidual a{};
+    a.y_dev = y;
+    a.residual_dev = x;
+    a.post_weight_dev = n->post_weight_dev;
+    a.gate_dev = n->gate_dev;
+    a.gate_kind = n->gate_kind;
+    a.residual_out_dev = out;
+    a.rows = rows;
+    a.hidden = hidden;
+    a.eps = n->eps;
+    a.residual_scale = n->residual_scale;
+    a.weight_offset = n->weight_offset;
+    return a;
+}
+
+int run_mlp(const XsMoeW4 *gu, const XsMoeW4 *dn, int32_t act, const void *x, int32_t tokens, void *out, uint8_t *scratch, cudaStream_t st)
+{
+    if (int rc = launch_w4(gu, true, act, x, tokens, scratch, st))
+        return rc;
+    return launch_w4(dn, false, 0, scratch, tokens, out, st);
+}
+
+// the fail() string may allocate: an exception of the host library becomes a status like every other failure
+template <typename F>
+int guarded(F &&f) noexcept
+{
+    try {
+        return f();
+    } catch (...) {
+        return XS_MOE_ERR_CUDA;
+    }
+}
+
+} // namespace
+
+extern "C" {
+
+int xs_moe_linear_w4_workspace_bytes(const XsMoeW4 *w, int32_t tokens, size_t *bytes)
+{
+    return guarded([&]() -> int {
+        if (int rc = check_w4_shape(w, tokens))
+            return rc;
+        if (!bytes)
+            return fail(XS_MOE_ERR_INVALID_ARG, "null out-pointer");
+        *bytes = kStatusBytes;
+        return 0;
+    });
+}
+
+int xs_moe_linear_w4(const XsMoeW4 *w, const void *x, int32_t tokens, void *out, void *ws, size_t ws_bytes, void *stream)
+{
+    return guarded([&]() -> int {
+        if (int rc = check_w4_shape(w, tokens))
+            return rc;
+        if (tokens == 0)
+            return 0;
+        if (int rc = check_workspace(ws, ws_bytes, kStatusBytes))
+            return rc;
+        int dev = 0;
+        if (int rc = current_device(&dev))
+            return rc;
+        if (int rc = check_w4_data(w, dev))
+            return rc;
+        if (int rc = check_io(x, static_cast<size_t>(tokens) * w->cols, out, static_cast<size_t>(tokens) * w->rows, ws, kStatusBytes, dev))
+            return rc;
+        return launch_w4(w, false, 0, x, tokens, out, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int xs_moe_gated_w4(const XsMoeW4 *gate_up, int32_t activation, const void *x, int32_t tokens, void *h, void *ws, size_t ws_bytes, void *stream)
+{
+    return guarded([&]() -> int {
+        if (int rc = check_gated_shape(gate_up, activation, tokens))
+            return rc;
+        if (tokens == 0)
+            return 0;
+        if (int rc = check_workspace(ws, ws_bytes, kStatusBytes))
+            return rc;
+        int dev = 0;
+        if (int rc = current_device(&dev))
+            return rc;
+        if (int rc = check_w4_data(gate_up, dev))
+            return rc;
+        if (int rc = check_io(x, static_cast<size_t>(tokens) * gate_up->cols, h, static_cast<size_t>(tokens) * (gate_up->rows / 2), ws, kStatusBytes, dev))
+            return rc;
+        return launch_w4(gate_up, true, activation, x, tokens, h, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int xs_moe_mlp_w4_workspace_bytes(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t tokens, size_t *bytes)
+{
+    return guarded([&]() -> int {
+        if (int rc = check_mlp_shape(gate_up, down, XS_MOE_SILU, tokens))
+            return rc;
+        if (!bytes)
+            return fail(XS_MOE_ERR_INVALID_ARG, "null out-pointer");
+        *bytes = kStatusBytes + bf16_bytes(tokens, gate_up->rows / 2);
+        return 0;
+    });
+}
+
+int xs_moe_mlp_w4(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t activation, const void *x, int32_t tokens, void *out, void *ws,
+                  size_t ws_bytes, void *stream)
+{
+    return guarded([&]() -> int {
+        if (int rc = check_mlp_shape(gate_up, down, activation, tokens))
+            return rc;
+        if (tokens == 0)
+            return 0;
+        const size_t need = kStatusBytes + bf16_bytes(tokens, gate_up->rows / 2);
+        if (int rc = check_workspace(ws, ws_bytes, need))
+            return rc;
+        int dev = 0;
+        if (int rc = current_device(&dev))
+            return rc;
+        if (int rc = check_w4_data(gate_up, dev))
+            return rc;
+        if (int rc = check_w4_data(down, dev))
+            return rc;
+        const size_t n = static_cast<size_t>(tokens) * gate_up->cols;
+        if (int rc = check_io(x, n, out, n, ws, need, dev))
+            return rc;
+        return run_mlp(gate_up, down, activation, x, tokens, out, static_cast<uint8_t *>(ws) + kStatusBytes, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int xs_moe_norm_residual(const XsMoeNormResidual *args, void *stream)
+{
+    return guarded([&]() -> int {
+        if (int rc = check_norm(args))
+            return rc;
+        return run_norm(args, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int xs_moe_mlp_w4_block_workspace_bytes(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t tokens, size_t *bytes)
+{
+    if (int rc = xs_moe_mlp_w4_workspace_bytes(gate_up, down, tokens, bytes))
+        return rc;
+    *bytes += 2 * bf16_bytes(tokens, gate_up->cols);
+    return 0;
+}
+
+int xs_moe_mlp_w4_block(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t activation, const XsMoeBlockNorms *norms, const void *x,
+                        int32_t tokens, void *out, void *ws, size_t ws_bytes, void *stream)
+{
+    return guarded([&]() -> int {
+        if (int rc = check_mlp_shape(gate_up, down, activation, tokens))
+            return rc;
+        int dev = 0;
+        if (int rc = current_device(&dev))
+            return rc;
+        const int32_t H = gate_up->cols;
+        if (int rc = check_block_norms(norms, tokens, H, dev))
+            return rc;
+        if (tokens == 0)
+            return 0;
+        const size_t act_bytes = bf16_bytes(tokens, gate_up->rows / 2), row_bytes = bf16_bytes(tokens, H);
+        const size_t need = kStatusBytes + act_bytes + 2 * row_bytes;
+        if (int rc = check_workspace(ws, ws_bytes, need))
+            return rc;
+        if (int rc = check_w4_data(gate_up, dev))
+            return rc;
+        if (int rc = check_w4_data(down, dev))
+            return rc;
+        const size_t n = static_cast<size_t>(tokens) * H;
+        if (int rc = check_io(x, n, out, n, ws, need, dev, true))
+            return rc;
+        if (int rc = check_block_overlap(norms, tokens, H, out, ws, need))
+            return rc;
+        uint8_t *h = static_cast<uint8_t *>(ws) + kStatusBytes, *xn = h + act_bytes, *y = xn + row_bytes;
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        const XsMoeNormResidual pre = pre_norm(norms, x, xn, tokens, H), tail = block_tail(norms, y, x, out, tokens, H);
+        if (int rc = run_norm(&pre, st))
+            return rc;
+        if (int rc = run_mlp(gate_up, down, activation, xn, tokens, y, h, st))
+            return rc;
+        return run_norm(&tail, st);
+    });
+}
+
+int xs_moe_normed_block_workspace_bytes(const XsMoeConfig *cfg, size_t *bytes)
+{
+    if (int rc = xs_moe_workspace_bytes(cfg, bytes))
+        return rc;
+    *bytes = align_up(*bytes, 256) + 2 * bf16_bytes(cfg->num_tokens, cfg->hidden);
+    return 0;
+}
+
+int xs_moe_normed_block_forward(const XsMoeConfig *cfg, const XsMoeWeights *w, const XsMoeBlockNorms *norms, const void *x, void *out,
+                                void *ws, size_t ws_bytes, void *stream)
+{
+    return guarded([&]() -> int {
+        size_t fwd = 0;
+        if (int rc = xs_moe_workspace_bytes(cfg, &fwd))
+            return rc;
+        const int32_t T = cfg->num_tokens, H = cfg->hidden;
+        int dev = 0;
+        if (int rc = current_device(&dev))
+            return rc;
+        if (int rc = check_block_norms(norms, T, H, dev))
+            return rc;
+        if (T == 0)
+            return 0;
+        const size_t row_bytes = bf16_bytes(T, H), inner = align_up(fwd, 256), need = inner + 2 * row_bytes;
+        if (int rc = check_workspace(ws, ws_bytes, need))
+            return rc;
+        const size_t n = static_cast<size_t>(T) * H;
+        if (int rc = check_io(x, n, out, n, ws, need, dev, true))
+            return rc;
+        if (int rc = check_block_overlap(norms, T, H, out, ws, need))
+            return rc;
+        uint8_t *xn = static_cast<uint8_t *>(ws) + inner, *y = xn + row_bytes;
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (norms->weight_offset == 0.0f && !misaligned(norms->pre_weight_dev, 16)) {
+            if (int rc = xs_moe_rmsnorm(x, norms->pre_weight_dev, xn, T, H, norms->eps, stream))
+                return rc;
+        } else {
+            const XsMoeNormResidual pre = pre_norm(norms, x, xn, T, H);
+            if (int rc = run_norm(&pre, st))
+                return rc;
+        }
+        if (int rc = xs_moe_forward(cfg, w, xn, y, ws, inner, stream))
+            return rc;
+        const XsMoeNormResidual tail = block_tail(norms, y, x, out, T, H);
+        return run_norm(&tail, st);
+    });
+}
+
+} // extern "C"

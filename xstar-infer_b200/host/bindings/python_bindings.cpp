@@ -9,6 +9,7 @@
 #include <cstring>
 
 #include "cuda/cuda_allocator.h"
+#include "ops/dense_w4.h"
 #include "ops/moe.h"
 #include "ops/moe_ep.h"
 #include "parallel/ep_group.h"
@@ -80,17 +81,39 @@ Tensor moe_py(const Tensor &x, const Tensor &router_weight, const Tensor &gate_u
     return moe(x, w, cfg);
 }
 
+W4Weight w4_of(const Tensor &codes, const Tensor &scales, py::object zeros)
+{
+    return {&codes, &scales, opt(zeros)};
+}
+
+NormResidual norm_of(float eps, py::object post_norm_weight, py::object gate, float residual_scale, float weight_offset,
+                     py::object next_norm_weight)
+{
+    NormResidual p;
+    p.eps = eps;
+    p.post_norm_weight = opt(post_norm_weight);
+    p.gate = opt(gate);
+    p.residual_scale = residual_scale;
+    p.weight_offset = weight_offset;
+    p.next_norm_weight = opt(next_norm_weight);
+    return p;
+}
+
+// post_norm_weight, gate and residual_scale put a norm, a gate and a scale on the layer's branch; without them this is the
+// plain block, x + moe(rmsnorm(x))
 Tensor moe_block_py(const Tensor &x, const Tensor &norm_weight, float eps, const Tensor &router_weight, const Tensor &gate_up_weight,
                     const Tensor &down_weight, std::int64_t top_k, py::object router_bias, py::object gate_up_scale, py::object down_scale,
                     py::object shared_gate_up_weight, py::object shared_down_weight, py::object shared_gate_up_scale,
-                    py::object shared_down_scale)
+                    py::object shared_down_scale, py::object post_norm_weight, py::object gate, float residual_scale, float weight_offset)
 {
     MoEWeights w = weights_of(router_weight, gate_up_weight, down_weight, router_bias, gate_up_scale, down_scale, shared_gate_up_weight,
                               shared_down_weight, shared_gate_up_scale, shared_down_scale);
     MoEConfig cfg;
     cfg.top_k = top_k;
+    const bool plain = post_norm_weight.is_none() && gate.is_none() && residual_scale == 1.0f && weight_offset == 0.0f;
+    const NormResidual p = norm_of(eps, post_norm_weight, gate, residual_scale, weight_offset, py::none());
     py::gil_scoped_release nogil;
-    return moe_block(x, norm_weight, eps, w, cfg);
+    return plain ? moe_block(x, norm_weight, eps, w, cfg) : moe_block(x, norm_weight, w, cfg, p);
 }
 
 EpShape ep_shape(std::int64_t max_tokens, std::int64_t hidden, std::int64_t experts, std::int64_t top_k, std::int64_t intermediate,
@@ -144,6 +167,7 @@ PYBIND11_MODULE(xstar_cpp, m)
         .value("UE8M0", DType::UE8M0)
         .value("Int32", DType::Int32)
         .value("UInt8", DType::UInt8)
+        .value("UInt4x2", DType::UInt4x2)
         .export_values();
     py::enum_<Device>(m, "Device").value("CPU", Device::CPU).value("CUDA", Device::CUDA).export_values();
 
@@ -201,7 +225,131 @@ PYBIND11_MODULE(xstar_cpp, m)
           py::arg("gate_up_weight"), py::arg("down_weight"), py::arg("top_k"), py::arg("router_bias") = py::none(),
           py::arg("gate_up_scale") = py::none(), py::arg("down_scale") = py::none(), py::arg("shared_gate_up_weight") = py::none(),
           py::arg("shared_down_weight") = py::none(), py::arg("shared_gate_up_scale") = py::none(),
-          py::arg("shared_down_scale") = py::none());
+          py::arg("shared_down_scale") = py::none(), py::arg("post_norm_weight") = py::none(), py::arg("gate") = py::none(),
+          py::arg("residual_scale") = 1.0f, py::arg("weight_offset") = 0.0f);
+    m.def(
+        "moe_block_into",
+        [](const Tensor &x, const Tensor &norm_weight, Tensor &out, MoEScratch &scratch, std::uintptr_t stream, float eps,
+           const Tensor &router_weight, const Tensor &gate_up_weight, const Tensor &down_weight, std::int64_t top_k, py::object router_bias,
+           py::object gate_up_scale, py::object down_scale, py::object shared_gate_up_weight, py::object shared_down_weight,
+           py::object shared_gate_up_scale, py::object shared_down_scale, py::object post_norm_weight, py::object gate, float residual_scale,
+           float weight_offset) {
+            MoEWeights w = weights_of(router_weight, gate_up_weight, down_weight, router_bias, gate_up_scale, down_scale, shared_gate_up_weight,
+                                      shared_down_weight, shared_gate_up_scale, shared_down_scale);
+            MoEConfig cfg;
+            cfg.top_k = top_k;
+            const NormResidual p = norm_of(eps, post_norm_weight, gate, residual_scale, weight_offset, py::none());
+            py::gil_scoped_release nogil;
+            moe_block_into(x, norm_weight, w, cfg, p, out, scratch, reinterpret_cast<void *>(stream));
+        },
+        py::arg("x"), py::arg("norm_weight"), py::arg("out"), py::arg("scratch"), py::arg("stream"), py::arg("eps"), py::arg("router_weight"),
+        py::arg("gate_up_weight"), py::arg("down_weight"), py::arg("top_k"), py::arg("router_bias") = py::none(),
+        py::arg("gate_up_scale") = py::none(), py::arg("down_scale") = py::none(), py::arg("shared_gate_up_weight") = py::none(),
+        py::arg("shared_down_weight") = py::none(), py::arg("shared_gate_up_scale") = py::none(), py::arg("shared_down_scale") = py::none(),
+        py::arg("post_norm_weight") = py::none(), py::arg("gate") = py::none(), py::arg("residual_scale") = 1.0f,
+        py::arg("weight_offset") = 0.0f);
+
+    // dense operators with 4-bit weights and the step between two blocks (ops/dense_w4.h).  The plain forms return finished
+    // results; the _into forms enqueue on `stream` (a cudaStream_t as an integer, 0 = the default stream) and return.
+    m.def(
+        "linear_w4",
+        [](const Tensor &x, const Tensor &codes, const Tensor &scales, py::object zeros) {
+            const W4Weight w = w4_of(codes, scales, zeros);
+            py::gil_scoped_release nogil;
+            return linear_w4(x, w);
+        },
+        py::arg("x"), py::arg("codes"), py::arg("scales"), py::arg("zeros") = py::none());
+    m.def(
+        "linear_w4_into",
+        [](const Tensor &x, const Tensor &codes, const Tensor &scales, Tensor &out, MoEScratch &scratch, std::uintptr_t stream, py::object zeros) {
+            const W4Weight w = w4_of(codes, scales, zeros);
+            py::gil_scoped_release nogil;
+            linear_w4_into(x, w, out, scratch, reinterpret_cast<void *>(stream));
+        },
+        py::arg("x"), py::arg("codes"), py::arg("scales"), py::arg("out"), py::arg("scratch"), py::arg("stream"), py::arg("zeros") = py::none());
+    m.def(
+        "mlp_w4",
+        [](const Tensor &x, const Tensor &gate_up_codes, const Tensor &gate_up_scales, const Tensor &down_codes, const Tensor &down_scales,
+           py::object gate_up_zeros, py::object down_zeros, const std::string &activation) {
+            const W4Weight gu = w4_of(gate_up_codes, gate_up_scales, gate_up_zeros), dn = w4_of(down_codes, down_scales, down_zeros);
+            const Activation act = activation_of(activation);
+            py::gil_scoped_release nogil;
+            return mlp_w4(x, gu, dn, act);
+        },
+        py::arg("x"), py::arg("gate_up_codes"), py::arg("gate_up_scales"), py::arg("down_codes"), py::arg("down_scales"),
+        py::arg("gate_up_zeros") = py::none(), py::arg("down_zeros") = py::none(), py::arg("activation") = "silu");
+    m.def(
+        "mlp_w4_into",
+        [](const Tensor &x, const Tensor &gate_up_codes, const Tensor &gate_up_scales, const Tensor &down_codes, const Tensor &down_scales,
+           Tensor &out, MoEScratch &scratch, std::uintptr_t stream, py::object gate_up_zeros, py::object down_zeros, const std::string &activation) {
+            const W4Weight gu = w4_of(gate_up_codes, gate_up_scales, gate_up_zeros), dn = w4_of(down_codes, down_scales, down_zeros);
+            const Activation act = activation_of(activation);
+            py::gil_scoped_release nogil;
+            mlp_w4_into(x, gu, dn, act, out, scratch, reinterpret_cast<void *>(stream));
+        },
+        py::arg("x"), py::arg("gate_up_codes"), py::arg("gate_up_scales"), py::arg("down_codes"), py::arg("down_scales"), py::arg("out"),
+        py::arg("scratch"), py::arg("stream"), py::arg("gate_up_zeros") = py::none(), py::arg("down_zeros") = py::none(),
+        py::arg("activation") = "silu");
+    m.def(
+        "norm_residual",
+        [](const Tensor &y, const Tensor &residual, float eps, py::object post_norm_weight, py::object gate, float residual_scale,
+           float weight_offset, py::object next_norm_weight) -> py::object {
+            const NormResidual p = norm_of(eps, post_norm_weight, gate, residual_scale, weight_offset, next_norm_weight);
+            NormResidualResult r;
+            {
+                py::gil_scoped_release nogil;
+                r = norm_residual(y, residual, p);
+            }
+            if (!p.next_norm_weight)
+                return py::make_tuple(py::cast(std::move(r.residual)), py::none());
+            return py::make_tuple(py::cast(std::move(r.residual)), py::cast(std::move(r.next)));
+        },
+        py::arg("y"), py::arg("residual"), py::arg("eps") = 1e-6f, py::arg("post_norm_weight") = py::none(), py::arg("gate") = py::none(),
+        py::arg("residual_scale") = 1.0f, py::arg("weight_offset") = 0.0f, py::arg("next_norm_weight") = py::none());
+    m.def(
+        "norm_residual_into",
+        [](const Tensor &y, const Tensor &residual, Tensor &out, std::uintptr_t stream, float eps, py::object post_norm_weight, py::object gate,
+           float residual_scale, float weight_offset, py::object next_norm_weight, py::object next_out) {
+            const NormResidual p = norm_of(eps, post_norm_weight, gate, residual_scale, weight_offset, next_norm_weight);
+            Tensor *next = next_out.is_none() ? nullptr : &next_out.cast<Tensor &>();
+            py::gil_scoped_release nogil;
+            norm_residual_into(y, residual, p, out, next, reinterpret_cast<void *>(stream));
+        },
+        py::arg("y"), py::arg("residual"), py::arg("out"), py::arg("stream"), py::arg("eps") = 1e-6f, py::arg("post_norm_weight") = py::none(),
+        py::arg("gate") = py::none(), py::arg("residual_scale") = 1.0f, py::arg("weight_offset") = 0.0f,
+        py::arg("next_norm_weight") = py::none(), py::arg("next_out") = py::none());
+    m.def(
+        "mlp_w4_block",
+        [](const Tensor &x, const Tensor &norm_weight, const Tensor &gate_up_codes, const Tensor &gate_up_scales, const Tensor &down_codes,
+           const Tensor &down_scales, float eps, py::object gate_up_zeros, py::object down_zeros, const std::string &activation,
+           py::object post_norm_weight, py::object gate, float residual_scale, float weight_offset) {
+            const W4Weight gu = w4_of(gate_up_codes, gate_up_scales, gate_up_zeros), dn = w4_of(down_codes, down_scales, down_zeros);
+            const Activation act = activation_of(activation);
+            const NormResidual p = norm_of(eps, post_norm_weight, gate, residual_scale, weight_offset, py::none());
+            py::gil_scoped_release nogil;
+            return mlp_w4_block(x, norm_weight, gu, dn, act, p);
+        },
+        py::arg("x"), py::arg("norm_weight"), py::arg("gate_up_codes"), py::arg("gate_up_scales"), py::arg("down_codes"),
+        py::arg("down_scales"), py::arg("eps") = 1e-6f, py::arg("gate_up_zeros") = py::none(), py::arg("down_zeros") = py::none(),
+        py::arg("activation") = "silu", py::arg("post_norm_weight") = py::none(), py::arg("gate") = py::none(),
+        py::arg("residual_scale") = 1.0f, py::arg("weight_offset") = 0.0f);
+    m.def(
+        "mlp_w4_block_into",
+        [](const Tensor &x, const Tensor &norm_weight, const Tensor &gate_up_codes, const Tensor &gate_up_scales, const Tensor &down_codes,
+           const Tensor &down_scales, Tensor &out, MoEScratch &scratch, std::uintptr_t stream, float eps, py::object gate_up_zeros,
+           py::object down_zeros, const std::string &activation, py::object post_norm_weight, py::object gate, float residual_scale,
+           float weight_offset) {
+            const W4Weight gu = w4_of(gate_up_codes, gate_up_scales, gate_up_zeros), dn = w4_of(down_codes, down_scales, down_zeros);
+            const Activation act = activation_of(activation);
+            const NormResidual p = norm_of(eps, post_norm_weight, gate, residual_scale, weight_offset, py::none());
+            py::gil_scoped_release nogil;
+            mlp_w4_block_into(x, norm_weight, gu, dn, act, p, out, scratch, reinterpret_cast<void *>(stream));
+        },
+        py::arg("x"), py::arg("norm_weight"), py::arg("gate_up_codes"), py::arg("gate_up_scales"), py::arg("down_codes"),
+        py::arg("down_scales"), py::arg("out"), py::arg("scratch"), py::arg("stream"), py::arg("eps") = 1e-6f,
+        py::arg("gate_up_zeros") = py::none(), py::arg("down_zeros") = py::none(), py::arg("activation") = "silu",
+        py::arg("post_norm_weight") = py::none(), py::arg("gate") = py::none(), py::arg("residual_scale") = 1.0f,
+        py::arg("weight_offset") = 0.0f);
     // checkpoint IO (same names as the reference's module: MMapFile, parse_safetensors_header, make_weight_view)
     py::class_<MMapFile>(m, "MMapFile").def(py::init<const std::string &>(), py::arg("path")).def("size", &MMapFile::size);
     py::class_<TensorMeta>(m, "TensorMeta")

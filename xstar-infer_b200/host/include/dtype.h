@@ -13,6 +13,7 @@ enum class DType {
     UE8M0,        // power-of-two scale, biased exponent
     Int32,
     UInt8, // raw bytes: how a checkpoint file stores packed FP4 codes and e8m0 scales before the loader tags them
+    UInt4x2, // two unsigned 4-bit codes per byte (low nibble = even index); shapes count BYTES in the last dim
 };
 
 inline std::size_t dtype_size(DType d)
@@ -27,6 +28,7 @@ inline std::size_t dtype_size(DType d)
     case DType::Float4E2M1x2:
     case DType::UE8M0:
     case DType::UInt8:
+    case DType::UInt4x2:
         return 1;
     }
     throw std::runtime_error("unknown DType");
@@ -42,6 +44,7 @@ inline const char *dtype_name(DType d)
     case DType::UE8M0: return "UE8M0";
     case DType::Int32: return "Int32";
     case DType::UInt8: return "UInt8";
+    case DType::UInt4x2: return "UInt4x2";
     }
     return "?";
 }

@@ -29,15 +29,29 @@ def _sources(d, exts):
     return out
 
 
+# one object per translation unit (compiled side by side), linked into one library
+UNITS = ("xs_moe_api", "xs_dense_api")
+OBJ_DIR = os.path.join(PKG, "build")
+
+
 def build_cuda(force=False, verbose=False):
     srcs = _sources(CSRC, (".cu", ".cuh", ".inl", ".h")) + _sources(os.path.join(ROOT, "include"), (".h",))
     if not (force or _newer(LIB, srcs)):
         return LIB
-    cmd = ["nvcc", *NVCC_FLAGS, "-shared", "-Xcompiler", "-fPIC", "-I" + os.path.join(ROOT, "include"), "-o", LIB,
-           os.path.join(CSRC, "xs_moe_api.cu"), "-ldl"]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-    subprocess.run(cmd, check=True)
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    jobs = []
+    for unit in UNITS:
+        cmd = ["nvcc", *NVCC_FLAGS, "-c", "-Xcompiler", "-fPIC", "-I" + os.path.join(ROOT, "include"), "-o", os.path.join(OBJ_DIR, unit + ".o"),
+               os.path.join(CSRC, unit + ".cu")]
+        if verbose:
+            cmd.insert(1, "-Xptxas=-v")
+        jobs.append((cmd, subprocess.Popen(cmd)))
+    codes = [(cmd, job.wait()) for cmd, job in jobs]
+    for cmd, code in codes:
+        if code:
+            raise subprocess.CalledProcessError(code, cmd)
+    subprocess.run(["nvcc", *NVCC_FLAGS, "-shared", "-Xcompiler", "-fPIC", "-o", LIB, *(os.path.join(OBJ_DIR, u + ".o") for u in UNITS), "-ldl"],
+                   check=True)
     return LIB
 
 

@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in include/xs_moe.h and include/xs_moe_tuning.h.
+"""ctypes binding of the C ABI in include/xs_moe.h, include/xs_moe_dense.h and include/xs_moe_tuning.h.
 
 This is plumbing for the tests and the benchmark: it passes raw device pointers (from torch tensors or
 from the library's own allocator) straight to the `extern "C"` entry points.  There is no fallback: if the
@@ -37,6 +37,26 @@ class XsMoeWeights(C.Structure):
         "shared_gate_up_w_dev", "shared_gate_up_scale_dev", "shared_down_w_dev", "shared_down_scale_dev")]
 
 
+class XsMoeW4(C.Structure):
+    _fields_ = [("codes_dev", C.c_void_p), ("scales_dev", C.c_void_p), ("zeros_dev", C.c_void_p), ("rows", C.c_int32), ("cols", C.c_int32),
+                ("group", C.c_int32), ("reserved", C.c_int32)]
+
+
+class XsMoeNormResidual(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("y_dev", "residual_dev", "post_weight_dev", "gate_dev", "next_weight_dev", "residual_out_dev",
+                                          "next_out_dev")] + [
+        ("gate_kind", C.c_int32), ("rows", C.c_int32), ("hidden", C.c_int32), ("eps", C.c_float), ("residual_scale", C.c_float),
+        ("weight_offset", C.c_float), ("reserved", C.c_int32 * 2)]
+
+
+class XsMoeBlockNorms(C.Structure):
+    _fields_ = [("pre_weight_dev", C.c_void_p), ("post_weight_dev", C.c_void_p), ("gate_dev", C.c_void_p), ("gate_kind", C.c_int32),
+                ("eps", C.c_float), ("residual_scale", C.c_float), ("weight_offset", C.c_float), ("reserved", C.c_int32 * 2)]
+
+
+SILU, GELU_TANH = 0, 1
+GATE_NONE, GATE_CHANNEL, GATE_ROW, GATE_FULL = 0, 1, 2, 3
+
 IPC_HANDLE_BYTES = 64
 
 EXPORTS = [
@@ -51,6 +71,9 @@ EXPORTS = [
     "xs_moe_comm_async_error", "xs_moe_comm_all_gather", "xs_moe_comm_barrier", "xs_moe_comm_all_to_all_v", "xs_moe_stream_create",
     "xs_moe_stream_destroy", "xs_moe_event_create", "xs_moe_event_destroy", "xs_moe_event_record", "xs_moe_stream_wait_event",
     "xs_moe_memset_async", "xs_moe_enable_peer_access",
+    "xs_moe_linear_w4_workspace_bytes", "xs_moe_linear_w4", "xs_moe_gated_w4", "xs_moe_mlp_w4_workspace_bytes", "xs_moe_mlp_w4",
+    "xs_moe_norm_residual", "xs_moe_mlp_w4_block_workspace_bytes", "xs_moe_mlp_w4_block", "xs_moe_normed_block_workspace_bytes",
+    "xs_moe_normed_block_forward",
 ]
 
 _lib = None
@@ -67,7 +90,18 @@ def lib():
         L.xs_moe_last_error.restype = C.c_char_p
         vp, sz, i32 = C.c_void_p, C.c_size_t, C.c_int32
         cfgp, wp = C.POINTER(XsMoeConfig), C.POINTER(XsMoeWeights)
+        w4p, normsp = C.POINTER(XsMoeW4), C.POINTER(XsMoeBlockNorms)
         sig = {
+            "xs_moe_linear_w4_workspace_bytes": [w4p, i32, C.POINTER(sz)],
+            "xs_moe_linear_w4": [w4p, vp, i32, vp, vp, sz, vp],
+            "xs_moe_gated_w4": [w4p, i32, vp, i32, vp, vp, sz, vp],
+            "xs_moe_mlp_w4_workspace_bytes": [w4p, w4p, i32, C.POINTER(sz)],
+            "xs_moe_mlp_w4": [w4p, w4p, i32, vp, i32, vp, vp, sz, vp],
+            "xs_moe_norm_residual": [C.POINTER(XsMoeNormResidual), vp],
+            "xs_moe_mlp_w4_block_workspace_bytes": [w4p, w4p, i32, C.POINTER(sz)],
+            "xs_moe_mlp_w4_block": [w4p, w4p, i32, normsp, vp, i32, vp, vp, sz, vp],
+            "xs_moe_normed_block_workspace_bytes": [cfgp, C.POINTER(sz)],
+            "xs_moe_normed_block_forward": [cfgp, wp, normsp, vp, vp, vp, sz, vp],
             "xs_moe_device_check": [],
             "xs_moe_device_count": [C.POINTER(i32)],
             "xs_moe_set_device": [i32],
@@ -176,6 +210,15 @@ def make_weights(d):
     w.shared_down_w_dev = ptr(d.get("shared_down_w"))
     w.shared_down_scale_dev = ptr(d.get("shared_down_scale"))
     return w
+
+
+def make_w4(w):
+    """w: dict(q (rows, cols / 2) uint8, s (rows, cols / group) bf16, z (rows, cols / group) uint8 | None) (see synth.int4_groups)."""
+    m = XsMoeW4()
+    m.codes_dev, m.scales_dev, m.zeros_dev = ptr(w["q"]), ptr(w["s"]), ptr(w["z"])
+    m.rows, m.cols = w["q"].shape[0], w["q"].shape[1] * 2
+    m.group = m.cols // w["s"].shape[1]
+    return m
 
 
 def workspace_bytes(cfg):

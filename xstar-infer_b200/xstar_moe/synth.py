@@ -88,6 +88,22 @@ def _fp4_mx32(shape, std, gen, device):
     return codes, scales
 
 
+def int4_groups(shape, group, zeros, std, gen, device):
+    """A matrix of 4-bit integers with one bf16 scale (and, with `zeros`, one zero point) per `group` columns, from N(0, std) weights:
+    dict(q = codes two per byte, even column in the low nibble, s, z | None); W = (q - z) * s, z = 8 without zero points."""
+    R, K = shape
+    w = (torch.randn((R, K), generator=gen, device=device, dtype=torch.float32) * std).view(R, K // group, group)
+    if zeros:
+        lo, hi = w.amin(-1).clamp_max(0.0), w.amax(-1).clamp_min(0.0)
+        s = ((hi - lo).clamp_min(1e-10) / 15.0).to(torch.bfloat16)
+        z = torch.round(-lo / s.float()).clamp_(0, 15)
+    else:
+        s = (w.abs().amax(-1).clamp_min(1e-10) / 7.0).to(torch.bfloat16)
+        z = torch.full(s.shape, 8.0, device=device)
+    code = (torch.round(w / s.float().unsqueeze(-1)) + z.unsqueeze(-1)).clamp_(0, 15).to(torch.uint8).view(R, K)
+    return dict(q=(code[:, 0::2] | (code[:, 1::2] << 4)).contiguous(), s=s, z=z.to(torch.uint8) if zeros else None)
+
+
 def make_inputs(cfg, seed=0, device="cpu"):
     """Returns a dict of torch tensors in storage form:
        x (T,H) bf16, router_w (E,H) bf16, router_bias (E) f32 | None,
