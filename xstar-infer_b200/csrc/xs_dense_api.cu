@@ -4,6 +4,7 @@
 #include "xs_api_common.cuh"
 #include "xs_norm_residual.cuh"
 #include "xs_w4_rows.cuh"
+#include "xs_w4_small.cuh"
 
 using namespace xs_api;
 
@@ -120,16 +121,60 @@ xs::W4Matrix matrix_of(const XsMoeW4 *w)
     return {static_cast<const uint8_t *>(w->codes_dev), static_cast<const __nv_bfloat16 *>(w->scales_dev), w->zeros_dev};
 }
 
-int launch_w4(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void *out, cudaStream_t st)
+constexpr int kSmallTokens = 16;
+
+template <int TN, int MT, bool GATED, int SUB, bool ZEROS>
+int launch_small_t(const xs::W4Matrix &w, const __nv_bfloat16 *x, int T, __nv_bfloat16 *out, int n_out, int K, int act, bool early, int sms, cudaStream_t st)
 {
-    const int n_out = gated ? w->rows / 2 : w->rows;
-    const dim3 grid((n_out + 7) / 8, (T + 7) / 8);
+    constexpr int smem = xs::sw_smem_bytes(MT, TN);
+    constexpr int features = GATED ? 16 : 16 * MT;
+    constexpr int resident = 227 * 1024 / (smem + 1024);
+    auto kern = xs::w4_small_kernel<TN, MT, GATED, SUB, ZEROS>;
+    XS_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    const int tiles = (n_out + features - 1) / features, slots = sms * resident;
+    XS_CUDA(launch_pdl(kern, tiles < slots ? tiles : slots, 32 * xs::kSwWarps, smem, st, w, x, out, n_out, T, K, act, early ? 1 : 0));
+    note_launch();
+    return 0;
+}
+
+template <int SUB, bool ZEROS>
+int launch_small(const xs::W4Matrix &w, bool gated, const __nv_bfloat16 *x, int T, __nv_bfloat16 *out, int n_out, int K, int act, bool early,
+                 int sms, cudaStream_t st)
+{
+    if (gated)
+        return T <= 8 ? launch_small_t<1, 2, true, SUB, ZEROS>(w, x, T, out, n_out, K, act, early, sms, st)
+                      : launch_small_t<2, 2, true, SUB, ZEROS>(w, x, T, out, n_out, K, act, early, sms, st);
+    if (T <= 8)
+        return launch_small_t<1, 1, false, SUB, ZEROS>(w, x, T, out, n_out, K, act, early, sms, st);
+    return launch_small_t<2, 2, false, SUB, ZEROS>(w, x, T, out, n_out, K, act, early, sms, st);
+}
+
+// early: nothing that may still be running when the kernel starts writes the weights (the second product of one call)
+int launch_w4(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void *out, bool early, cudaStream_t st)
+{
+    DeviceInfo di;
+    if (int rc = device_info(&di))
+        return rc;
+    const int n_out = gated ? w->rows / 2 : w->rows, K = w->cols;
     const __nv_bfloat16 *xb = static_cast<const __nv_bfloat16 *>(x);
     __nv_bfloat16 *ob = static_cast<__nv_bfloat16 *>(out);
+    const xs::W4Matrix m = matrix_of(w);
+    if (T <= kSmallTokens) {
+        const bool z = w->zeros_dev != nullptr;
+        if (w->group == 32)
+            return z ? launch_small<1, true>(m, gated, xb, T, ob, n_out, K, act, early, di.sms, st)
+                     : launch_small<1, false>(m, gated, xb, T, ob, n_out, K, act, early, di.sms, st);
+        if (w->group == 64)
+            return z ? launch_small<2, true>(m, gated, xb, T, ob, n_out, K, act, early, di.sms, st)
+                     : launch_small<2, false>(m, gated, xb, T, ob, n_out, K, act, early, di.sms, st);
+        return z ? launch_small<4, true>(m, gated, xb, T, ob, n_out, K, act, early, di.sms, st)
+                 : launch_small<4, false>(m, gated, xb, T, ob, n_out, K, act, early, di.sms, st);
+    }
+    const dim3 grid((n_out + 7) / 8, (T + 7) / 8);
     if (gated)
-        XS_CUDA(launch_pdl(xs::w4_rows_kernel<true>, grid, 256, 0, st, matrix_of(w), xb, ob, n_out, T, w->cols, w->group, act));
+        XS_CUDA(launch_pdl(xs::w4_rows_kernel<true>, grid, 256, 0, st, m, xb, ob, n_out, T, K, w->group, act));
     else
-        XS_CUDA(launch_pdl(xs::w4_rows_kernel<false>, grid, 256, 0, st, matrix_of(w), xb, ob, n_out, T, w->cols, w->group, act));
+        XS_CUDA(launch_pdl(xs::w4_rows_kernel<false>, grid, 256, 0, st, m, xb, ob, n_out, T, K, w->group, act));
     note_launch();
     return 0;
 }
@@ -294,9 +339,9 @@ XsMoeNormResidual block_tail(const XsMoeBlockNorms *n, const void *y, const void
 
 int run_mlp(const XsMoeW4 *gu, const XsMoeW4 *dn, int32_t act, const void *x, int32_t tokens, void *out, uint8_t *scratch, cudaStream_t st)
 {
-    if (int rc = launch_w4(gu, true, act, x, tokens, scratch, st))
+    if (int rc = launch_w4(gu, true, act, x, tokens, scratch, false, st))
         return rc;
-    return launch_w4(dn, false, 0, scratch, tokens, out, st);
+    return launch_w4(dn, false, 0, scratch, tokens, out, true, st);
 }
 
 // the fail() string may allocate: an exception of the host library becomes a status like every other failure
@@ -342,7 +387,7 @@ int xs_moe_linear_w4(const XsMoeW4 *w, const void *x, int32_t tokens, void *out,
             return rc;
         if (int rc = check_io(x, static_cast<size_t>(tokens) * w->cols, out, static_cast<size_t>(tokens) * w->rows, ws, kStatusBytes, dev))
             return rc;
-        return launch_w4(w, false, 0, x, tokens, out, static_cast<cudaStream_t>(stream));
+        return launch_w4(w, false, 0, x, tokens, out, false, static_cast<cudaStream_t>(stream));
     });
 }
 
@@ -362,7 +407,7 @@ int xs_moe_gated_w4(const XsMoeW4 *gate_up, int32_t activation, const void *x, i
             return rc;
         if (int rc = check_io(x, static_cast<size_t>(tokens) * gate_up->cols, h, static_cast<size_t>(tokens) * (gate_up->rows / 2), ws, kStatusBytes, dev))
             return rc;
-        return launch_w4(gate_up, true, activation, x, tokens, h, static_cast<cudaStream_t>(stream));
+        return launch_w4(gate_up, true, activation, x, tokens, h, false, static_cast<cudaStream_t>(stream));
     });
 }
 

@@ -5,21 +5,9 @@
 #include <stdint.h>
 
 #include "xs_ptx.cuh"
+#include "xs_w4_common.cuh"
 
 namespace xs {
-
-struct W4Matrix {
-    const uint8_t *codes;        // (rows, K / 2)
-    const __nv_bfloat16 *scales; // (rows, K / G)
-    const uint8_t *zeros;        // (rows, K / G) or null: 8
-};
-
-__device__ __forceinline__ float w4_activation(float v, int act)
-{
-    if (act == 0)
-        return v / (1.0f + expf(-v));
-    return 0.5f * v * (1.0f + tanhf(0.7978845608028654f * (v + 0.044715f * v * v * v)));
-}
 
 template <bool GATED>
 __global__ void __launch_bounds__(256)
