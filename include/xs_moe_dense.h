@@ -40,7 +40,7 @@ typedef enum XsMoeActivation {
     XS_MOE_GELU_TANH = 1 /* v / 2 * (1 + tanh(sqrt(2 / pi) * (v + 0.044715 v^3))) */
 } XsMoeActivation;
 
-/* out (tokens, rows) bf16 = x (tokens, cols) bf16 times W^T; f32 sums, one rounding at the end.  Up to 16 tokens the weights
+/* out (tokens, rows) bf16 = x (tokens, cols) bf16 times W^T; f32 sums, one rounding at the end.  Up to 8 tokens the weights
  * enter the products exactly; larger batches round (q - z) * s to bf16 once for the tensor core (half a bf16 step per weight).
  * x is 16-byte aligned and does not overlap out.  Takes the role of gemm_launch behind linear
  * (xstar_cpp/include/ops/gemm.h:165-176). */

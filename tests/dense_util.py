@@ -12,7 +12,7 @@ F = torch.float64
 HALF = 2.0**-8  # half a bf16 step, relative to the value
 ACT = {"silu": capi.SILU, "gelu": capi.GELU_TANH}
 GATE = {"none": capi.GATE_NONE, "channel": capi.GATE_CHANNEL, "row": capi.GATE_ROW, "full": capi.GATE_FULL}
-EXACT_WEIGHT_TOKENS = 16  # up to here the weights enter the products unrounded
+EXACT_WEIGHT_TOKENS = 8  # up to here the weights enter the products unrounded
 
 
 def workspace(nbytes):

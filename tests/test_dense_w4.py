@@ -1,7 +1,7 @@
 """4-bit dense operators and the step between two blocks: refusals (no GPU needed) and results against 64-bit definitions.
 
 Tolerances: element by element from the roundings the operators are documented to make (dense_util), and in the norm: the
-roundings to bf16 (output, weights beyond 16 tokens, the gated product, the intermediate rows of a block) are off by at most
+roundings to bf16 (output, weights beyond 8 tokens, the gated product, the intermediate rows of a block) are off by at most
 half a step each, 2^-8, spread evenly, so each adds at most 2^-8 / sqrt(3) of the result in the root mean square, and no chain
 here has more than six: sqrt(6 / 3) * 2^-8 < 2^-7."""
 import ctypes as C

@@ -121,15 +121,12 @@ xs::W4Matrix matrix_of(const XsMoeW4 *w)
     return {static_cast<const uint8_t *>(w->codes_dev), static_cast<const __nv_bfloat16 *>(w->scales_dev), w->zeros_dev};
 }
 
-constexpr int kSmallTokens = 16;
-
-template <int TN, int MT, bool GATED, int SUB, bool ZEROS>
+template <int MT, bool GATED, int SUB, bool ZEROS>
 int launch_small_t(const xs::W4Matrix &w, const __nv_bfloat16 *x, int T, __nv_bfloat16 *out, int n_out, int K, int act, bool early, int sms, cudaStream_t st)
 {
-    constexpr int smem = xs::sw_smem_bytes(MT, TN);
     constexpr int features = GATED ? 16 : 16 * MT;
-    constexpr int resident = 227 * 1024 / (smem + 1024);
-    auto kern = xs::w4_small_kernel<TN, MT, GATED, SUB, ZEROS>;
+    const int smem = xs::sw_smem_bytes(MT, T), resident = 227 * 1024 / (smem + 1024);
+    auto kern = xs::w4_small_kernel<MT, GATED, SUB, ZEROS>;
     XS_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     const int tiles = (n_out + features - 1) / features, slots = sms * resident;
     XS_CUDA(launch_pdl(kern, tiles < slots ? tiles : slots, 32 * xs::kSwWarps, smem, st, w, x, out, n_out, T, K, act, early ? 1 : 0));
@@ -142,11 +139,10 @@ int launch_small(const xs::W4Matrix &w, bool gated, const __nv_bfloat16 *x, int 
                  int sms, cudaStream_t st)
 {
     if (gated)
-        return T <= 8 ? launch_small_t<1, 2, true, SUB, ZEROS>(w, x, T, out, n_out, K, act, early, sms, st)
-                      : launch_small_t<2, 2, true, SUB, ZEROS>(w, x, T, out, n_out, K, act, early, sms, st);
-    if (T <= 8)
-        return launch_small_t<1, 1, false, SUB, ZEROS>(w, x, T, out, n_out, K, act, early, sms, st);
-    return launch_small_t<2, 2, false, SUB, ZEROS>(w, x, T, out, n_out, K, act, early, sms, st);
+        return launch_small_t<2, true, SUB, ZEROS>(w, x, T, out, n_out, K, act, early, sms, st);
+    if (n_out >= 32 * 2 * sms)
+        return launch_small_t<2, false, SUB, ZEROS>(w, x, T, out, n_out, K, act, early, sms, st);
+    return launch_small_t<1, false, SUB, ZEROS>(w, x, T, out, n_out, K, act, early, sms, st);
 }
 
 // early: nothing that may still be running when the kernel starts writes the weights (the second product of one call)
@@ -159,7 +155,7 @@ int launch_w4(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void 
     const __nv_bfloat16 *xb = static_cast<const __nv_bfloat16 *>(x);
     __nv_bfloat16 *ob = static_cast<__nv_bfloat16 *>(out);
     const xs::W4Matrix m = matrix_of(w);
-    if (T <= kSmallTokens) {
+    if (T <= xs::kSwTokens) {
         const bool z = w->zeros_dev != nullptr;
         if (w->group == 32)
             return z ? launch_small<1, true>(m, gated, xb, T, ob, n_out, K, act, early, di.sms, st)
