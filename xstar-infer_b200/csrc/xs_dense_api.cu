@@ -121,32 +121,111 @@ xs::W4Matrix matrix_of(const XsMoeW4 *w)
     return {static_cast<const uint8_t *>(w->codes_dev), static_cast<const __nv_bfloat16 *>(w->scales_dev), w->zeros_dev};
 }
 
-template <int MT, bool GATED, int SUB, bool ZEROS>
-int launch_small_t(const xs::W4Matrix &w, const __nv_bfloat16 *x, int T, __nv_bfloat16 *out, int n_out, int K, int act, bool early, int sms, cudaStream_t st)
+// The codes as `parts` byte matrices one after the other (gate and up, or one), read in boxes of 128 bytes x box_rows of
+// each, 128-byte swizzle; bytes and rows past the end read as zero.
+int make_tmap_codes(CUtensorMap *m, const XsMoeW4 *w, int parts, uint32_t box_rows)
 {
-    constexpr int features = GATED ? 16 : 16 * MT;
-    const int smem = xs::sw_smem_bytes(MT, T), resident = 227 * 1024 / (smem + 1024);
-    auto kern = xs::w4_small_kernel<MT, GATED, SUB, ZEROS>;
-    XS_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    const int tiles = (n_out + features - 1) / features, slots = sms * resident;
-    XS_CUDA(launch_pdl(kern, tiles < slots ? tiles : slots, 32 * xs::kSwWarps, smem, st, w, x, out, n_out, T, K, act, early ? 1 : 0));
+    EncodeTiledFn fn = get_encode_fn();
+    if (!fn)
+        return fail(XS_MOE_ERR_CUDA, "CUDA error: cuTensorMapEncodeTiled entry point not available");
+    const cuuint64_t bytes = static_cast<cuuint64_t>(w->cols) / 2, rows = static_cast<cuuint64_t>(w->rows) / parts;
+    const cuuint64_t dims[3] = {bytes, rows, static_cast<cuuint64_t>(parts)}, strides[2] = {bytes, bytes * rows};
+    const cuuint32_t box[3] = {128, box_rows, static_cast<cuuint32_t>(parts)}, one[3] = {1, 1, 1};
+    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(w->codes_dev), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(XS_MOE_ERR_CUDA, "CUDA error: cuTensorMapEncodeTiled failed with code %d (rows=%d cols=%d)", (int)r, w->rows, w->cols);
+    return 0;
+}
+
+// A programmatic dependent launch in clusters of `cluster` blocks.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_pdl_cluster(void (*kern)(KArgs...), int grid, int block, int cluster, size_t smem, cudaStream_t st, Args &&...args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kern, KArgs(std::forward<Args>(args))...);
+}
+
+struct SmallPlan {
+    int ways = 1, cluster = 1, chunks_per_block = 0, stages = 2, grid = 0, smem = 0;
+};
+
+// How the warps share the work: `ways` warps of a block on the same rows, `cluster` blocks on the same tile.  Taken is what gives
+// the busiest block the least work, counted in chunks of a warp; a tile's sum, barrier and store take about as long as
+// kTileCost of them, a cluster's kClusterCost more.
+SmallPlan plan_small(int T, int K, int n_out, int band_rows, int sms, int max_smem)
+{
+    constexpr float kTileCost = 0.4f, kClusterCost = 0.6f;
+    const int chunks = (K + xs::kSwChunk - 1) / xs::kSwChunk;
+    SmallPlan best;
+    float best_cost = 0.0f;
+    for (int c = 1; c <= 8; c *= 2) {
+        SmallPlan p;
+        p.cluster = c;
+        p.chunks_per_block = (chunks + c - 1) / c;
+        if (c > 1 && p.chunks_per_block * (c - 1) >= chunks)
+            break; // a block would have none
+        if (xs::sw_smem_bytes(T, p.chunks_per_block, 2) > max_smem)
+            continue;
+        for (p.stages = xs::kSwMaxStages; xs::sw_smem_bytes(T, p.chunks_per_block, p.stages) > max_smem; p.stages--) {
+        }
+        p.smem = xs::sw_smem_bytes(T, p.chunks_per_block, p.stages);
+        for (p.ways = xs::kSwWarps; p.ways >= 1; p.ways /= 2) {
+            const int tiles = (n_out + xs::kSwWarps / p.ways * band_rows - 1) / (xs::kSwWarps / p.ways * band_rows);
+            const int clusters = tiles < sms / c ? tiles : sms / c, rounds = (tiles + clusters - 1) / clusters;
+            const int per_warp = (p.chunks_per_block + p.ways - 1) / p.ways;
+            const float cost = rounds * (per_warp + kTileCost + (c > 1 ? kClusterCost : 0.0f));
+            if (best.grid == 0 || cost < best_cost) {
+                best = p;
+                best.grid = clusters * c;
+                best_cost = cost;
+            }
+        }
+    }
+    return best;
+}
+
+template <bool GATED, int SUB, bool ZEROS>
+int launch_small_t(const XsMoeW4 *w, const SmallPlan &p, const __nv_bfloat16 *x, int T, __nv_bfloat16 *out, int act, bool early, int32_t *status,
+                   cudaStream_t st)
+{
+    CUtensorMap map;
+    if (int rc = make_tmap_codes(&map, w, GATED ? 2 : 1, GATED ? 16 : 32))
+        return rc;
+    auto kern = xs::w4_small_kernel<GATED, SUB, ZEROS>;
+    XS_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
+    XS_CUDA(launch_pdl_cluster(kern, p.grid, 32 * xs::kSwWarps, p.cluster, p.smem, st, map, matrix_of(w), x, out, GATED ? w->rows / 2 : w->rows, T,
+                               w->cols, act, early ? 1 : 0, p.ways, p.cluster, p.chunks_per_block, p.stages, status));
     note_launch();
     return 0;
 }
 
-template <int SUB, bool ZEROS>
-int launch_small(const xs::W4Matrix &w, bool gated, const __nv_bfloat16 *x, int T, __nv_bfloat16 *out, int n_out, int K, int act, bool early,
-                 int sms, cudaStream_t st)
+template <int SUB>
+int launch_small(const XsMoeW4 *w, bool gated, const __nv_bfloat16 *x, int T, __nv_bfloat16 *out, int act, bool early, const DeviceInfo &di,
+                 int32_t *status, cudaStream_t st)
 {
-    if (gated)
-        return launch_small_t<2, true, SUB, ZEROS>(w, x, T, out, n_out, K, act, early, sms, st);
-    if (n_out >= 32 * 2 * sms)
-        return launch_small_t<2, false, SUB, ZEROS>(w, x, T, out, n_out, K, act, early, sms, st);
-    return launch_small_t<1, false, SUB, ZEROS>(w, x, T, out, n_out, K, act, early, sms, st);
+    const SmallPlan p = plan_small(T, w->cols, gated ? w->rows / 2 : w->rows, gated ? 16 : 32, di.sms, di.max_smem);
+    if (w->zeros_dev)
+        return gated ? launch_small_t<true, SUB, true>(w, p, x, T, out, act, early, status, st)
+                     : launch_small_t<false, SUB, true>(w, p, x, T, out, act, early, status, st);
+    return gated ? launch_small_t<true, SUB, false>(w, p, x, T, out, act, early, status, st)
+                 : launch_small_t<false, SUB, false>(w, p, x, T, out, act, early, status, st);
 }
 
 // early: nothing that may still be running when the kernel starts writes the weights (the second product of one call)
-int launch_w4(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void *out, bool early, cudaStream_t st)
+int launch_w4(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void *out, bool early, int32_t *status, cudaStream_t st)
 {
     DeviceInfo di;
     if (int rc = device_info(&di))
@@ -154,18 +233,14 @@ int launch_w4(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void 
     const int n_out = gated ? w->rows / 2 : w->rows, K = w->cols;
     const __nv_bfloat16 *xb = static_cast<const __nv_bfloat16 *>(x);
     __nv_bfloat16 *ob = static_cast<__nv_bfloat16 *>(out);
-    const xs::W4Matrix m = matrix_of(w);
-    if (T <= xs::kSwTokens) {
-        const bool z = w->zeros_dev != nullptr;
+    if (T <= xs::kSwTokens && xs::sw_smem_bytes(T, ((K + xs::kSwChunk - 1) / xs::kSwChunk + 7) / 8, 2) <= di.max_smem) {
         if (w->group == 32)
-            return z ? launch_small<1, true>(m, gated, xb, T, ob, n_out, K, act, early, di.sms, st)
-                     : launch_small<1, false>(m, gated, xb, T, ob, n_out, K, act, early, di.sms, st);
+            return launch_small<1>(w, gated, xb, T, ob, act, early, di, status, st);
         if (w->group == 64)
-            return z ? launch_small<2, true>(m, gated, xb, T, ob, n_out, K, act, early, di.sms, st)
-                     : launch_small<2, false>(m, gated, xb, T, ob, n_out, K, act, early, di.sms, st);
-        return z ? launch_small<4, true>(m, gated, xb, T, ob, n_out, K, act, early, di.sms, st)
-                 : launch_small<4, false>(m, gated, xb, T, ob, n_out, K, act, early, di.sms, st);
+            return launch_small<2>(w, gated, xb, T, ob, act, early, di, status, st);
+        return launch_small<4>(w, gated, xb, T, ob, act, early, di, status, st);
     }
+    const xs::W4Matrix m = matrix_of(w);
     const dim3 grid((n_out + 7) / 8, (T + 7) / 8);
     if (gated)
         XS_CUDA(launch_pdl(xs::w4_rows_kernel<true>, grid, 256, 0, st, m, xb, ob, n_out, T, K, w->group, act));
@@ -333,11 +408,11 @@ XsMoeNormResidual block_tail(const XsMoeBlockNorms *n, const void *y, const void
     return a;
 }
 
-int run_mlp(const XsMoeW4 *gu, const XsMoeW4 *dn, int32_t act, const void *x, int32_t tokens, void *out, uint8_t *scratch, cudaStream_t st)
+int run_mlp(const XsMoeW4 *gu, const XsMoeW4 *dn, int32_t act, const void *x, int32_t tokens, void *out, uint8_t *scratch, int32_t *status, cudaStream_t st)
 {
-    if (int rc = launch_w4(gu, true, act, x, tokens, scratch, false, st))
+    if (int rc = launch_w4(gu, true, act, x, tokens, scratch, false, status, st))
         return rc;
-    return launch_w4(dn, false, 0, scratch, tokens, out, true, st);
+    return launch_w4(dn, false, 0, scratch, tokens, out, true, status, st);
 }
 
 // the fail() string may allocate: an exception of the host library becomes a status like every other failure
@@ -383,7 +458,7 @@ int xs_moe_linear_w4(const XsMoeW4 *w, const void *x, int32_t tokens, void *out,
             return rc;
         if (int rc = check_io(x, static_cast<size_t>(tokens) * w->cols, out, static_cast<size_t>(tokens) * w->rows, ws, kStatusBytes, dev))
             return rc;
-        return launch_w4(w, false, 0, x, tokens, out, false, static_cast<cudaStream_t>(stream));
+        return launch_w4(w, false, 0, x, tokens, out, false, static_cast<int32_t *>(ws), static_cast<cudaStream_t>(stream));
     });
 }
 
@@ -403,7 +478,7 @@ int xs_moe_gated_w4(const XsMoeW4 *gate_up, int32_t activation, const void *x, i
             return rc;
         if (int rc = check_io(x, static_cast<size_t>(tokens) * gate_up->cols, h, static_cast<size_t>(tokens) * (gate_up->rows / 2), ws, kStatusBytes, dev))
             return rc;
-        return launch_w4(gate_up, true, activation, x, tokens, h, false, static_cast<cudaStream_t>(stream));
+        return launch_w4(gate_up, true, activation, x, tokens, h, false, static_cast<int32_t *>(ws), static_cast<cudaStream_t>(stream));
     });
 }
 
@@ -440,7 +515,8 @@ int xs_moe_mlp_w4(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t activatio
         const size_t n = static_cast<size_t>(tokens) * gate_up->cols;
         if (int rc = check_io(x, n, out, n, ws, need, dev))
             return rc;
-        return run_mlp(gate_up, down, activation, x, tokens, out, static_cast<uint8_t *>(ws) + kStatusBytes, static_cast<cudaStream_t>(stream));
+        return run_mlp(gate_up, down, activation, x, tokens, out, static_cast<uint8_t *>(ws) + kStatusBytes, static_cast<int32_t *>(ws),
+                       static_cast<cudaStream_t>(stream));
     });
 }
 
@@ -493,7 +569,7 @@ int xs_moe_mlp_w4_block(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t act
         const XsMoeNormResidual pre = pre_norm(norms, x, xn, tokens, H), tail = block_tail(norms, y, x, out, tokens, H);
         if (int rc = run_norm(&pre, st))
             return rc;
-        if (int rc = run_mlp(gate_up, down, activation, xn, tokens, y, h, st))
+        if (int rc = run_mlp(gate_up, down, activation, xn, tokens, y, h, static_cast<int32_t *>(ws), st))
             return rc;
         return run_norm(&tail, st);
     });

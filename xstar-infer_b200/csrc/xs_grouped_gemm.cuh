@@ -24,7 +24,6 @@ constexpr int kBlockK = 64;    // bf16 elements per 128-byte swizzled row
 constexpr int kUmmaK = 16;     // K of one tcgen05.mma kind::f16
 
 // status bits written by kernels (also used by the other kernels of the library)
-constexpr int kStatusWaitTimeout = 1;
 constexpr int kStatusBadIndex = 2;
 
 // overflow-stable SiLU, the reference's form (xstar_cpp/src/ops/mlp.cpp:10-26): never exponentiates a positive argument

@@ -45,6 +45,8 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity)
     return ok != 0;
 }
 
+constexpr int kStatusWaitTimeout = 1; // bit of a workspace's status word
+
 // Bounded wait.  Polls fast first, then backs off with nanosleep.  `abort_flag` (shared memory) lets one
 // role that gave up release all the others.  Returns false on time-out or abort.
 constexpr uint32_t kFastPolls = 2048;

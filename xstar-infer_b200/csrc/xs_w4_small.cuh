@@ -1,19 +1,19 @@
 // Products with 4-bit weights for up to eight tokens: out[t][n] = sum_k (q[n][k] - z[n][k/G]) * s[n][k/G] * x[t][k].
 //
-// The weights are read once and nothing else is large, so the kernel is a stream: every warp owns a ring of 256-column chunks of
-// 16 weight rows (32 for MT = 2), with the tokens' 256 columns beside them, that cp.async fills ahead across row tiles; scales
-// are loaded one chunk ahead into registers, since they come from memory as well.  No block-wide barrier stands between a
-// load and its use.  The eight warps of a block take alternate chunks of the same rows (the split over K) and meet once per
-// row tile, in shared memory, in a fixed order.
+// The weights are read once and nothing else is large, so the kernel is a stream.  A warp works on 32 weight rows in chunks of
+// 256 columns, and owns a ring of such chunks (32 rows x 128 bytes) that TMA fills ahead, across tiles.  Scales come from memory as
+// well and are loaded two chunks ahead into registers.  The tokens' columns are laid out once in shared memory.  Of a block's
+// sixteen warps, `ways` share the same rows and take alternate chunks of them; they meet once per tile, in shared memory, in a
+// fixed order, and no other block-wide barrier stands between a load and its use.  Where the tokens' columns would not fit, or
+// where there are too few tiles for the SMs, a cluster of 2, 4 or 8 blocks shares a tile, each with a slice of K, and sums
+// through distributed shared memory.  The host picks ways and cluster (plan_small).
 //
-// The arithmetic must stay below the rate that the stream allows: at 6.5 TB/s an SM receives 46 weights a cycle, while its
-// integer pipe does 64 lanes and its schedulers issue 128.  So the products go to mma.m16n8k16 with the weights as the 16 rows
-// and the tokens as the 8 columns, and a weight costs less than one integer instruction: four nibbles of two columns are cut
-// out with one AND-OR that plants the exponent of 128 (0x4300 | q is 128 + q in bf16), and subtracting 128 + z, exact in
-// bf16, leaves q - z.  The order of k inside an MMA is free as long as both operands agree: a lane's 32-bit word holds columns
-// 8t .. 8t+7, which come out as the pairs (0,4) (1,5) (2,6) (3,7), and x is paired the same way.  ldmatrix hands word t of
-// row g to lane (g, t), which is the fragment layout.  The MMA sums q - z times x in f32; the scale multiplies the f32 sum
-// of a group, so the weights are never rounded.
+// The arithmetic must stay below the rate that the stream allows: at 6.5 TB/s an SM receives 46 weights a cycle, and its
+// schedulers issue 128 lanes a cycle.  So the products go to mma.m16n8k16 with the weights as the 16 rows and the tokens as the 8
+// columns, and eight codes become (q - z) / 64 with nine instructions (w4_unpack).  The order of k inside an MMA is free as
+// long as both operands agree: a lane's 32-bit word holds columns 8t .. 8t+7, which come out as the pairs (0,4) (1,5) (2,6)
+// (3,7), and x is laid out in the same pairs.  ldmatrix hands word t of row g to lane (g, t), which is the fragment layout.  The
+// MMA sums (q - z) x in f32; the scale multiplies the f32 sum of a group, so the weights are never rounded.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -25,28 +25,37 @@
 namespace xs {
 
 constexpr int kSwTokens = 8;
-constexpr int kSwWarps = 8;
-constexpr int kSwChunk = 256; // columns of one stage: 128 bytes a row
+constexpr int kSwWarps = 16;
+constexpr int kSwChunk = 256;               // columns of one stage: 128 bytes a row
+constexpr int kSwStageBytes = 32 * 128;     // 32 rows
+constexpr int kSwPartStride = 33;           // floats between tokens in the partial sums of a warp
+constexpr int kSwMaxStages = 4;
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool in_range)
+__host__ __device__ constexpr int sw_x_bytes(int T, int chunks_per_block)
 {
-    // out of range: nothing is read, the 16 bytes become zero
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in_range ? 16 : 0) : "memory");
+    return T * chunks_per_block * kSwChunk * 2;
 }
-__device__ __forceinline__ void cp_async_commit()
+__host__ __device__ constexpr int sw_part_bytes(int T)
 {
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    return 2 * kSwWarps * T * kSwPartStride * 4;
 }
-template <int N>
-__device__ __forceinline__ void cp_async_wait()
+__host__ __device__ constexpr int sw_smem_bytes(int T, int chunks_per_block, int stages)
 {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+    return 1024 + kSwWarps * stages * (kSwStageBytes + 8) + sw_x_bytes(T, chunks_per_block) + sw_part_bytes(T) + 16;
+}
+
+// the same onto zero
+__device__ __forceinline__ void mma_16816_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // Four 8 x 8 matrices of 16-bit elements: lane (g, t) receives the 32-bit word t of row g of each.  Lane l gives the address of row l % 8 of
 // matrix l / 8.
@@ -54,7 +63,8 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr)
 {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr));
+                 : "r"(addr)
+                 : "memory");
 }
 __device__ __forceinline__ uint4 lds128(uint32_t a)
 {
@@ -62,198 +72,203 @@ __device__ __forceinline__ uint4 lds128(uint32_t a)
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
     return v;
 }
+// 3-D tiled load: c0 and c1 as in tma_load_2d, c2 the outermost coordinate.
+__device__ __forceinline__ void tma_load_3d(void *smem_dst, const CUtensorMap *m, uint64_t *bar, int32_t c0, int32_t c1, int32_t c2, uint64_t policy)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%3, %4, %5}], [%2], %6;"
+        :
+        : "r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "l"(policy)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_barrier()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr, uint32_t rank)
+{
+    float v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}" : "=f"(v) : "r"(addr), "r"(rank) : "memory");
+    return v;
+}
 
-// chunks of a warp's ring, one in use and the others on their way: 48 to 64 KB of weights in flight an SM
-__host__ __device__ constexpr int sw_stages(int mt)
+// GATED: a warp's 32 rows are the 16 gate rows and the 16 up rows of 16 features.  SUB: 32-column steps in a scale group.
+// early: the weights were complete before the predecessor began.  Cluster size C, chunks_per_block: K in slices.
+template <bool GATED, int SUB, bool ZEROS>
+__global__ void __launch_bounds__(32 * kSwWarps, 1)
+w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, const __nv_bfloat16 *x, __nv_bfloat16 *out, int n_out, int T, int K,
+                int act, int early, int ways, int C, int chunks_per_block, int stages, int32_t *status)
 {
-    return mt == 1 ? 4 : 3;
-}
-__host__ __device__ constexpr int sw_stage_bytes(int mt, int T)
-{
-    return mt * 16 * (kSwChunk / 2) + T * kSwChunk * 2;
-}
-__host__ __device__ constexpr int sw_part_stride(int mt)
-{
-    return mt * 16 + 4; // tokens apart in the partial sums; + 4: the fragments' stores meet no bank twice
-}
-__host__ __device__ constexpr int sw_smem_bytes(int mt, int T)
-{
-    return kSwWarps * (sw_stages(mt) * sw_stage_bytes(mt, T) + 2 * T * sw_part_stride(mt) * 4);
-}
-
-// MT: 16-row groups of a tile; GATED: MT = 2, the 16 gate rows and the 16 up rows of one feature block.  SUB: 32-column steps
-// in a scale group.  early: the weights were complete before the predecessor began.
-template <int MT, bool GATED, int SUB, bool ZEROS>
-__global__ void __launch_bounds__(32 * kSwWarps)
-w4_small_kernel(const W4Matrix w, const __nv_bfloat16 *x, __nv_bfloat16 *out, int n_out, int T, int K, int act, int early)
-{
-    static_assert(!GATED || MT == 2, "a gated tile is one gate group and one up group");
     constexpr int G = 32 * SUB, GROUPS = kSwChunk / G, SLOTS = (GROUPS + 3) / 4; // scale slots a lane holds per row and chunk
-    constexpr int FEATURES = GATED ? 16 : 16 * MT;
-    constexpr int STAGES = sw_stages(MT);
-    constexpr int W_BYTES = MT * 16 * (kSwChunk / 2);
+    constexpr int ROWS = GATED ? 16 : 32; // features a warp works on
 
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int stage_bytes = sw_stage_bytes(MT, T);
-    const uint32_t ring = smem_u32(smem) + warp * STAGES * stage_bytes;
-    float *part = reinterpret_cast<float *>(smem + kSwWarps * STAGES * stage_bytes);
-    const int groups = K / G, part_floats = T * sw_part_stride(MT);
-    const int tiles = (n_out + FEATURES - 1) / FEATURES, chunks = (K + kSwChunk - 1) / kSwChunk;
-    const int row_bytes = K / 2;
-    const size_t half_rows = GATED ? static_cast<size_t>(n_out) - 16 : 0; // rows 16.. of a gated tile lie n_out below the first
+    const int bands = kSwWarps / ways, band = warp % bands, way = warp / bands; // 32-row bands of a tile
+    const int features = bands * ROWS;
+    uint8_t *x_smem = smem + kSwWarps * stages * kSwStageBytes;
+    float *part = reinterpret_cast<float *>(x_smem + sw_x_bytes(T, chunks_per_block));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(reinterpret_cast<uint8_t *>(part) + (sw_part_bytes(T) + 7) / 8 * 8);
+    volatile uint32_t *abort_flag = reinterpret_cast<uint32_t *>(bars + kSwWarps * stages);
+    const uint32_t ring = smem_u32(smem) + warp * stages * kSwStageBytes;
+    uint64_t *full = bars + warp * stages;
 
-    // Everything past the end of K or of the rows reads as zero: codes, x and scales, so that it adds 0 * 0 * 0.
-    // The load side of codes and x: one chunk of one tile.
-    struct {
+    const int groups = K / G, part_floats = T * kSwPartStride;
+    const int tiles = (n_out + features - 1) / features, all_chunks = (K + kSwChunk - 1) / kSwChunk;
+    const int rank = C > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int chunk0 = rank * chunks_per_block, chunk_end = min(chunk0 + chunks_per_block, all_chunks);
+    const int first = chunk0 + way; // this warp's chunks: first, first + ways, ... below chunk_end
+    const int tile0 = blockIdx.x / C, tile_step = gridDim.x / C;
+
+    if (lane == 0) {
+        for (int i = 0; i < stages; i++)
+            mbar_init(&full[i], 1);
+        if (warp == 0) {
+            *abort_flag = 0;
+            prefetch_tmap(&tmap);
+        }
+        fence_mbar_init();
+    }
+    __syncwarp();
+
+    // Everything past the end of K or of the rows counts as zero: codes that TMA did not find, x and scales.
+    struct Place { // one chunk of one tile
         int tile, chunk;
-        const uint8_t *w; // this lane's piece of row lane / 8
-    } ld{};
-    auto ld_start = [&](int tile) {
-        ld.tile = tile;
-        ld.chunk = warp;
-        ld.w = w.codes + (static_cast<size_t>(tile) * FEATURES + (lane >> 3)) * row_bytes + warp * (kSwChunk / 2) + (lane & 7) * 16;
     };
-    auto ld_next = [&]() {
-        ld.chunk += kSwWarps;
-        ld.w += kSwWarps * (kSwChunk / 2);
-        if (ld.chunk >= chunks)
-            ld_start(ld.tile + gridDim.x);
-    };
-    const int lane_dst = (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4), lane_dst4 = lane_dst ^ 64; // rows 4 .. 7 of every 8
-    auto fetch_w = [&](int stage) {
-        if (ld.tile < tiles) {
-            const uint32_t dst = ring + stage * stage_bytes;
-            const bool in = ld.chunk * (kSwChunk / 2) + (lane & 7) * 16 < row_bytes;
-            const int rows = n_out - ld.tile * FEATURES - (lane >> 3); // rows from this lane's first to the end
-            const uint8_t *src = ld.w;
-#pragma unroll
-            for (int i = 0; i < 4 * MT; i++) {
-                if (GATED && i == 4)
-                    src += half_rows * row_bytes;
-                const bool ok = in && (GATED ? i % 4 : i) * 4 < rows;
-                cp_async16(dst + (i / 2) * 1024 + (i % 2 ? 512 + lane_dst4 : lane_dst), ok ? src : w.codes, ok);
-                src += 4 * static_cast<size_t>(row_bytes);
-            }
+    auto advance = [&](Place &p) {
+        p.chunk += ways;
+        if (p.chunk >= chunk_end) {
+            p.chunk = first;
+            p.tile += tile_step;
         }
     };
-    // 16-byte piece c of a token's 512: at c, or c ^ 4 for odd tokens, so that the eight lanes of a quarter read meet no bank twice
-    auto fetch_x = [&](int stage) {
-        if (ld.tile < tiles) {
-            uint32_t dst = ring + stage * stage_bytes + W_BYTES + (lane << 4);
-            const int k = ld.chunk * kSwChunk + lane * 8;
-            const bool in = k < K;
-            const __nv_bfloat16 *src = x + (in ? k : 0);
-            const int odd = lane & 4 ? -64 : 64;
-            for (int n = 0; n < T; n++) {
-                cp_async16(dst + (n & 1 ? odd : 0), src, in);
-                dst += kSwChunk * 2;
-                src += K;
-            }
+    const Place begin{first < chunk_end ? tile0 : tiles, first};
+    Place ld = begin, ls = begin;
+    const uint64_t policy = policy_evict_first(); // every weight is read once
+    auto fetch = [&](int stage) {
+        if (lane == 0 && ld.tile < tiles) {
+            mbar_arrive_expect_tx(&full[stage], kSwStageBytes);
+            tma_load_3d(smem + (warp * stages + stage) * kSwStageBytes, &tmap, &full[stage], ld.chunk * (kSwChunk / 2), ld.tile * features + band * ROWS, 0, policy);
         }
-        cp_async_commit(); // a group for every call, so that counting groups counts chunks
+        advance(ld);
     };
-    // scale (bits 16..31) and zero point (bits 0..3) of a chunk: lane t of a quad holds groups t and t + 4 of rows g and g + 8
-    struct {
-        int tile, chunk;
-    } ls{};
-    auto load_scales = [&](uint32_t (&v)[MT][2][SLOTS]) {
-        const int gi = ls.chunk * GROUPS + t % GROUPS, rows = ls.tile < tiles ? n_out - ls.tile * FEATURES - g : 0;
-        const size_t o = (static_cast<size_t>(ls.tile) * FEATURES + g) * groups + gi;
+    // scale (bits 16..31) and zero point (bits 0..3) of a chunk: lane t of a quad holds groups t and t + 4 of rows g + 8 h of the
+    // band, h = 0 .. 3 (GATED: h = 2, 3 are the up rows)
+    const size_t up_groups = static_cast<size_t>(n_out) * groups;
+    auto load_scales = [&](uint32_t (&v)[4][SLOTS]) {
+        const int gi = ls.chunk * GROUPS + t % GROUPS, row = ls.tile * features + band * ROWS + g;
+        const size_t o = static_cast<size_t>(row) * groups + gi;
+        const uint16_t *sp = reinterpret_cast<const uint16_t *>(w.scales) + o;
+        const uint8_t *zp = ZEROS ? w.zeros + o : nullptr;
+        const int rows = ls.tile < tiles ? n_out - row : 0;
+        const bool whole = rows > ROWS - 8 && gi + (SLOTS - 1) * 4 < groups; // every one of them is there
 #pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const size_t oh = o + (GATED && m ? half_rows * groups : 0) + static_cast<size_t>((m * 2 + h) * 8 * groups);
-#pragma unroll
-                for (int j = 0; j < SLOTS; j++) {
-                    v[m][h][j] = 0u;
-                    if (((GATED ? 0 : m * 2) + h) * 8 < rows && gi + j * 4 < groups)
-                        v[m][h][j] = static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(w.scales)[oh + j * 4]) << 16 |
-                                     (ZEROS ? w.zeros[oh + j * 4] & 15u : 0u);
-                }
+        for (int h = 0; h < 4; h++) {
+            if (h > 0) {
+                const size_t step = GATED && h == 2 ? up_groups - 8 * groups : static_cast<size_t>(8) * groups;
+                sp += step;
+                if (ZEROS)
+                    zp += step;
             }
-        ls.chunk += kSwWarps;
-        if (ls.chunk >= chunks) {
-            ls.chunk = warp;
-            ls.tile += gridDim.x;
+#pragma unroll
+            for (int j = 0; j < SLOTS; j++) {
+                v[h][j] = 0u;
+                if (whole || ((GATED ? h % 2 : h) * 8 < rows && gi + j * 4 < groups))
+                    v[h][j] = static_cast<uint32_t>(sp[j * 4]) << 16 | (ZEROS ? zp[j * 4] & 15u : 0u);
+            }
         }
+        advance(ls);
     };
 
-    // a warp without chunks of its own (K <= 256 warp) only joins the sums
-    const int first_tile = warp < chunks ? static_cast<int>(blockIdx.x) : tiles;
     if (!early)
         pdl_wait();
-    uint32_t sc[MT][2][SLOTS], sc_next[MT][2][SLOTS];
-    ld_start(first_tile);
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; i++, ld_next())
-        fetch_w(i);
-    ls.tile = first_tile;
-    ls.chunk = warp;
+    for (int i = 0; i < stages - 1; i++)
+        fetch(i);
+    uint32_t sc[4][SLOTS], sc_next[4][SLOTS];
     load_scales(sc);
     load_scales(sc_next);
     if (early)
         pdl_wait();
-    ld_start(first_tile);
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; i++, ld_next())
-        fetch_x(i);
     pdl_launch_dependents(); // after the wait: what the next kernel may load early was complete before this one began
+    // x as the MMA's second operand: [32-column step][token][t] pieces of 16 bytes, the pairs (0,4) (1,5) (2,6) (3,7) of columns 8t ..
+    {
+        const int pieces = (chunk_end - chunk0) * (kSwChunk / 8);
+        for (int p = threadIdx.x; p < pieces; p += 32 * kSwWarps) {
+            const int k = chunk0 * kSwChunk + p * 8;
+            uint4 v[kSwTokens];
+#pragma unroll
+            for (int n = 0; n < kSwTokens; n++) {
+                v[n] = make_uint4(0, 0, 0, 0);
+                if (n < T && k < K)
+                    v[n] = *reinterpret_cast<const uint4 *>(x + static_cast<size_t>(n) * K + k);
+            }
+#pragma unroll
+            for (int n = 0; n < kSwTokens; n++)
+                if (n < T)
+                    *reinterpret_cast<uint4 *>(x_smem + (((p >> 2) * T + n) * 4 + (p & 3)) * 16) =
+                        make_uint4(__byte_perm(v[n].x, v[n].z, 0x5410), __byte_perm(v[n].x, v[n].z, 0x7632), __byte_perm(v[n].y, v[n].w, 0x5410),
+                                   __byte_perm(v[n].y, v[n].w, 0x7632));
+        }
+    }
+    __syncthreads();
 
-    // lane l addresses row l % 8 of matrix l / 8: rows 0..7 and 8..15 of two groups (MT = 2), or of two 32-column steps (MT = 1)
-    const int mat = lane >> 3, mrow = lane & 7;
-    const uint32_t frag = ((MT == 2 ? mat : mat & 1) * 8 + mrow) * 128;
+    // lane l addresses row l % 8 of matrix l / 8; TMA swizzles the 16-byte pieces of a row with the row, and a stage begins at a
+    // multiple of 1024, so piece j is one XOR away
+    const uint32_t frag = lane * 128 + ((lane & 7) << 4);
     // lanes of tokens that are not there read the last one: a column of its own, which is not stored
-    const int xg = g < T ? g : T - 1;
-    const uint32_t x_even = W_BYTES + xg * (kSwChunk * 2) + (t << 4) + ((xg & 1) << 6), x_odd = x_even + 64 - ((xg & 1) << 7);
+    const uint32_t x_lane = smem_u32(x_smem) + ((g < T ? g : T - 1) * 4 + t) * 16;
+    const int x_step = T * 64;
+    const int share = features / C, share_log = 31 - __clz(share); // features of a tile that this block finishes: a power of two
     int stage = 0, parity = 0;
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, parity ^= 1) {
-        float acc[MT][4] = {};
-        for (int chunk = warp; chunk < chunks; chunk += kSwWarps) {
-            const int fill = stage == 0 ? STAGES - 1 : stage - 1;
-            fetch_w(fill);
-            fetch_x(fill);
-            ld_next();
-            uint32_t sc_after[MT][2][SLOTS];
+    uint32_t phase = 0;
+    for (int tile = tile0; tile < tiles; tile += tile_step, parity ^= 1) {
+        float acc[2][4] = {};
+        for (int chunk = first; chunk < chunk_end; chunk += ways) {
+            fetch(stage == 0 ? stages - 1 : stage - 1);
+            uint32_t sc_after[4][SLOTS];
             load_scales(sc_after);
-            cp_async_wait<STAGES - 1>();
+            if (!mbar_wait(&full[stage], phase, abort_flag)) {
+                *abort_flag = 1;
+                atomicOr(status, kStatusWaitTimeout);
+            }
             __syncwarp();
-            const uint32_t st = ring + stage * stage_bytes;
-            float c[MT][4];
-            uint32_t qq[4];
-            float s[MT][2];
-            uint32_t z[MT][2];
+            const uint32_t st = ring + stage * kSwStageBytes + frag;
+            uint32_t xa = x_lane + (chunk - chunk0) * (kSwChunk / 32) * x_step;
+            float c[2][4], s[2][2];
+            uint32_t z[2][2];
 #pragma unroll
             for (int j = 0; j < kSwChunk / 32; j++) {
-                const uint4 xv = lds128(st + (j % 2 ? x_odd : x_even) + (j / 2) * 128);
-                const uint32_t b[4] = {__byte_perm(xv.x, xv.z, 0x5410), __byte_perm(xv.x, xv.z, 0x7632), __byte_perm(xv.y, xv.w, 0x5410),
-                                       __byte_perm(xv.y, xv.w, 0x7632)};
-                if (MT == 2)
-                    ldmatrix_x4(qq, st + frag + ((j ^ mrow) << 4));
-                else if (j % 2 == 0)
-                    ldmatrix_x4(qq, st + frag + (((j + (mat >> 1)) ^ mrow) << 4));
+                const uint4 b = lds128(xa);
+                xa += x_step;
+                uint32_t q[4];
+                ldmatrix_x4(q, st ^ (j << 4));
 #pragma unroll
-                for (int m = 0; m < MT; m++) {
+                for (int m = 0; m < 2; m++) {
                     if (j % SUB == 0) {
-                        c[m][0] = c[m][1] = c[m][2] = c[m][3] = 0.0f;
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            const uint32_t v = __shfl_sync(0xffffffffu, sc[m][h][(j / SUB) / 4], (lane & ~3) | ((j / SUB) & 3));
+                            const uint32_t v = __shfl_sync(0xffffffffu, sc[m * 2 + h][(j / SUB) / 4], (lane & ~3) | ((j / SUB) & 3));
                             s[m][h] = __uint_as_float(ZEROS ? v & 0xffff0000u : v);
-                            z[m][h] = ZEROS ? (v & 15u) * 0x00010001u + 0x43004300u : 0x43084308u;
+                            z[m][h] = ZEROS ? w4_minus_zero(v & 15u) : kW4Minus8;
                         }
                     }
                     uint32_t a[2][4];
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint32_t q = qq[(MT == 2 ? m * 2 : (j % 2) * 2) + h];
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            a[h][i] = w4_minus(w4_magic(q >> (4 * i)), z[m][h]);
-                    }
-                    mma_16816(c[m], a[0][0], a[1][0], a[0][1], a[1][1], b[0], b[1]);
-                    mma_16816(c[m], a[0][2], a[1][2], a[0][3], a[1][3], b[2], b[3]);
+                    for (int h = 0; h < 2; h++)
+                        w4_unpack(a[h], q[m * 2 + h], z[m][h]);
+                    if (j % SUB == 0)
+                        mma_16816_first(c[m], a[0][0], a[1][0], a[0][1], a[1][1], b.x, b.y);
+                    else
+                        mma_16816(c[m], a[0][0], a[1][0], a[0][1], a[1][1], b.x, b.y);
+                    mma_16816(c[m], a[0][2], a[1][2], a[0][3], a[1][3], b.z, b.w);
                     if (j % SUB == SUB - 1) {
                         acc[m][0] = fmaf(s[m][0], c[m][0], acc[m][0]);
                         acc[m][1] = fmaf(s[m][0], c[m][1], acc[m][1]);
@@ -263,40 +278,50 @@ w4_small_kernel(const W4Matrix w, const __nv_bfloat16 *x, __nv_bfloat16 *out, in
                 }
             }
 #pragma unroll
-            for (int m = 0; m < MT; m++)
+            for (int h = 0; h < 4; h++)
 #pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int j = 0; j < SLOTS; j++) {
-                        sc[m][h][j] = sc_next[m][h][j];
-                        sc_next[m][h][j] = sc_after[m][h][j];
-                    }
+                for (int j = 0; j < SLOTS; j++) {
+                    sc[h][j] = sc_next[h][j];
+                    sc_next[h][j] = sc_after[h][j];
+                }
             __syncwarp(); // every lane has read the stage before the next fetch may fill it again
-            stage = stage + 1 == STAGES ? 0 : stage + 1;
+            if (++stage == stages) {
+                stage = 0;
+                phase ^= 1;
+            }
         }
         float *mine = part + (parity * kSwWarps + warp) * part_floats;
 #pragma unroll
-        for (int m = 0; m < MT; m++)
+        for (int m = 0; m < 2; m++)
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 if (2 * t + (e & 1) < T)
-                    mine[(2 * t + (e & 1)) * sw_part_stride(MT) + m * 16 + (e >> 1) * 8 + g] = acc[m][e];
-        __syncthreads(); // one barrier a tile: the next tile's sums go to the other half of `part`
-        for (int i = threadIdx.x; i < FEATURES * T; i += 32 * kSwWarps) {
-            const int token = i / FEATURES, f = i - token * FEATURES, feature = tile * FEATURES + f;
-            const float *p = part + parity * kSwWarps * part_floats + token * sw_part_stride(MT) + f;
+                    mine[(2 * t + (e & 1)) * kSwPartStride + m * 16 + (e >> 1) * 8 + g] = acc[m][e];
+        // one barrier a tile: the next tile's sums go to the other half of `part`
+        if (C > 1)
+            cluster_barrier();
+        else
+            __syncthreads();
+        for (int i = threadIdx.x; i < share * T; i += 32 * kSwWarps) {
+            const int token = i >> share_log, f = rank * share + (i & (share - 1)), feature = tile * features + f;
+            const float *p = part + (parity * kSwWarps + f / ROWS) * part_floats + token * kSwPartStride + f % ROWS;
             float v = 0.0f, u = 0.0f;
-#pragma unroll
-            for (int k = 0; k < kSwWarps; k++) {
-                v += p[k * part_floats];
-                if (GATED)
-                    u += p[k * part_floats + 16];
-            }
+            for (int r = 0; r < C; r++)
+                for (int k = 0; k < ways; k++) {
+                    const float *pk = p + k * bands * part_floats;
+                    v += C > 1 ? ld_cluster_f32(smem_u32(pk), r) : *pk;
+                    if (GATED)
+                        u += C > 1 ? ld_cluster_f32(smem_u32(pk + 16), r) : pk[16];
+                }
             if (feature < n_out)
-                out[static_cast<size_t>(token) * n_out + feature] = __float2bfloat16_rn(GATED ? w4_activation(v, act) * u : v);
+                out[static_cast<size_t>(token) * n_out + feature] = __float2bfloat16_rn(GATED ? w4_activation(kW4Unit * v, act) * (kW4Unit * u) : kW4Unit * v);
         }
     }
-    cp_async_wait<0>();
+    if (C > 1)
+        cluster_barrier(); // nobody leaves while its sums may still be read
+    if (*abort_flag)
+        for (int i = 0; i < 64; i++)
+            __nanosleep(4096);
 }
 
 } // namespace xs
