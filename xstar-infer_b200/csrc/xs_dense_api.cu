@@ -3,8 +3,8 @@
 
 #include "xs_api_common.cuh"
 #include "xs_norm_residual.cuh"
-#include "xs_w4_rows.cuh"
 #include "xs_w4_small.cuh"
+#include "xs_w4_tc.cuh"
 
 using namespace xs_api;
 
@@ -224,13 +224,97 @@ int launch_small(const XsMoeW4 *w, bool gated, const __nv_bfloat16 *x, int T, __
                  : launch_small_t<false, SUB, false>(w, p, x, T, out, act, early, status, st);
 }
 
+// A batch of bf16 rows read in boxes of 64 columns x box_rows, 128-byte swizzle; past the end of rows and columns there are zeros.
+int make_tmap_rows(CUtensorMap *m, const void *x, int T, int K, uint32_t box_rows)
+{
+    EncodeTiledFn fn = get_encode_fn();
+    if (!fn)
+        return fail(XS_MOE_ERR_CUDA, "CUDA error: cuTensorMapEncodeTiled entry point not available");
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(T)}, strides[1] = {static_cast<cuuint64_t>(K) * 2};
+    const cuuint32_t box[2] = {64, box_rows}, one[2] = {1, 1};
+    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(x), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(XS_MOE_ERR_CUDA, "CUDA error: cuTensorMapEncodeTiled failed with code %d (rows=%d cols=%d)", (int)r, T, K);
+    return 0;
+}
+
+struct TcPlan {
+    int cg = 1, n_tile = 32, grid = 0;
+    xs::TcShape shape{};
+};
+
+// Tile and split by estimated cycles of the busiest block: a 64-column block of a tile takes the larger of the MMAs (2 cycles a
+// token of a 128-row tile) and of the conversion of its codes (180), a tile's start, sum and store a fixed part more.
+TcPlan plan_tc(const XsMoeW4 *w, bool gated, int T, int sms)
+{
+    const int n_out = gated ? w->rows / 2 : w->rows, K = w->cols;
+    const int all_raw = (K + 255) / 256;
+    TcPlan best;
+    float best_cost = 0.0f;
+    for (int cg = 1; cg <= 2; cg++)
+        for (int n_tile = cg == 1 ? 32 : 256; n_tile <= (cg == 1 ? 128 : 256); n_tile *= 2)
+            for (int split = 1; split <= (cg == 1 ? 8 : 1); split *= 2) {
+                const int raw_per = (all_raw + split - 1) / split;
+                if (raw_per * (split - 1) >= all_raw)
+                    break;
+                TcPlan p;
+                p.cg = cg;
+                p.n_tile = n_tile;
+                const int features = (gated ? xs::kTcRows / 2 : xs::kTcRows) * cg;
+                p.shape = {n_out, T, K, w->group == 32 ? 5 : w->group == 64 ? 6 : 7, (n_out + features - 1) / features, (T + n_tile - 1) / n_tile, split};
+                const long items = static_cast<long>(p.shape.w_tiles) * p.shape.t_tiles;
+                const int slots = sms / (cg * split);
+                if (split > 1 && items > slots)
+                    break; // a split block has one tile
+                const long rounds = (items + slots - 1) / slots;
+                p.grid = static_cast<int>(items < slots ? items : slots) * cg * split;
+                const float mma = 2.0f * n_tile, block = mma > 180.0f ? mma : 180.0f;
+                const float cost = rounds * (raw_per * 4 * block + 1500.0f + 8.0f * n_tile + (split > 1 ? 1500.0f : 0.0f));
+                if (best.grid == 0 || cost < best_cost) {
+                    best = p;
+                    best_cost = cost;
+                }
+            }
+    return best;
+}
+
+template <int CG, int N_TILE, bool GATED>
+int launch_tc_t(const XsMoeW4 *w, const TcPlan &p, const __nv_bfloat16 *x, __nv_bfloat16 *out, int act, int32_t *status, cudaStream_t st)
+{
+    auto kern = xs::w4_tc_kernel<CG, N_TILE, GATED>;
+    constexpr int smem = xs::tc_smem_bytes(CG, N_TILE);
+    XS_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    CUtensorMap mw, mx;
+    if (int rc = make_tmap_codes(&mw, w, GATED ? 2 : 1, GATED ? xs::kTcRows / 2 : xs::kTcRows))
+        return rc;
+    if (int rc = make_tmap_rows(&mx, x, p.shape.T, p.shape.K, N_TILE / CG))
+        return rc;
+    XS_CUDA(launch_pdl_cluster(kern, p.grid, xs::kTcThreads, CG * p.shape.split, smem, st, mw, mx, matrix_of(w), out, p.shape, act, status));
+    note_launch();
+    return 0;
+}
+
+template <bool GATED>
+int launch_tc(const XsMoeW4 *w, const __nv_bfloat16 *x, int T, __nv_bfloat16 *out, int act, int sms, int32_t *status, cudaStream_t st)
+{
+    const TcPlan p = plan_tc(w, GATED, T, sms);
+    if (p.cg == 2)
+        return launch_tc_t<2, 256, GATED>(w, p, x, out, act, status, st);
+    if (p.n_tile == 128)
+        return launch_tc_t<1, 128, GATED>(w, p, x, out, act, status, st);
+    if (p.n_tile == 64)
+        return launch_tc_t<1, 64, GATED>(w, p, x, out, act, status, st);
+    return launch_tc_t<1, 32, GATED>(w, p, x, out, act, status, st);
+}
+
 // early: nothing that may still be running when the kernel starts writes the weights (the second product of one call)
 int launch_w4(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void *out, bool early, int32_t *status, cudaStream_t st)
 {
     DeviceInfo di;
     if (int rc = device_info(&di))
         return rc;
-    const int n_out = gated ? w->rows / 2 : w->rows, K = w->cols;
+    const int K = w->cols;
     const __nv_bfloat16 *xb = static_cast<const __nv_bfloat16 *>(x);
     __nv_bfloat16 *ob = static_cast<__nv_bfloat16 *>(out);
     if (T <= xs::kSwTokens && xs::sw_smem_bytes(T, ((K + xs::kSwChunk - 1) / xs::kSwChunk + 7) / 8, 2) <= di.max_smem) {
@@ -240,14 +324,7 @@ int launch_w4(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void 
             return launch_small<2>(w, gated, xb, T, ob, act, early, di, status, st);
         return launch_small<4>(w, gated, xb, T, ob, act, early, di, status, st);
     }
-    const xs::W4Matrix m = matrix_of(w);
-    const dim3 grid((n_out + 7) / 8, (T + 7) / 8);
-    if (gated)
-        XS_CUDA(launch_pdl(xs::w4_rows_kernel<true>, grid, 256, 0, st, m, xb, ob, n_out, T, K, w->group, act));
-    else
-        XS_CUDA(launch_pdl(xs::w4_rows_kernel<false>, grid, 256, 0, st, m, xb, ob, n_out, T, K, w->group, act));
-    note_launch();
-    return 0;
+    return gated ? launch_tc<true>(w, xb, T, ob, act, di.sms, status, st) : launch_tc<false>(w, xb, T, ob, act, di.sms, status, st);
 }
 
 int launch_norm_residual(const xs::NormResidualArgs &a, cudaStream_t st)

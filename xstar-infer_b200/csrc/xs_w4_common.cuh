@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "xs_ptx.cuh"
+
 namespace xs {
 
 struct W4Matrix {
@@ -41,12 +43,46 @@ __device__ __forceinline__ uint32_t w4_minus_zero(uint32_t z)
     return w4_fma(z * 0x00010001u, 0xff00ff00u, 0u); // times -2^127
 }
 
-// silu: v / (1 + exp(-v)); gelu: v / 2 * (1 + tanh(c (v + 0.044715 v^3))).
+// silu: v / (1 + exp(-v)); gelu: v / 2 * (1 + tanh(c (v + 0.044715 v^3))), and (1 + tanh(a)) / 2 = 1 / (1 + exp(-2 a)).  The fast
+// exponential and division are off by a few f32 steps, far below the bf16 step of the result; far below zero both end at 0.
 __device__ __forceinline__ float w4_activation(float v, int act)
 {
-    if (act == 0)
-        return v / (1.0f + expf(-v));
-    return 0.5f * v * (1.0f + tanhf(0.7978845608028654f * (v + 0.044715f * v * v * v)));
+    const float a = act == 0 ? v : 1.5957691216057308f * (v + 0.044715f * v * v * v);
+    const float e = 1.0f + __expf(-a);
+    return e < 1e37f ? __fdividef(v, e) : (v != v ? v : v * 0.0f);
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t a)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+// 3-D tiled load: c0 and c1 as in tma_load_2d, c2 the outermost coordinate.
+__device__ __forceinline__ void tma_load_3d(void *smem_dst, const CUtensorMap *m, uint64_t *bar, int32_t c0, int32_t c1, int32_t c2, uint64_t policy)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%3, %4, %5}], [%2], %6;"
+        :
+        : "r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "l"(policy)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_barrier()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr, uint32_t rank)
+{
+    float v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}" : "=f"(v) : "r"(addr), "r"(rank) : "memory");
+    return v;
 }
 
 } // namespace xs

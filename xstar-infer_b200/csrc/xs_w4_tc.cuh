@@ -1,0 +1,497 @@
+// Products with 4-bit weights on the tensor core, for batches from nine tokens up: out = x W^T (or act(x Wg^T) * (x Wu^T)).
+//
+// tcgen05.mma with the WEIGHTS as its M rows, taken from TMEM, and the tokens as its N columns, taken from shared memory.  The codes
+// arrive by TMA as they lie in memory; eight warps turn them into bf16, thread = weight row, and store them with tcgen05.st
+// straight into TMEM columns, so a dequantised weight never passes through shared memory, whose bandwidth the tokens need.
+// Weights in TMEM also make the group scale a scalar of the thread.  (q - z) / 64 is exact in bf16 (w4 unpacking below); times s it is
+// rounded once, half a bf16 step: the price of the tensor core, whose operands have one type.  Sums are f32 in TMEM.
+//
+// CG = 2 pairs two SMs on a 256 x 256 tile (cta_group::2): each dequantises its 128 rows and loads its 128 tokens, so the
+// traffic out of L2 and the dequantisation per product halve against two 128 x 256 tiles.  CG = 1 serves smaller batches, where
+// the weights' bytes are the work: tiles of 128 rows x up to 128 tokens, K split over a cluster of C blocks that sum through
+// distributed shared memory when there are too few tiles for the SMs.
+//
+// Warps: 0 token loads | 1 MMA | 2 code loads | 3 TMEM allocation | 4..11 dequantisation (two warpgroups, alternate 64-column
+// blocks, lane quarter = warp % 4) | 12..19 epilogue (lane quarter = warp % 4, half of the token columns each).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "xs_ptx.cuh"
+#include "xs_w4_common.cuh"
+
+namespace xs {
+
+constexpr int kTcThreads = 640;
+constexpr int kTcRows = 128;       // weight rows (TMEM lanes) of a block's tile
+constexpr int kTcBlockK = 64;      // columns of one operand block
+constexpr int kTcRawBlocks = 4;    // operand blocks in one load of codes: 256 columns, 128 bytes a row
+constexpr int kTcRawBytes = kTcRows * 128;
+constexpr int kTcStages = 8;       // operand blocks in flight: TMEM columns of weights, shared memory of tokens
+constexpr int kTcAccCol = kTcStages * (kTcBlockK / 2);
+
+__host__ __device__ constexpr int tc_x_bytes(int cg, int n_tile)
+{
+    return n_tile / cg * kTcBlockK * 2;
+}
+// loads of codes in flight: what the tokens leave of shared memory
+__host__ __device__ constexpr int tc_raw_stages(int cg, int n_tile)
+{
+    return n_tile / cg >= 128 ? 5 : 8;
+}
+__host__ __device__ constexpr int tc_smem_bytes(int cg, int n_tile)
+{
+    return 1024 + tc_raw_stages(cg, n_tile) * kTcRawBytes + kTcStages * tc_x_bytes(cg, n_tile) + 512;
+}
+
+template <int CG>
+__device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+{
+    if constexpr (CG == 1)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
+                     "r"(idesc), "r"(accumulate)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
+                     "r"(idesc), "r"(accumulate)
+                     : "memory");
+}
+// arrive on the barrier (CG = 2: on that of both blocks) when the MMAs issued so far are done
+template <int CG>
+__device__ __forceinline__ void tc_done(uint64_t *bar)
+{
+    if constexpr (CG == 1)
+        tc_commit(bar);
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                     "h"(static_cast<uint16_t>(3))
+                     : "memory");
+}
+// the address of the leading block's copy of a barrier
+__device__ __forceinline__ uint32_t leader_addr(uint64_t *bar)
+{
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(bar)));
+    return a;
+}
+template <int CG>
+__device__ __forceinline__ void tc_arrive_leader(uint64_t *bar)
+{
+    if constexpr (CG == 1)
+        mbar_arrive(bar);
+    else
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(bar)) : "memory");
+}
+// 2-D tiled load into this block's shared memory; CG = 2: the bytes are counted on the leading block's barrier
+template <int CG>
+__device__ __forceinline__ void tc_load_x(void *dst, const CUtensorMap *m, uint64_t *bar, int32_t c0, int32_t c1, uint64_t policy)
+{
+    if constexpr (CG == 1)
+        tma_load_2d(dst, m, bar, c0, c1, policy);
+    else
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+                     " [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(smem_u32(dst)),
+                     "l"(reinterpret_cast<uint64_t>(m)), "r"(leader_addr(bar)), "r"(c0), "r"(c1), "l"(policy)
+                     : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+                 "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+                 "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+                 "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait()
+{
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t bf16x2_mul(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// a wait of all lanes with one outcome: what follows is executed by whole warps
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag)
+{
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+
+struct TcShape {
+    int n_out, T, K, G_log; // G_log: log2 of the group
+    int w_tiles, t_tiles;   // tiles along the features and along the tokens
+    int split;              // blocks that share a tile (CG = 1)
+};
+
+// Work item -> tile.  Eight token tiles go with each weight tile before the next one, so that what runs at one time shares both.
+__device__ __forceinline__ void tc_tile(const TcShape &s, int item, int &wt, int &tt)
+{
+    constexpr int kGroup = 8;
+    const int per = kGroup * s.w_tiles, g = item / per, first = g * kGroup;
+    const int width = s.t_tiles - first < kGroup ? s.t_tiles - first : kGroup, r = item - g * per;
+    wt = r / width;
+    tt = first + r - wt * width;
+}
+
+template <int CG, int N_TILE, bool GATED>
+__global__ void __launch_bounds__(kTcThreads, 1)
+w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const W4Matrix w, __nv_bfloat16 *__restrict__ out,
+             const TcShape s, int act, int32_t *__restrict__ status)
+{
+    constexpr int RAW = tc_raw_stages(CG, N_TILE), X_BYTES = tc_x_bytes(CG, N_TILE);
+    constexpr int FEATURES = GATED ? kTcRows / 2 : kTcRows; // of a block
+    constexpr int NBUF = N_TILE <= 128 ? 2 : 1;             // accumulators
+    constexpr uint32_t IDESC = make_idesc(1, 1, kTcRows * CG, N_TILE);
+
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *x_smem = smem + RAW * kTcRawBytes;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(x_smem + kTcStages * X_BYTES);
+    uint64_t *raw_full = bars, *raw_empty = raw_full + RAW;
+    uint64_t *x_full = raw_empty + RAW, *a_full = x_full + kTcStages, *empty = a_full + kTcStages;
+    uint64_t *acc_full = empty + kTcStages, *acc_empty = acc_full + NBUF;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + NBUF);
+    volatile uint32_t *abort_flag = tmem_slot + 1;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = CG > 1 || s.split > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const bool leader = CG == 1 || rank == 0;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < RAW; i++) {
+            mbar_init(&raw_full[i], 1);
+            mbar_init(&raw_empty[i], 8);
+        }
+        for (int i = 0; i < kTcStages; i++) {
+            mbar_init(&x_full[i], 1);
+            mbar_init(&a_full[i], 4 * CG);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < NBUF; i++) {
+            mbar_init(&acc_full[i], 1);
+            mbar_init(&acc_empty[i], 8 * CG);
+        }
+        *abort_flag = 0;
+        fence_mbar_init();
+        prefetch_tmap(&tmap_w);
+        prefetch_tmap(&tmap_x);
+    }
+    if (warp == 3) {
+        if constexpr (CG == 1) {
+            tmem_alloc(tmem_slot, 512);
+            tmem_relinquish();
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        }
+    }
+    tc_fence_before();
+    if constexpr (CG > 1)
+        cluster_barrier(); // the other block arrives on barriers of this one
+    else
+        __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait(); // everything above touches only shared memory and TMEM
+
+    const int all_raw = (s.K + kTcRawBlocks * kTcBlockK - 1) / (kTcRawBlocks * kTcBlockK);
+    const int raw_per = (all_raw + s.split - 1) / s.split;
+    const int raw0 = CG == 1 ? rank * raw_per : 0, raw1 = min(raw0 + raw_per, all_raw); // this block's loads of codes
+    const int kb0 = raw0 * kTcRawBlocks, kb1 = min(raw1 * kTcRawBlocks, (s.K + kTcBlockK - 1) / kTcBlockK);
+    const int n_kb = kb1 - kb0;
+    const int per_item = CG > 1 ? CG : s.split; // blocks working on one item
+    const int items = s.w_tiles * s.t_tiles, item0 = blockIdx.x / per_item, item_step = gridDim.x / per_item;
+    // first feature of this block's part of a weight tile, first token of its part of a token tile
+    const int block_feature = CG > 1 ? rank * FEATURES : 0, block_token = CG > 1 ? rank * (N_TILE / CG) : 0;
+
+    bool ok = true;
+    if (warp == 0 && lane == 0) {
+        const uint64_t policy = policy_evict_last();
+        uint32_t n = 0;
+        for (int item = item0; item < items && ok; item += item_step) {
+            int wt, tt;
+            tc_tile(s, item, wt, tt);
+            for (int kb = kb0; kb < kb1; kb++, n++) {
+                const uint32_t st = n % kTcStages;
+                if (!mbar_wait(&empty[st], ((n / kTcStages) & 1) ^ 1, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                if (leader)
+                    mbar_arrive_expect_tx(&x_full[st], X_BYTES * CG);
+                tc_load_x<CG>(x_smem + st * X_BYTES, &tmap_x, &x_full[st], kb * kTcBlockK, tt * N_TILE + block_token, policy);
+            }
+        }
+    } else if (warp == 2 && lane == 0) {
+        const uint64_t policy = s.t_tiles > 1 ? policy_evict_last() : policy_evict_first();
+        uint32_t n = 0;
+        for (int item = item0; item < items && ok; item += item_step) {
+            int wt, tt;
+            tc_tile(s, item, wt, tt);
+            for (int r = raw0; r < raw1; r++, n++) {
+                const uint32_t st = n % RAW;
+                if (!mbar_wait(&raw_empty[st], ((n / RAW) & 1) ^ 1, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                mbar_arrive_expect_tx(&raw_full[st], kTcRawBytes);
+                tma_load_3d(smem + st * kTcRawBytes, &tmap_w, &raw_full[st], r * 128, wt * FEATURES * CG + block_feature, 0, policy);
+            }
+        }
+    } else if (warp == 1 && lane == 0 && leader) {
+        uint32_t n = 0, use = 0;
+        for (int item = item0; item < items && ok; item += item_step, use++) {
+            const uint32_t buf = use % NBUF, acc = tmem + kTcAccCol + buf * N_TILE;
+            if (!mbar_wait(&acc_empty[buf], ((use / NBUF) & 1) ^ 1, abort_flag)) {
+                ok = false;
+                break;
+            }
+            for (int kb = 0; kb < n_kb; kb++, n++) {
+                const uint32_t st = n % kTcStages, ph = (n / kTcStages) & 1;
+                if (!mbar_wait(&x_full[st], ph, abort_flag) || !mbar_wait(&a_full[st], ph, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint64_t db = make_desc_sw128(smem_u32(x_smem + st * X_BYTES));
+                const uint32_t a = tmem + st * (kTcBlockK / 2);
+#pragma unroll
+                for (int kk = 0; kk < kTcBlockK / 16; kk++)
+                    tc_mma<CG>(acc, a + kk * 8, db + 2 * kk, IDESC, (kb | kk) ? 1u : 0u);
+                tc_done<CG>(&empty[st]);
+            }
+            if (ok)
+                tc_done<CG>(&acc_full[buf]);
+        }
+    } else if (warp >= 4 && warp < 12) {
+        const int group = (warp - 4) >> 2, q = warp & 3;
+        // the row of the codes (as the load laid them out) that this thread's TMEM lane holds; GATED: 16 gate rows, then their 16 up rows
+        const int raw_row = GATED ? (lane >> 4) * 64 + q * 16 + (lane & 15) : q * 32 + lane;
+        const int feature = GATED ? q * 16 + (lane & 15) : raw_row;
+        const uint32_t raw_addr = smem_u32(smem) + raw_row * 128, swz = (raw_row & 7) << 4;
+        const int groups = s.K >> s.G_log;
+        const bool vec = groups % 8 == 0 && reinterpret_cast<uintptr_t>(w.scales) % 16 == 0 && reinterpret_cast<uintptr_t>(w.zeros) % 8 == 0;
+        // Scales and zero points of this row, eight groups (a segment) at a time, loaded two segments ahead.  A segment begins
+        // where a load of codes does.
+        struct Segment {
+            uint4 s;
+            uint2 z;
+        };
+        const int seg_log = s.G_log - 5; // loads of codes in a segment
+        const int seg0 = raw0 >> seg_log, seg1 = (raw1 - 1) >> seg_log;
+        int ld_item = item0, ld_seg = seg0;
+        auto load_segment = [&]() {
+            Segment r;
+            r.s = make_uint4(0, 0, 0, 0);
+            r.z = make_uint2(0x08080808u, 0x08080808u);
+            if (ld_item < items) {
+                int wt, tt;
+                tc_tile(s, ld_item, wt, tt);
+                const int f = min(wt * FEATURES * CG + block_feature + feature, s.n_out - 1);
+                const size_t o = (static_cast<size_t>(f) + (GATED && lane >= 16 ? s.n_out : 0)) * groups + ld_seg * 8;
+                const uint16_t *sp = reinterpret_cast<const uint16_t *>(w.scales) + o;
+                if (vec) {
+                    r.s = __ldg(reinterpret_cast<const uint4 *>(sp));
+                    if (w.zeros)
+                        r.z = __ldg(reinterpret_cast<const uint2 *>(w.zeros + o));
+                } else {
+                    const int have = groups - ld_seg * 8;
+                    uint32_t sv[4] = {}, zv[2] = {};
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        if (i < have)
+                            sv[i / 2] |= static_cast<uint32_t>(__ldg(sp + i)) << (i % 2 * 16);
+                    r.s = make_uint4(sv[0], sv[1], sv[2], sv[3]);
+                    if (w.zeros) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            if (i < have)
+                                zv[i / 4] |= static_cast<uint32_t>(__ldg(w.zeros + o + i)) << (i % 4 * 8);
+                        r.z = make_uint2(zv[0], zv[1]);
+                    }
+                }
+                if (++ld_seg > seg1) {
+                    ld_seg = seg0;
+                    ld_item += item_step;
+                }
+            }
+            return r;
+        };
+        Segment cur, next, after;
+#pragma unroll 1
+        for (int i = 0; i < 2; i++) {
+            next = after;
+            after = load_segment();
+        }
+        uint32_t n = 0, nr = 0;
+        for (int item = item0; item < items && ok; item += item_step) {
+            int seg = -1;
+            for (int r = raw0; r < raw1; r++, nr++) {
+                if (r >> seg_log != seg) {
+                    seg = r >> seg_log;
+                    cur = next;
+                    next = after;
+                    after = load_segment();
+                }
+                const uint32_t rs = nr % RAW;
+                if (!warp_wait(&raw_full[rs], (nr / RAW) & 1, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+#pragma unroll 1
+                for (int b = group; b < kTcRawBlocks; b += 2) {
+                    const int kb = r * kTcRawBlocks + b;
+                    if (kb >= kb1)
+                        break;
+                    const uint32_t g_kb = n + kb - kb0, st = g_kb % kTcStages;
+                    uint32_t a[32];
+#pragma unroll
+                    for (int h = 0; h < 2; h++) { // 32 columns: one 16-byte piece of codes, one group
+                        const int i = ((2 * kb + h) >> seg_log) & 7;
+                        uint32_t sv = i & 4 ? (i & 2 ? cur.s.w : cur.s.z) : (i & 2 ? cur.s.y : cur.s.x);
+                        sv = __byte_perm(sv, 0, i & 1 ? 0x3232 : 0x1010);
+                        if ((2 * kb + h) * 32 >= s.K)
+                            sv = 0; // past the end: the codes read as zero, and so must the weight, whatever the zero point
+                        const uint32_t mz = w4_minus_zero(((i & 4 ? cur.z.y : cur.z.x) >> (i & 3) * 8) & 15u);
+                        const uint4 qv = lds128(raw_addr + rs * kTcRawBytes + (((b * 2 + h) << 4) ^ swz));
+                        const uint32_t words[4] = {qv.x, qv.y, qv.z, qv.w};
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+#pragma unroll
+                            for (int c = 0; c < 4; c++) {
+                                // byte c in both halves: its low nibble stays in the first, its high nibble in the second
+                                const uint32_t v = __byte_perm(words[j], 0, 0x4040 | c << 8 | c) & 0x00f0000fu;
+                                a[h * 16 + j * 4 + c] = bf16x2_mul(w4_fma(v, 0x7d007f00u, mz), sv); // times 2^127 and 2^123
+                            }
+                    }
+                    if (!warp_wait(&empty[st], ((g_kb / kTcStages) & 1) ^ 1, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    tmem_st32(tmem + (static_cast<uint32_t>(q * 32) << 16) + st * (kTcBlockK / 2), a);
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0)
+                        tc_arrive_leader<CG>(&a_full[st]);
+                }
+                if (!ok)
+                    break;
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(&raw_empty[rs]);
+            }
+            n += n_kb;
+        }
+    } else if (warp >= 12) {
+        const int q = warp & 3, part = (warp - 12) >> 2;
+        constexpr int COLS = N_TILE / 2; // of this warp
+        const int lane_feature = GATED ? q * 16 + (lane & 15) : q * 32 + lane;
+        uint32_t use = 0;
+        for (int item = item0; item < items; item += item_step, use++) {
+            int wt, tt;
+            tc_tile(s, item, wt, tt);
+            const uint32_t buf = use % NBUF;
+            if (!warp_wait(&acc_full[buf], (use / NBUF) & 1, abort_flag)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16) + kTcAccCol + buf * N_TILE + part * COLS;
+            const int feature = wt * FEATURES * CG + block_feature + lane_feature, token0 = tt * N_TILE + part * COLS;
+            if (CG == 1 && s.split > 1) {
+                // the sums of this block's slice of K, [token][lane], over the operand ring, which nothing reads or fills any more
+                float *red = reinterpret_cast<float *>(smem);
+                for (int c = 0; c < COLS; c += 16) {
+                    uint32_t v[16];
+                    tmem_ld16(acc + c, v);
+                    tmem_ld_wait_16(v);
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        red[(part * COLS + c + i) * kTcRows + q * 32 + lane] = __uint_as_float(v[i]);
+                }
+                break; // one tile a block; summed below
+            }
+#pragma unroll 2
+            for (int c = 0; c < COLS; c += 16) {
+                uint32_t v[16];
+                tmem_ld16(acc + c, v);
+                tmem_ld_wait_16(v);
+                if (c + 16 == COLS) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0)
+                        tc_arrive_leader<CG>(&acc_empty[buf]);
+                }
+                __nv_bfloat16 *o = out + static_cast<size_t>(token0 + c) * s.n_out + feature;
+                if constexpr (GATED) {
+                    // lanes 0..15 hold gate sums and 16..31 the up sums of the same features: of each pair of tokens the first half
+                    // of the warp finishes the even one, the second half the odd one
+                    const bool up = lane >= 16;
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        const float give = __uint_as_float(up ? v[i] : v[i + 1]), got = __shfl_xor_sync(0xffffffffu, give, 16);
+                        const float g = kW4Unit * (up ? got : __uint_as_float(v[i])), u = kW4Unit * (up ? __uint_as_float(v[i + 1]) : got);
+                        const int t = i + (up ? 1 : 0);
+                        if (feature < s.n_out && token0 + c + t < s.T)
+                            o[static_cast<size_t>(t) * s.n_out] = __float2bfloat16_rn(w4_activation(g, act) * u);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (feature < s.n_out && token0 + c + i < s.T)
+                            o[static_cast<size_t>(i) * s.n_out] = __float2bfloat16_rn(kW4Unit * __uint_as_float(v[i]));
+                }
+            }
+        }
+    }
+    if (!ok) {
+        *abort_flag = 1;
+        atomicOr(status, kStatusWaitTimeout);
+    }
+    __syncwarp();
+    if (CG == 1 && s.split > 1)
+        cluster_barrier();
+    if (CG == 1 && s.split > 1 && warp >= 12) {
+        // this block's tokens of the tile: the slices' sums in the order of the slices
+        int wt, tt;
+        tc_tile(s, item0, wt, tt);
+        const uint32_t red = smem_u32(smem);
+        const int share = N_TILE / s.split;
+        for (int i = threadIdx.x - 384; i < share * FEATURES; i += 256) {
+            const int c = rank * share + i / FEATURES, f = i % FEATURES, feature = wt * FEATURES + f, token = tt * N_TILE + c;
+            if (feature >= s.n_out || token >= s.T)
+                continue;
+            const int row = GATED ? (f >> 4) * 32 + (f & 15) : f;
+            float v = 0.0f, u = 0.0f;
+            for (int r = 0; r < s.split; r++) {
+                v += ld_cluster_f32(red + (c * kTcRows + row) * 4, r);
+                if (GATED)
+                    u += ld_cluster_f32(red + (c * kTcRows + row + 16) * 4, r);
+            }
+            out[static_cast<size_t>(token) * s.n_out + feature] = __float2bfloat16_rn(GATED ? w4_activation(kW4Unit * v, act) * (kW4Unit * u) : kW4Unit * v);
+        }
+    }
+    if (*abort_flag)
+        for (int i = 0; i < 64; i++)
+            __nanosleep(4096); // copies in flight land before the shared memory is given up
+    tc_fence_before();
+    if (CG > 1 || s.split > 1)
+        cluster_barrier(); // nobody leaves while the other block may read its shared memory or write its TMEM
+    else
+        __syncthreads();
+    if (warp == 3) {
+        tc_fence_after();
+        if constexpr (CG == 1)
+            tmem_dealloc(tmem, 512);
+        else
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+} // namespace xs
