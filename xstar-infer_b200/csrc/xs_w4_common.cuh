@@ -52,6 +52,15 @@ __device__ __forceinline__ float w4_activation(float v, int act)
     return e < 1e37f ? __fdividef(v, e) : (v != v ? v : v * 0.0f);
 }
 
+// A bounded wait of a whole warp with one outcome.  One lane polls: a poll by 32 lanes is 32 operations on the barrier's word, and
+// waiting warps then slow down those that work.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag)
+{
+    bool ok = true;
+    if ((threadIdx.x & 31) == 0)
+        ok = mbar_wait(bar, parity, abort_flag);
+    return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+}
 __device__ __forceinline__ uint4 lds128(uint32_t a)
 {
     uint4 v;

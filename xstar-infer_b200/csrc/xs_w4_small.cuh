@@ -202,11 +202,10 @@ w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, cons
             fetch(stage == 0 ? stages - 1 : stage - 1);
             uint32_t sc_after[4][SLOTS];
             load_scales(sc_after);
-            if (!mbar_wait(&full[stage], phase, abort_flag)) {
+            if (!warp_wait(&full[stage], phase, abort_flag)) {
                 *abort_flag = 1;
                 atomicOr(status, kStatusWaitTimeout);
             }
-            __syncwarp();
             const uint32_t st = ring + stage * kSwStageBytes + frag;
             uint32_t xa = x_lane + (chunk - chunk0) * (kSwChunk / 32) * x_step;
             float c[2][4], s[2][2];

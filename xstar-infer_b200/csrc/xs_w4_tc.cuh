@@ -45,6 +45,12 @@ __host__ __device__ constexpr int tc_smem_bytes(int cg, int n_tile)
     return 1024 + tc_raw_stages(cg, n_tile) * kTcRawBytes + kTcStages * tc_x_bytes(cg, n_tile) + 512;
 }
 
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
 template <int CG>
 __device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
 {
@@ -81,7 +87,9 @@ __device__ __forceinline__ void tc_arrive_leader(uint64_t *bar)
     if constexpr (CG == 1)
         mbar_arrive(bar);
     else
-        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(bar)) : "memory");
+        // what is handed over lies in TMEM, ordered by the tcgen05 fences around the barrier; a release at cluster scope would
+        // hold the warp for more than a thousand cycles
+        asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(bar)) : "memory");
 }
 // 2-D tiled load into this block's shared memory; CG = 2: the bytes are counted on the leading block's barrier
 template <int CG>
@@ -115,12 +123,6 @@ __device__ __forceinline__ uint32_t bf16x2_mul(uint32_t a, uint32_t b)
     return r;
 }
 
-// a wait of all lanes with one outcome: what follows is executed by whole warps
-__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag)
-{
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
-}
-
 struct TcShape {
     int n_out, T, K, G_log; // G_log: log2 of the group
     int w_tiles, t_tiles;   // tiles along the features and along the tokens
@@ -152,12 +154,12 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
     uint8_t *x_smem = smem + RAW * kTcRawBytes;
     uint64_t *bars = reinterpret_cast<uint64_t *>(x_smem + kTcStages * X_BYTES);
     uint64_t *raw_full = bars, *raw_empty = raw_full + RAW;
-    uint64_t *x_full = raw_empty + RAW, *a_full = x_full + kTcStages, *empty = a_full + kTcStages;
+    uint64_t *full = raw_empty + RAW, *empty = full + kTcStages; // full: both operands of a block are there
     uint64_t *acc_full = empty + kTcStages, *acc_empty = acc_full + NBUF;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + NBUF);
     volatile uint32_t *abort_flag = tmem_slot + 1;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31; // warp: known to be uniform
     const int rank = CG > 1 || s.split > 1 ? static_cast<int>(cluster_rank()) : 0;
     const bool leader = CG == 1 || rank == 0;
 
@@ -167,8 +169,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
             mbar_init(&raw_empty[i], 8);
         }
         for (int i = 0; i < kTcStages; i++) {
-            mbar_init(&x_full[i], 1);
-            mbar_init(&a_full[i], 4 * CG);
+            mbar_init(&full[i], 4 * CG + 1); // the dequantising warps, and the token load with its bytes
             mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < NBUF; i++) {
@@ -222,8 +223,8 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                     break;
                 }
                 if (leader)
-                    mbar_arrive_expect_tx(&x_full[st], X_BYTES * CG);
-                tc_load_x<CG>(x_smem + st * X_BYTES, &tmap_x, &x_full[st], kb * kTcBlockK, tt * N_TILE + block_token, policy);
+                    mbar_arrive_expect_tx(&full[st], X_BYTES * CG);
+                tc_load_x<CG>(x_smem + st * X_BYTES, &tmap_x, &full[st], kb * kTcBlockK, tt * N_TILE + block_token, policy);
             }
         }
     } else if (warp == 2 && lane == 0) {
@@ -242,29 +243,38 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                 tma_load_3d(smem + st * kTcRawBytes, &tmap_w, &raw_full[st], r * 128, wt * FEATURES * CG + block_feature, 0, policy);
             }
         }
-    } else if (warp == 1 && lane == 0 && leader) {
-        uint32_t n = 0, use = 0;
+    } else if (warp == 1 && leader) {
+        // The whole warp walks the loop and one elected lane issues, so that addresses and descriptors stay in uniform registers;
+        // the waits poll without parking the warp.  What this warp does between blocks is time the tensor pipe may stand still.
+        const bool elected = elect_one();
+        const uint64_t desc0 = make_desc_sw128(smem_u32(x_smem));
+        uint32_t st = 0, ph = 0, use = 0;
         for (int item = item0; item < items && ok; item += item_step, use++) {
             const uint32_t buf = use % NBUF, acc = tmem + kTcAccCol + buf * N_TILE;
-            if (!mbar_wait(&acc_empty[buf], ((use / NBUF) & 1) ^ 1, abort_flag)) {
+            if (!mbar_spin_wait(&acc_empty[buf], ((use / NBUF) & 1) ^ 1, abort_flag)) {
                 ok = false;
                 break;
             }
-            for (int kb = 0; kb < n_kb; kb++, n++) {
-                const uint32_t st = n % kTcStages, ph = (n / kTcStages) & 1;
-                if (!mbar_wait(&x_full[st], ph, abort_flag) || !mbar_wait(&a_full[st], ph, abort_flag)) {
+            for (int kb = 0; kb < n_kb; kb++) {
+                if (!mbar_spin_wait(&full[st], ph, abort_flag)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint64_t db = make_desc_sw128(smem_u32(x_smem + st * X_BYTES));
+                const uint64_t db = desc0 + st * (X_BYTES >> 4);
                 const uint32_t a = tmem + st * (kTcBlockK / 2);
+                if (elected) {
 #pragma unroll
-                for (int kk = 0; kk < kTcBlockK / 16; kk++)
-                    tc_mma<CG>(acc, a + kk * 8, db + 2 * kk, IDESC, (kb | kk) ? 1u : 0u);
-                tc_done<CG>(&empty[st]);
+                    for (int kk = 0; kk < kTcBlockK / 16; kk++)
+                        tc_mma<CG>(acc, a + kk * 8, db + 2 * kk, IDESC, (kb | kk) ? 1u : 0u);
+                    tc_done<CG>(&empty[st]);
+                }
+                if (++st == kTcStages) {
+                    st = 0;
+                    ph ^= 1;
+                }
             }
-            if (ok)
+            if (ok && elected)
                 tc_done<CG>(&acc_full[buf]);
         }
     } else if (warp >= 4 && warp < 12) {
@@ -338,7 +348,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                     after = load_segment();
                 }
                 const uint32_t rs = nr % RAW;
-                if (!warp_wait(&raw_full[rs], (nr / RAW) & 1, abort_flag)) {
+                if (!__all_sync(0xffffffffu, mbar_spin_wait(&raw_full[rs], (nr / RAW) & 1, abort_flag))) {
                     ok = false;
                     break;
                 }
@@ -347,7 +357,8 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                     const int kb = r * kTcRawBlocks + b;
                     if (kb >= kb1)
                         break;
-                    const uint32_t g_kb = n + kb - kb0, st = g_kb % kTcStages;
+                    const uint32_t g_kb = n + kb - kb0, st = g_kb % kTcStages, free = ((g_kb / kTcStages) & 1) ^ 1;
+                    const bool is_free = mbar_test_wait(&empty[st], free); // asked early, its answer is there after the arithmetic
                     uint32_t a[32];
 #pragma unroll
                     for (int h = 0; h < 2; h++) { // 32 columns: one 16-byte piece of codes, one group
@@ -368,7 +379,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                                 a[h * 16 + j * 4 + c] = bf16x2_mul(w4_fma(v, 0x7d007f00u, mz), sv); // times 2^127 and 2^123
                             }
                     }
-                    if (!warp_wait(&empty[st], ((g_kb / kTcStages) & 1) ^ 1, abort_flag)) {
+                    if (!__all_sync(0xffffffffu, is_free || mbar_spin_wait(&empty[st], free, abort_flag))) {
                         ok = false;
                         break;
                     }
@@ -378,7 +389,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0)
-                        tc_arrive_leader<CG>(&a_full[st]);
+                        tc_arrive_leader<CG>(&full[st]);
                 }
                 if (!ok)
                     break;
