@@ -11,8 +11,13 @@
 // the weights' bytes are the work: tiles of 128 rows x up to 128 tokens, K split over a cluster of C blocks that sum through
 // distributed shared memory when there are too few tiles for the SMs.
 //
-// Warps: 0 token loads | 1 MMA | 2 code loads | 3 TMEM allocation | 4..11 dequantisation (two warpgroups, alternate 64-column
-// blocks, lane quarter = warp % 4) | 12..19 epilogue (lane quarter = warp % 4, half of the token columns each).
+// Warps: 0, 3 token loads, alternate blocks (3 owns the TMEM allocation) | 1 MMA | 2 code loads | 4..11 dequantisation (two
+// warpgroups, one half of each operand block, lane quarter = warp % 4) | 12..19 epilogue (lane quarter = warp % 4, half of the
+// token columns each).
+//
+// An operand block is 128 columns because every hand-over costs its roles a few hundred cycles (a poll of a barrier about 110, a
+// parked wait about 300, an expect or a load 100 each): with 64 columns one loading thread took 600 cycles a block, whatever the
+// tile, and everybody else waited for it.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -25,10 +30,10 @@ namespace xs {
 
 constexpr int kTcThreads = 640;
 constexpr int kTcRows = 128;       // weight rows (TMEM lanes) of a block's tile
-constexpr int kTcBlockK = 64;      // columns of one operand block
-constexpr int kTcRawBlocks = 4;    // operand blocks in one load of codes: 256 columns, 128 bytes a row
+constexpr int kTcBlockK = 128;     // columns of one operand block: two 128-byte pieces of a token's row
+constexpr int kTcRawBlocks = 2;    // operand blocks in one load of codes: 256 columns, 128 bytes a row
 constexpr int kTcRawBytes = kTcRows * 128;
-constexpr int kTcStages = 8;       // operand blocks in flight: TMEM columns of weights, shared memory of tokens
+constexpr int kTcStages = 4;       // operand blocks in flight: TMEM columns of weights, shared memory of tokens
 constexpr int kTcAccCol = kTcStages * (kTcBlockK / 2);
 
 __host__ __device__ constexpr int tc_x_bytes(int cg, int n_tile)
@@ -169,7 +174,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
             mbar_init(&raw_empty[i], 8);
         }
         for (int i = 0; i < kTcStages; i++) {
-            mbar_init(&full[i], 4 * CG + 1); // the dequantising warps, and the token load with its bytes
+            mbar_init(&full[i], 8 * CG + 1); // the dequantising warps, and the token load with its bytes
             mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < NBUF; i++) {
@@ -210,21 +215,25 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
     const int block_feature = CG > 1 ? rank * FEATURES : 0, block_token = CG > 1 ? rank * (N_TILE / CG) : 0;
 
     bool ok = true;
-    if (warp == 0 && lane == 0) {
+    if ((warp == 0 || warp == 3) && lane == 0) {
         const uint64_t policy = policy_evict_last();
         uint32_t n = 0;
         for (int item = item0; item < items && ok; item += item_step) {
             int wt, tt;
             tc_tile(s, item, wt, tt);
+            const int token = tt * N_TILE + block_token;
             for (int kb = kb0; kb < kb1; kb++, n++) {
+                if ((n & 1) != (warp == 3 ? 1u : 0u))
+                    continue;
                 const uint32_t st = n % kTcStages;
-                if (!mbar_wait(&empty[st], ((n / kTcStages) & 1) ^ 1, abort_flag)) {
+                if (!mbar_spin_wait(&empty[st], ((n / kTcStages) & 1) ^ 1, abort_flag)) {
                     ok = false;
                     break;
                 }
                 if (leader)
                     mbar_arrive_expect_tx(&full[st], X_BYTES * CG);
-                tc_load_x<CG>(x_smem + st * X_BYTES, &tmap_x, &full[st], kb * kTcBlockK, tt * N_TILE + block_token, policy);
+                tc_load_x<CG>(x_smem + st * X_BYTES, &tmap_x, &full[st], kb * kTcBlockK, token, policy);
+                tc_load_x<CG>(x_smem + st * X_BYTES + X_BYTES / 2, &tmap_x, &full[st], kb * kTcBlockK + 64, token, policy);
             }
         }
     } else if (warp == 2 && lane == 0) {
@@ -235,7 +244,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
             tc_tile(s, item, wt, tt);
             for (int r = raw0; r < raw1; r++, n++) {
                 const uint32_t st = n % RAW;
-                if (!mbar_wait(&raw_empty[st], ((n / RAW) & 1) ^ 1, abort_flag)) {
+                if (!mbar_spin_wait(&raw_empty[st], ((n / RAW) & 1) ^ 1, abort_flag)) {
                     ok = false;
                     break;
                 }
@@ -266,7 +275,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                 if (elected) {
 #pragma unroll
                     for (int kk = 0; kk < kTcBlockK / 16; kk++)
-                        tc_mma<CG>(acc, a + kk * 8, db + 2 * kk, IDESC, (kb | kk) ? 1u : 0u);
+                        tc_mma<CG>(acc, a + kk * 8, db + (kk / 4) * (X_BYTES / 2 >> 4) + 2 * (kk % 4), IDESC, (kb | kk) ? 1u : 0u);
                     tc_done<CG>(&empty[st]);
                 }
                 if (++st == kTcStages) {
@@ -337,38 +346,39 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
             next = after;
             after = load_segment();
         }
-        uint32_t n = 0, nr = 0;
+        const uint32_t dst0 = tmem + (static_cast<uint32_t>(q * 32) << 16) + group * 32;
+        uint32_t rs = 0, rph = 0, st = 0, free = 1;
+        bool raw_there = mbar_test_wait(&raw_full[0], 0);
         for (int item = item0; item < items && ok; item += item_step) {
             int seg = -1;
-            for (int r = raw0; r < raw1; r++, nr++) {
+            for (int r = raw0; r < raw1 && ok; r++) {
                 if (r >> seg_log != seg) {
                     seg = r >> seg_log;
                     cur = next;
                     next = after;
                     after = load_segment();
                 }
-                const uint32_t rs = nr % RAW;
-                if (!__all_sync(0xffffffffu, mbar_spin_wait(&raw_full[rs], (nr / RAW) & 1, abort_flag))) {
+                if (!__all_sync(0xffffffffu, raw_there || mbar_spin_wait(&raw_full[rs], rph, abort_flag))) {
                     ok = false;
                     break;
                 }
+                const uint32_t codes = raw_addr + rs * kTcRawBytes;
 #pragma unroll 1
-                for (int b = group; b < kTcRawBlocks; b += 2) {
-                    const int kb = r * kTcRawBlocks + b;
-                    if (kb >= kb1)
+                for (int b = 0; b < kTcRawBlocks; b++) {
+                    if (r * kTcRawBlocks + b >= kb1)
                         break;
-                    const uint32_t g_kb = n + kb - kb0, st = g_kb % kTcStages, free = ((g_kb / kTcStages) & 1) ^ 1;
                     const bool is_free = mbar_test_wait(&empty[st], free); // asked early, its answer is there after the arithmetic
                     uint32_t a[32];
 #pragma unroll
                     for (int h = 0; h < 2; h++) { // 32 columns: one 16-byte piece of codes, one group
-                        const int i = ((2 * kb + h) >> seg_log) & 7;
+                        const int piece = b * 4 + group * 2 + h, half = r * 8 + piece;
+                        const int i = (half >> seg_log) & 7;
                         uint32_t sv = i & 4 ? (i & 2 ? cur.s.w : cur.s.z) : (i & 2 ? cur.s.y : cur.s.x);
                         sv = __byte_perm(sv, 0, i & 1 ? 0x3232 : 0x1010);
-                        if ((2 * kb + h) * 32 >= s.K)
+                        if (half * 32 >= s.K)
                             sv = 0; // past the end: the codes read as zero, and so must the weight, whatever the zero point
                         const uint32_t mz = w4_minus_zero(((i & 4 ? cur.z.y : cur.z.x) >> (i & 3) * 8) & 15u);
-                        const uint4 qv = lds128(raw_addr + rs * kTcRawBytes + (((b * 2 + h) << 4) ^ swz));
+                        const uint4 qv = lds128(codes + ((piece << 4) ^ swz));
                         const uint32_t words[4] = {qv.x, qv.y, qv.z, qv.w};
 #pragma unroll
                         for (int j = 0; j < 4; j++)
@@ -384,20 +394,26 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                         break;
                     }
                     tc_fence_after();
-                    tmem_st32(tmem + (static_cast<uint32_t>(q * 32) << 16) + st * (kTcBlockK / 2), a);
+                    tmem_st32(dst0 + st * (kTcBlockK / 2), a);
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0)
                         tc_arrive_leader<CG>(&full[st]);
+                    if (++st == kTcStages) {
+                        st = 0;
+                        free ^= 1;
+                    }
                 }
-                if (!ok)
-                    break;
                 __syncwarp();
                 if (lane == 0)
                     mbar_arrive(&raw_empty[rs]);
+                if (++rs == RAW) {
+                    rs = 0;
+                    rph ^= 1;
+                }
+                raw_there = mbar_test_wait(&raw_full[rs], rph);
             }
-            n += n_kb;
         }
     } else if (warp >= 12) {
         const int q = warp & 3, part = (warp - 12) >> 2;
