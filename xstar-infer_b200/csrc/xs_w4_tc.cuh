@@ -11,9 +11,9 @@
 // the weights' bytes are the work: tiles of 128 rows x up to 128 tokens, K split over a cluster of C blocks that sum through
 // distributed shared memory when there are too few tiles for the SMs.
 //
-// Warps: 0, 3 token loads, alternate blocks (3 owns the TMEM allocation) | 1 MMA | 2 code loads | 4..11 dequantisation (two
-// warpgroups, one half of each operand block, lane quarter = warp % 4) | 12..19 epilogue (lane quarter = warp % 4, half of the
-// token columns each).
+// Warps: 0, 3 token loads, alternate blocks (3 owns the TMEM allocation) | 1 MMA | 2 code loads | 4..19 dequantisation (four
+// warpgroups: two on the even operand blocks and two on the odd ones, each on half of the block's columns; lane quarter =
+// warp % 4) | 20..27 epilogue (lane quarter = warp % 4, half of the token columns each).
 //
 // An operand block is 128 columns because every hand-over costs its roles a few hundred cycles (a poll of a barrier about 110, a
 // parked wait about 300, an expect or a load 100 each): with 64 columns one loading thread took 600 cycles a block, whatever the
@@ -28,7 +28,9 @@
 
 namespace xs {
 
-constexpr int kTcThreads = 640;
+constexpr int kTcDequantWarps = 16;
+constexpr int kTcEpilogueWarp = 4 + kTcDequantWarps;
+constexpr int kTcThreads = 32 * (kTcEpilogueWarp + 8);
 constexpr int kTcRows = 128;       // weight rows (TMEM lanes) of a block's tile
 constexpr int kTcBlockK = 128;     // columns of one operand block: two 128-byte pieces of a token's row
 constexpr int kTcRawBlocks = 2;    // operand blocks in one load of codes: 256 columns, 128 bytes a row
@@ -108,13 +110,11 @@ __device__ __forceinline__ void tc_load_x(void *dst, const CUtensorMap *m, uint6
                      "l"(reinterpret_cast<uint64_t>(m)), "r"(leader_addr(bar)), "r"(c0), "r"(c1), "l"(policy)
                      : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32])
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16])
 {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
-                 "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
                  "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-                 "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
-                 "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+                 "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                  : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait()
@@ -171,7 +171,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
     if (threadIdx.x == 0) {
         for (int i = 0; i < RAW; i++) {
             mbar_init(&raw_full[i], 1);
-            mbar_init(&raw_empty[i], 8);
+            mbar_init(&raw_empty[i], kTcDequantWarps);
         }
         for (int i = 0; i < kTcStages; i++) {
             mbar_init(&full[i], 8 * CG + 1); // the dequantising warps, and the token load with its bytes
@@ -286,8 +286,8 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
             if (ok && elected)
                 tc_done<CG>(&acc_full[buf]);
         }
-    } else if (warp >= 4 && warp < 12) {
-        const int group = (warp - 4) >> 2, q = warp & 3;
+    } else if (warp >= 4 && warp < kTcEpilogueWarp) {
+        const int group = ((warp - 4) >> 2) & 1, odd = (warp - 4) >> 3, q = warp & 3; // half of the block, which block of a load
         // the row of the codes (as the load laid them out) that this thread's TMEM lane holds; GATED: 16 gate rows, then their 16 up rows
         const int raw_row = GATED ? (lane >> 4) * 64 + q * 16 + (lane & 15) : q * 32 + lane;
         const int feature = GATED ? q * 16 + (lane & 15) : raw_row;
@@ -347,11 +347,11 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
             after = load_segment();
         }
         const uint32_t dst0 = tmem + (static_cast<uint32_t>(q * 32) << 16) + group * 32;
-        uint32_t rs = 0, rph = 0, st = 0, free = 1;
+        uint32_t rs = 0, rph = 0, n = 0; // n: operand blocks before this item
         bool raw_there = mbar_test_wait(&raw_full[0], 0);
-        for (int item = item0; item < items && ok; item += item_step) {
+        for (int item = item0; item < items && ok; item += item_step, n += n_kb) {
             int seg = -1;
-            for (int r = raw0; r < raw1 && ok; r++) {
+            for (int r = raw0; r < raw1; r++) {
                 if (r >> seg_log != seg) {
                     seg = r >> seg_log;
                     cur = next;
@@ -362,48 +362,45 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                     ok = false;
                     break;
                 }
-                const uint32_t codes = raw_addr + rs * kTcRawBytes;
-#pragma unroll 1
-                for (int b = 0; b < kTcRawBlocks; b++) {
-                    if (r * kTcRawBlocks + b >= kb1)
-                        break;
+                const int kb = r * kTcRawBlocks + odd;
+                if (kb < kb1) {
+                    const uint32_t block = n + kb - kb0, st = block % kTcStages, free = ((block / kTcStages) & 1) ^ 1;
                     const bool is_free = mbar_test_wait(&empty[st], free); // asked early, its answer is there after the arithmetic
-                    uint32_t a[32];
 #pragma unroll
                     for (int h = 0; h < 2; h++) { // 32 columns: one 16-byte piece of codes, one group
-                        const int piece = b * 4 + group * 2 + h, half = r * 8 + piece;
+                        const int piece = odd * 4 + group * 2 + h, half = r * 8 + piece;
                         const int i = (half >> seg_log) & 7;
                         uint32_t sv = i & 4 ? (i & 2 ? cur.s.w : cur.s.z) : (i & 2 ? cur.s.y : cur.s.x);
                         sv = __byte_perm(sv, 0, i & 1 ? 0x3232 : 0x1010);
                         if (half * 32 >= s.K)
                             sv = 0; // past the end: the codes read as zero, and so must the weight, whatever the zero point
                         const uint32_t mz = w4_minus_zero(((i & 4 ? cur.z.y : cur.z.x) >> (i & 3) * 8) & 15u);
-                        const uint4 qv = lds128(codes + ((piece << 4) ^ swz));
+                        const uint4 qv = lds128(raw_addr + rs * kTcRawBytes + ((piece << 4) ^ swz));
                         const uint32_t words[4] = {qv.x, qv.y, qv.z, qv.w};
+                        uint32_t a[16];
 #pragma unroll
                         for (int j = 0; j < 4; j++)
 #pragma unroll
                             for (int c = 0; c < 4; c++) {
                                 // byte c in both halves: its low nibble stays in the first, its high nibble in the second
                                 const uint32_t v = __byte_perm(words[j], 0, 0x4040 | c << 8 | c) & 0x00f0000fu;
-                                a[h * 16 + j * 4 + c] = bf16x2_mul(w4_fma(v, 0x7d007f00u, mz), sv); // times 2^127 and 2^123
+                                a[j * 4 + c] = bf16x2_mul(w4_fma(v, 0x7d007f00u, mz), sv); // times 2^127 and 2^123
                             }
+                        if (h == 0) {
+                            ok = __all_sync(0xffffffffu, is_free || mbar_spin_wait(&empty[st], free, abort_flag));
+                            if (!ok)
+                                break;
+                            tc_fence_after();
+                        }
+                        tmem_st16(dst0 + st * (kTcBlockK / 2) + h * 16, a);
                     }
-                    if (!__all_sync(0xffffffffu, is_free || mbar_spin_wait(&empty[st], free, abort_flag))) {
-                        ok = false;
+                    if (!ok)
                         break;
-                    }
-                    tc_fence_after();
-                    tmem_st32(dst0 + st * (kTcBlockK / 2), a);
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0)
                         tc_arrive_leader<CG>(&full[st]);
-                    if (++st == kTcStages) {
-                        st = 0;
-                        free ^= 1;
-                    }
                 }
                 __syncwarp();
                 if (lane == 0)
@@ -415,8 +412,8 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                 raw_there = mbar_test_wait(&raw_full[rs], rph);
             }
         }
-    } else if (warp >= 12) {
-        const int q = warp & 3, part = (warp - 12) >> 2;
+    } else if (warp >= kTcEpilogueWarp) {
+        const int q = warp & 3, part = (warp - kTcEpilogueWarp) >> 2;
         constexpr int COLS = N_TILE / 2; // of this warp
         const int lane_feature = GATED ? q * 16 + (lane & 15) : q * 32 + lane;
         uint32_t use = 0;
@@ -484,13 +481,13 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
     __syncwarp();
     if (CG == 1 && s.split > 1)
         cluster_barrier();
-    if (CG == 1 && s.split > 1 && warp >= 12) {
+    if (CG == 1 && s.split > 1 && warp >= kTcEpilogueWarp) {
         // this block's tokens of the tile: the slices' sums in the order of the slices
         int wt, tt;
         tc_tile(s, item0, wt, tt);
         const uint32_t red = smem_u32(smem);
         const int share = N_TILE / s.split;
-        for (int i = threadIdx.x - 384; i < share * FEATURES; i += 256) {
+        for (int i = threadIdx.x - 32 * kTcEpilogueWarp; i < share * FEATURES; i += 256) {
             const int c = rank * share + i / FEATURES, f = i % FEATURES, feature = wt * FEATURES + f, token = tt * N_TILE + c;
             if (feature >= s.n_out || token >= s.T)
                 continue;
