@@ -52,13 +52,31 @@ __device__ __forceinline__ float w4_activation(float v, int act)
     return e < 1e37f ? __fdividef(v, e) : (v != v ? v : v * 0.0f);
 }
 
-// A bounded wait of a whole warp with one outcome.  One lane polls: a poll by 32 lanes is 32 operations on the barrier's word, and
-// waiting warps then slow down those that work.
+// A bounded wait of a whole warp with one outcome; one lane polls for all.
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag)
 {
     bool ok = true;
     if ((threadIdx.x & 31) == 0)
         ok = mbar_wait(bar, parity, abort_flag);
+    return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+}
+// The same for waits that are long by nature: sleeps between polls, so that the warp takes no issue slots from those that work.
+// Gives up after about a quarter of a second.
+__device__ __forceinline__ bool warp_sleep_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag)
+{
+    bool ok = true;
+    if ((threadIdx.x & 31) == 0) {
+        ok = false;
+        for (uint32_t i = 0; i < (1u << 21); i++) {
+            if (mbar_test_wait(bar, parity)) {
+                ok = true;
+                break;
+            }
+            if (*abort_flag)
+                break;
+            __nanosleep(128);
+        }
+    }
     return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
 }
 __device__ __forceinline__ uint4 lds128(uint32_t a)

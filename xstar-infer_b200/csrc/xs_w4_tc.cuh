@@ -226,7 +226,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                 if ((n & 1) != (warp == 3 ? 1u : 0u))
                     continue;
                 const uint32_t st = n % kTcStages;
-                if (!mbar_spin_wait(&empty[st], ((n / kTcStages) & 1) ^ 1, abort_flag)) {
+                if (!mbar_wait(&empty[st], ((n / kTcStages) & 1) ^ 1, abort_flag)) {
                     ok = false;
                     break;
                 }
@@ -244,7 +244,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
             tc_tile(s, item, wt, tt);
             for (int r = raw0; r < raw1; r++, n++) {
                 const uint32_t st = n % RAW;
-                if (!mbar_spin_wait(&raw_empty[st], ((n / RAW) & 1) ^ 1, abort_flag)) {
+                if (!mbar_wait(&raw_empty[st], ((n / RAW) & 1) ^ 1, abort_flag)) {
                     ok = false;
                     break;
                 }
@@ -292,31 +292,34 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
         const int raw_row = GATED ? (lane >> 4) * 64 + q * 16 + (lane & 15) : q * 32 + lane;
         const int feature = GATED ? q * 16 + (lane & 15) : raw_row;
         const uint32_t raw_addr = smem_u32(smem) + raw_row * 128, swz = (raw_row & 7) << 4;
-        const int groups = s.K >> s.G_log;
+        const int groups = s.K >> s.G_log, seg_log = s.G_log - 5; // loads of codes in a segment: 2^seg_log
         const bool vec = groups % 8 == 0 && reinterpret_cast<uintptr_t>(w.scales) % 16 == 0 && reinterpret_cast<uintptr_t>(w.zeros) % 8 == 0;
+        const bool zeros = w.zeros != nullptr;
         // Scales and zero points of this row, eight groups (a segment) at a time, loaded two segments ahead.  A segment begins
         // where a load of codes does.
         struct Segment {
             uint4 s;
             uint2 z;
         };
-        const int seg_log = s.G_log - 5; // loads of codes in a segment
         const int seg0 = raw0 >> seg_log, seg1 = (raw1 - 1) >> seg_log;
         int ld_item = item0, ld_seg = seg0;
+        size_t ld_at = 0; // element of the scales
+        auto ld_start = [&]() {
+            int wt, tt;
+            tc_tile(s, ld_item, wt, tt);
+            const int f = min(wt * FEATURES * CG + block_feature + feature, s.n_out - 1);
+            ld_at = (static_cast<size_t>(f) + (GATED && lane >= 16 ? s.n_out : 0)) * groups + seg0 * 8;
+        };
         auto load_segment = [&]() {
             Segment r;
             r.s = make_uint4(0, 0, 0, 0);
-            r.z = make_uint2(0x08080808u, 0x08080808u);
+            r.z = make_uint2(0, 0);
             if (ld_item < items) {
-                int wt, tt;
-                tc_tile(s, ld_item, wt, tt);
-                const int f = min(wt * FEATURES * CG + block_feature + feature, s.n_out - 1);
-                const size_t o = (static_cast<size_t>(f) + (GATED && lane >= 16 ? s.n_out : 0)) * groups + ld_seg * 8;
-                const uint16_t *sp = reinterpret_cast<const uint16_t *>(w.scales) + o;
+                const uint16_t *sp = reinterpret_cast<const uint16_t *>(w.scales) + ld_at;
                 if (vec) {
                     r.s = __ldg(reinterpret_cast<const uint4 *>(sp));
-                    if (w.zeros)
-                        r.z = __ldg(reinterpret_cast<const uint2 *>(w.zeros + o));
+                    if (zeros)
+                        r.z = __ldg(reinterpret_cast<const uint2 *>(w.zeros + ld_at));
                 } else {
                     const int have = groups - ld_seg * 8;
                     uint32_t sv[4] = {}, zv[2] = {};
@@ -325,27 +328,37 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                         if (i < have)
                             sv[i / 2] |= static_cast<uint32_t>(__ldg(sp + i)) << (i % 2 * 16);
                     r.s = make_uint4(sv[0], sv[1], sv[2], sv[3]);
-                    if (w.zeros) {
+                    if (zeros) {
 #pragma unroll
                         for (int i = 0; i < 8; i++)
                             if (i < have)
-                                zv[i / 4] |= static_cast<uint32_t>(__ldg(w.zeros + o + i)) << (i % 4 * 8);
+                                zv[i / 4] |= static_cast<uint32_t>(__ldg(w.zeros + ld_at + i)) << (i % 4 * 8);
                         r.z = make_uint2(zv[0], zv[1]);
                     }
                 }
+                ld_at += 8;
                 if (++ld_seg > seg1) {
                     ld_seg = seg0;
                     ld_item += item_step;
+                    if (ld_item < items)
+                        ld_start();
                 }
             }
             return r;
         };
+        if (ld_item < items)
+            ld_start();
         Segment cur, next, after;
 #pragma unroll 1
         for (int i = 0; i < 2; i++) {
             next = after;
             after = load_segment();
         }
+        // Group of this warp's 32-column steps h = 0, 1 of load r, inside its segment: with 32-column groups odd * 4 + group * 2 + h,
+        // with 64 (r % 2) * 4 + odd * 2 + group, with 128 (r % 4) * 2 + odd.
+        const uint32_t pick0 = seg_log == 0 ? 0x1010u : (seg_log == 1 ? group : odd) ? 0x3232u : 0x1010u; // its 16 bits of a pair
+        const uint32_t pick1 = seg_log == 0 ? 0x3232u : pick0;
+        const uint32_t codes0 = raw_addr + ((((odd * 4 + group * 2) << 4)) ^ swz), codes1 = raw_addr + ((((odd * 4 + group * 2 + 1) << 4)) ^ swz);
         const uint32_t dst0 = tmem + (static_cast<uint32_t>(q * 32) << 16) + group * 32;
         uint32_t rs = 0, rph = 0, n = 0; // n: operand blocks before this item
         bool raw_there = mbar_test_wait(&raw_full[0], 0);
@@ -366,16 +379,21 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                 if (kb < kb1) {
                     const uint32_t block = n + kb - kb0, st = block % kTcStages, free = ((block / kTcStages) & 1) ^ 1;
                     const bool is_free = mbar_test_wait(&empty[st], free); // asked early, its answer is there after the arithmetic
+                    const int pair = seg_log == 0 ? odd * 2 + group : seg_log == 1 ? (r & 1) * 2 + odd : r & 3;
+                    const uint32_t two = pair & 2 ? (pair & 1 ? cur.s.w : cur.s.z) : (pair & 1 ? cur.s.y : cur.s.x);
+                    const int k0 = kb * kTcBlockK + group * 64;
+                    uint32_t mz[2] = {kW4Minus8, kW4Minus8};
+                    if (zeros) {
+                        const uint32_t z = (pair & 2 ? cur.z.y : cur.z.x) >> (pair & 1) * 16; // the pair's two bytes
+                        mz[0] = w4_minus_zero((pick0 & 2 ? z >> 8 : z) & 15u);
+                        mz[1] = w4_minus_zero((pick1 & 2 ? z >> 8 : z) & 15u);
+                    }
 #pragma unroll
                     for (int h = 0; h < 2; h++) { // 32 columns: one 16-byte piece of codes, one group
-                        const int piece = odd * 4 + group * 2 + h, half = r * 8 + piece;
-                        const int i = (half >> seg_log) & 7;
-                        uint32_t sv = i & 4 ? (i & 2 ? cur.s.w : cur.s.z) : (i & 2 ? cur.s.y : cur.s.x);
-                        sv = __byte_perm(sv, 0, i & 1 ? 0x3232 : 0x1010);
-                        if (half * 32 >= s.K)
+                        uint32_t sv = __byte_perm(two, 0, h ? pick1 : pick0);
+                        if (k0 + h * 32 >= s.K)
                             sv = 0; // past the end: the codes read as zero, and so must the weight, whatever the zero point
-                        const uint32_t mz = w4_minus_zero(((i & 4 ? cur.z.y : cur.z.x) >> (i & 3) * 8) & 15u);
-                        const uint4 qv = lds128(raw_addr + rs * kTcRawBytes + ((piece << 4) ^ swz));
+                        const uint4 qv = lds128((h ? codes1 : codes0) + rs * kTcRawBytes);
                         const uint32_t words[4] = {qv.x, qv.y, qv.z, qv.w};
                         uint32_t a[16];
 #pragma unroll
@@ -384,7 +402,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                             for (int c = 0; c < 4; c++) {
                                 // byte c in both halves: its low nibble stays in the first, its high nibble in the second
                                 const uint32_t v = __byte_perm(words[j], 0, 0x4040 | c << 8 | c) & 0x00f0000fu;
-                                a[j * 4 + c] = bf16x2_mul(w4_fma(v, 0x7d007f00u, mz), sv); // times 2^127 and 2^123
+                                a[j * 4 + c] = bf16x2_mul(w4_fma(v, 0x7d007f00u, mz[h]), sv); // times 2^127 and 2^123
                             }
                         if (h == 0) {
                             ok = __all_sync(0xffffffffu, is_free || mbar_spin_wait(&empty[st], free, abort_flag));
@@ -421,7 +439,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
             int wt, tt;
             tc_tile(s, item, wt, tt);
             const uint32_t buf = use % NBUF;
-            if (!warp_wait(&acc_full[buf], (use / NBUF) & 1, abort_flag)) {
+            if (!warp_sleep_wait(&acc_full[buf], (use / NBUF) & 1, abort_flag)) {
                 ok = false;
                 break;
             }
