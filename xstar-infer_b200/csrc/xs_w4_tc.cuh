@@ -1,10 +1,10 @@
 // Products with 4-bit weights on the tensor core, for batches from nine tokens up: out = x W^T (or act(x Wg^T) * (x Wu^T)).
 //
 // tcgen05.mma with the WEIGHTS as its M rows, taken from TMEM, and the tokens as its N columns, taken from shared memory.  The codes
-// arrive by TMA as they lie in memory; eight warps turn them into bf16, thread = weight row, and store them with tcgen05.st
+// arrive by TMA as they lie in memory; sixteen warps turn them into bf16, thread = weight row, and store them with tcgen05.st
 // straight into TMEM columns, so a dequantised weight never passes through shared memory, whose bandwidth the tokens need.
-// Weights in TMEM also make the group scale a scalar of the thread.  (q - z) / 64 is exact in bf16 (w4 unpacking below); times s it is
-// rounded once, half a bf16 step: the price of the tensor core, whose operands have one type.  Sums are f32 in TMEM.
+// Weights in TMEM also make the group scale a scalar of the thread.  (q - z) s is rounded to bf16 once, half a step: the price of
+// the tensor core, whose operands have one type.  Sums are f32 in TMEM, scaled by 2^-10.
 //
 // CG = 2 pairs two SMs on a 256 x 256 tile (cta_group::2): each dequantises its 128 rows and loads its 128 tokens, so the
 // traffic out of L2 and the dequantisation per product halve against two 128 x 256 tiles.  CG = 1 serves smaller batches, where
@@ -12,8 +12,8 @@
 // distributed shared memory when there are too few tiles for the SMs.
 //
 // Warps: 0, 3 token loads, alternate blocks (3 owns the TMEM allocation) | 1 MMA | 2 code loads | 4..19 dequantisation (four
-// warpgroups: two on the even operand blocks and two on the odd ones, each on half of the block's columns; lane quarter =
-// warp % 4) | 20..27 epilogue (lane quarter = warp % 4, half of the token columns each).
+// warpgroups, every fourth operand block each, lane quarter = warp % 4) | 20..27 epilogue (lane quarter = warp % 4, half of the
+// token columns each).
 //
 // An operand block is 128 columns because every hand-over costs its roles a few hundred cycles (a poll of a barrier about 110, a
 // parked wait about 300, an expect or a load 100 each): with 64 columns one loading thread took 600 cycles a block, whatever the
@@ -38,6 +38,8 @@ constexpr int kTcRawBytes = kTcRows * 128;
 constexpr int kTcStages = 4;       // operand blocks in flight: TMEM columns of weights, shared memory of tokens
 constexpr int kTcAccCol = kTcStages * (kTcBlockK / 2);
 
+constexpr float kTcUnit = 1024.0f; // the sums are 2^-10 of the products
+
 __host__ __device__ constexpr int tc_x_bytes(int cg, int n_tile)
 {
     return n_tile / cg * kTcBlockK * 2;
@@ -45,7 +47,7 @@ __host__ __device__ constexpr int tc_x_bytes(int cg, int n_tile)
 // loads of codes in flight: what the tokens leave of shared memory
 __host__ __device__ constexpr int tc_raw_stages(int cg, int n_tile)
 {
-    return n_tile / cg >= 128 ? 5 : 8;
+    return n_tile / cg >= 128 ? 4 : 8;
 }
 __host__ __device__ constexpr int tc_smem_bytes(int cg, int n_tile)
 {
@@ -121,11 +123,32 @@ __device__ __forceinline__ void tmem_st_wait()
 {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel)
+{
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
+    return r;
+}
+// Byte c of a word of codes as a pair: its low nibble (the even column) in the first half, sixteen times its high nibble in the
+// second.  The upper byte of each half is the sign of a low nibble's byte, replicated: zero.
+__device__ __forceinline__ uint32_t w4_pair(uint32_t word, int c)
+{
+    const uint32_t low = word & 0x0f0f0f0fu, high = word & 0xf0f0f0f0u;
+    return prmt(low, high, c | (8 | c) << 4 | (4 + c) << 8 | (8 | c) << 12);
+}
 __device__ __forceinline__ uint32_t bf16x2_mul(uint32_t a, uint32_t b)
 {
     uint32_t r;
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
+}
+
+// Barrier 1 among the eight epilogue warps; the conjunction of their predicates.
+__device__ __forceinline__ bool named_barrier_and(bool ok)
+{
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"(ok ? 1u : 0u) : "memory");
+    return r != 0;
 }
 
 struct TcShape {
@@ -171,10 +194,10 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
     if (threadIdx.x == 0) {
         for (int i = 0; i < RAW; i++) {
             mbar_init(&raw_full[i], 1);
-            mbar_init(&raw_empty[i], kTcDequantWarps);
+            mbar_init(&raw_empty[i], 8); // two blocks, four warps each
         }
         for (int i = 0; i < kTcStages; i++) {
-            mbar_init(&full[i], 8 * CG + 1); // the dequantising warps, and the token load with its bytes
+            mbar_init(&full[i], 4 * CG + 1); // the dequantising warps, and the token load with its bytes
             mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < NBUF; i++) {
@@ -287,58 +310,58 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                 tc_done<CG>(&acc_full[buf]);
         }
     } else if (warp >= 4 && warp < kTcEpilogueWarp) {
-        const int group = ((warp - 4) >> 2) & 1, odd = (warp - 4) >> 3, q = warp & 3; // half of the block, which block of a load
+        const int wg = (warp - 4) >> 2, q = warp & 3; // this warpgroup's operand blocks: kb % 4 == wg
         // the row of the codes (as the load laid them out) that this thread's TMEM lane holds; GATED: 16 gate rows, then their 16 up rows
         const int raw_row = GATED ? (lane >> 4) * 64 + q * 16 + (lane & 15) : q * 32 + lane;
         const int feature = GATED ? q * 16 + (lane & 15) : raw_row;
         const uint32_t raw_addr = smem_u32(smem) + raw_row * 128, swz = (raw_row & 7) << 4;
-        const int groups = s.K >> s.G_log, seg_log = s.G_log - 5; // loads of codes in a segment: 2^seg_log
-        const bool vec = groups % 8 == 0 && reinterpret_cast<uintptr_t>(w.scales) % 16 == 0 && reinterpret_cast<uintptr_t>(w.zeros) % 8 == 0;
+        // Groups of a block (4, 2 or 1) with their scales and zero points, loaded two of this warpgroup's blocks ahead.
+        const int groups = s.K >> s.G_log, per_block = 1 << (7 - s.G_log);
+        const bool vec = groups % per_block == 0 && reinterpret_cast<uintptr_t>(w.scales) % (2 * per_block) == 0 &&
+                         reinterpret_cast<uintptr_t>(w.zeros) % per_block == 0;
         const bool zeros = w.zeros != nullptr;
-        // Scales and zero points of this row, eight groups (a segment) at a time, loaded two segments ahead.  A segment begins
-        // where a load of codes does.
-        struct Segment {
-            uint4 s;
-            uint2 z;
+        const int first = kb0 + ((wg - kb0) & 3);
+        struct Scales {
+            uint2 s;    // 16 bits each
+            uint32_t z; // 8 bits each
         };
-        const int seg0 = raw0 >> seg_log, seg1 = (raw1 - 1) >> seg_log;
-        int ld_item = item0, ld_seg = seg0;
-        size_t ld_at = 0; // element of the scales
+        int ld_item = first < kb1 ? item0 : items, ld_kb = first;
+        size_t ld_row = 0; // first group of the row
         auto ld_start = [&]() {
             int wt, tt;
             tc_tile(s, ld_item, wt, tt);
             const int f = min(wt * FEATURES * CG + block_feature + feature, s.n_out - 1);
-            ld_at = (static_cast<size_t>(f) + (GATED && lane >= 16 ? s.n_out : 0)) * groups + seg0 * 8;
+            ld_row = (static_cast<size_t>(f) + (GATED && lane >= 16 ? s.n_out : 0)) * groups;
         };
-        auto load_segment = [&]() {
-            Segment r;
-            r.s = make_uint4(0, 0, 0, 0);
-            r.z = make_uint2(0, 0);
+        auto load_scales = [&]() {
+            Scales r;
+            r.s = make_uint2(0, 0);
+            r.z = 0;
             if (ld_item < items) {
-                const uint16_t *sp = reinterpret_cast<const uint16_t *>(w.scales) + ld_at;
+                const int g0 = ld_kb * per_block;
+                const uint16_t *sp = reinterpret_cast<const uint16_t *>(w.scales) + ld_row + g0;
+                const uint8_t *zp = w.zeros + ld_row + g0;
                 if (vec) {
-                    r.s = __ldg(reinterpret_cast<const uint4 *>(sp));
+                    if (per_block == 4)
+                        r.s = __ldg(reinterpret_cast<const uint2 *>(sp));
+                    else if (per_block == 2)
+                        r.s.x = __ldg(reinterpret_cast<const uint32_t *>(sp));
+                    else
+                        r.s.x = __ldg(sp);
                     if (zeros)
-                        r.z = __ldg(reinterpret_cast<const uint2 *>(w.zeros + ld_at));
+                        r.z = per_block == 4 ? __ldg(reinterpret_cast<const uint32_t *>(zp)) : per_block == 2 ? __ldg(reinterpret_cast<const uint16_t *>(zp)) : __ldg(zp);
                 } else {
-                    const int have = groups - ld_seg * 8;
-                    uint32_t sv[4] = {}, zv[2] = {};
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (i < have)
-                            sv[i / 2] |= static_cast<uint32_t>(__ldg(sp + i)) << (i % 2 * 16);
-                    r.s = make_uint4(sv[0], sv[1], sv[2], sv[3]);
-                    if (zeros) {
-#pragma unroll
-                        for (int i = 0; i < 8; i++)
-                            if (i < have)
-                                zv[i / 4] |= static_cast<uint32_t>(__ldg(w.zeros + ld_at + i)) << (i % 4 * 8);
-                        r.z = make_uint2(zv[0], zv[1]);
-                    }
+                    for (int i = 0; i < 4; i++)
+                        if (i < per_block && g0 + i < groups) {
+                            (i < 2 ? r.s.x : r.s.y) |= static_cast<uint32_t>(__ldg(sp + i)) << (i % 2 * 16);
+                            if (zeros)
+                                r.z |= static_cast<uint32_t>(__ldg(zp + i)) << (i * 8);
+                        }
                 }
-                ld_at += 8;
-                if (++ld_seg > seg1) {
-                    ld_seg = seg0;
+                ld_kb += 4;
+                if (ld_kb >= kb1) {
+                    ld_kb = first;
                     ld_item += item_step;
                     if (ld_item < items)
                         ld_start();
@@ -348,86 +371,83 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
         };
         if (ld_item < items)
             ld_start();
-        Segment cur, next, after;
+        Scales cur, next, after;
 #pragma unroll 1
         for (int i = 0; i < 2; i++) {
             next = after;
-            after = load_segment();
+            after = load_scales();
         }
-        // Group of this warp's 32-column steps h = 0, 1 of load r, inside its segment: with 32-column groups odd * 4 + group * 2 + h,
-        // with 64 (r % 2) * 4 + odd * 2 + group, with 128 (r % 4) * 2 + odd.
-        const uint32_t pick0 = seg_log == 0 ? 0x1010u : (seg_log == 1 ? group : odd) ? 0x3232u : 0x1010u; // its 16 bits of a pair
-        const uint32_t pick1 = seg_log == 0 ? 0x3232u : pick0;
-        const uint32_t codes0 = raw_addr + ((((odd * 4 + group * 2) << 4)) ^ swz), codes1 = raw_addr + ((((odd * 4 + group * 2 + 1) << 4)) ^ swz);
-        const uint32_t dst0 = tmem + (static_cast<uint32_t>(q * 32) << 16) + group * 32;
-        uint32_t rs = 0, rph = 0, n = 0; // n: operand blocks before this item
-        bool raw_there = mbar_test_wait(&raw_full[0], 0);
-        for (int item = item0; item < items && ok; item += item_step, n += n_kb) {
-            int seg = -1;
-            for (int r = raw0; r < raw1; r++) {
-                if (r >> seg_log != seg) {
-                    seg = r >> seg_log;
-                    cur = next;
-                    next = after;
-                    after = load_segment();
-                }
-                if (!__all_sync(0xffffffffu, raw_there || mbar_spin_wait(&raw_full[rs], rph, abort_flag))) {
-                    ok = false;
-                    break;
-                }
-                const int kb = r * kTcRawBlocks + odd;
+        const uint32_t tmem_lane = tmem + (static_cast<uint32_t>(q * 32) << 16);
+        uint32_t n = 0, nr = 0; // operand blocks and loads of codes before this item
+        for (int item = item0; item < items && ok; item += item_step, n += n_kb, nr += raw1 - raw0) {
+            // up to the last load's second block, which may not be there: its codes are given back all the same
+            for (int kb = first; kb < raw1 * kTcRawBlocks; kb += 4) {
+                const uint32_t rc = nr + (kb >> 1) - raw0, rs = rc % RAW;
+                const bool raw_there = mbar_test_wait(&raw_full[rs], (rc / RAW) & 1);
                 if (kb < kb1) {
                     const uint32_t block = n + kb - kb0, st = block % kTcStages, free = ((block / kTcStages) & 1) ^ 1;
                     const bool is_free = mbar_test_wait(&empty[st], free); // asked early, its answer is there after the arithmetic
-                    const int pair = seg_log == 0 ? odd * 2 + group : seg_log == 1 ? (r & 1) * 2 + odd : r & 3;
-                    const uint32_t two = pair & 2 ? (pair & 1 ? cur.s.w : cur.s.z) : (pair & 1 ? cur.s.y : cur.s.x);
-                    const int k0 = kb * kTcBlockK + group * 64;
-                    uint32_t mz[2] = {kW4Minus8, kW4Minus8};
-                    if (zeros) {
-                        const uint32_t z = (pair & 2 ? cur.z.y : cur.z.x) >> (pair & 1) * 16; // the pair's two bytes
-                        mz[0] = w4_minus_zero((pick0 & 2 ? z >> 8 : z) & 15u);
-                        mz[1] = w4_minus_zero((pick1 & 2 ? z >> 8 : z) & 15u);
+                    cur = next;
+                    next = after;
+                    after = load_scales();
+                    // A scale below 32 and the zero point 8 need one multiply-add: s 2^123 is finite and 8 s exact, so the
+                    // difference is rounded once; else (q - z) / 64 is made first, exactly, and multiplied by s / 16.
+                    const bool one_step =
+                        !zeros && __all_sync(0xffffffffu, ((((cur.s.x & 0x7fff7fffu) + 0x3e003e00u) | ((cur.s.y & 0x7fff7fffu) + 0x3e003e00u)) & 0x80008000u) == 0);
+                    if (!__all_sync(0xffffffffu, raw_there || mbar_wait(&raw_full[rs], (rc / RAW) & 1, abort_flag))) {
+                        ok = false;
+                        break;
                     }
+                    const uint32_t codes = raw_addr + rs * kTcRawBytes, dst = tmem_lane + st * (kTcBlockK / 2);
 #pragma unroll
-                    for (int h = 0; h < 2; h++) { // 32 columns: one 16-byte piece of codes, one group
-                        uint32_t sv = __byte_perm(two, 0, h ? pick1 : pick0);
-                        if (k0 + h * 32 >= s.K)
+                    for (int h = 0; h < 4; h++) { // 32 columns: one 16-byte piece of codes, one group
+                        const int e = (h * per_block) >> 2;
+                        uint32_t sv = prmt(cur.s.x, cur.s.y, 0x1010u + 0x2222u * e);
+                        if (kb * kTcBlockK + h * 32 >= s.K)
                             sv = 0; // past the end: the codes read as zero, and so must the weight, whatever the zero point
-                        const uint4 qv = lds128((h ? codes1 : codes0) + rs * kTcRawBytes);
+                        const uint4 qv = lds128(codes + ((((kb & 1) * 4 + h) << 4) ^ swz));
                         const uint32_t words[4] = {qv.x, qv.y, qv.z, qv.w};
                         uint32_t a[16];
+                        if (one_step) {
+                            const uint32_t mul = bf16x2_mul(sv, 0x7b007d00u), add = bf16x2_mul(sv, 0xbc00bc00u); // 2^119 2^123, -2^-7
 #pragma unroll
-                        for (int j = 0; j < 4; j++)
+                            for (int j = 0; j < 4; j++)
 #pragma unroll
-                            for (int c = 0; c < 4; c++) {
-                                // byte c in both halves: its low nibble stays in the first, its high nibble in the second
-                                const uint32_t v = __byte_perm(words[j], 0, 0x4040 | c << 8 | c) & 0x00f0000fu;
-                                a[j * 4 + c] = bf16x2_mul(w4_fma(v, 0x7d007f00u, mz[h]), sv); // times 2^127 and 2^123
-                            }
+                                for (int c = 0; c < 4; c++)
+                                    a[j * 4 + c] = w4_fma(w4_pair(words[j], c), mul, add);
+                        } else {
+                            const uint32_t mz = zeros ? w4_minus_zero((cur.z >> (8 * e)) & 15u) : kW4Minus8, ms = bf16x2_mul(sv, 0x3d803d80u); // 2^-4
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+#pragma unroll
+                                for (int c = 0; c < 4; c++)
+                                    a[j * 4 + c] = bf16x2_mul(w4_fma(w4_pair(words[j], c), 0x7d007f00u, mz), ms); // 2^123 2^127
+                        }
                         if (h == 0) {
-                            ok = __all_sync(0xffffffffu, is_free || mbar_spin_wait(&empty[st], free, abort_flag));
+                            ok = __all_sync(0xffffffffu, is_free || mbar_wait(&empty[st], free, abort_flag));
                             if (!ok)
                                 break;
                             tc_fence_after();
                         }
-                        tmem_st16(dst0 + st * (kTcBlockK / 2) + h * 16, a);
+                        tmem_st16(dst + h * 16, a);
                     }
                     if (!ok)
                         break;
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0)
+                    if (lane == 0) {
                         tc_arrive_leader<CG>(&full[st]);
+                        mbar_arrive(&raw_empty[rs]);
+                    }
+                } else {
+                    if (!__all_sync(0xffffffffu, raw_there || mbar_wait(&raw_full[rs], (rc / RAW) & 1, abort_flag))) {
+                        ok = false;
+                        break;
+                    }
+                    if (lane == 0)
+                        mbar_arrive(&raw_empty[rs]);
                 }
-                __syncwarp();
-                if (lane == 0)
-                    mbar_arrive(&raw_empty[rs]);
-                if (++rs == RAW) {
-                    rs = 0;
-                    rph ^= 1;
-                }
-                raw_there = mbar_test_wait(&raw_full[rs], rph);
             }
         }
     } else if (warp >= kTcEpilogueWarp) {
@@ -439,7 +459,10 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
             int wt, tt;
             tc_tile(s, item, wt, tt);
             const uint32_t buf = use % NBUF;
-            if (!warp_sleep_wait(&acc_full[buf], (use / NBUF) & 1, abort_flag)) {
+            // one warp asks, sleeping in between, and the others wait at a barrier that costs no issue slots
+            if (warp == kTcEpilogueWarp)
+                ok = warp_sleep_wait(&acc_full[buf], (use / NBUF) & 1, abort_flag);
+            if (!named_barrier_and(ok)) {
                 ok = false;
                 break;
             }
@@ -478,7 +501,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
                         const float give = __uint_as_float(up ? v[i] : v[i + 1]), got = __shfl_xor_sync(0xffffffffu, give, 16);
-                        const float g = kW4Unit * (up ? got : __uint_as_float(v[i])), u = kW4Unit * (up ? __uint_as_float(v[i + 1]) : got);
+                        const float g = kTcUnit * (up ? got : __uint_as_float(v[i])), u = kTcUnit * (up ? __uint_as_float(v[i + 1]) : got);
                         const int t = i + (up ? 1 : 0);
                         if (feature < s.n_out && token0 + c + t < s.T)
                             o[static_cast<size_t>(t) * s.n_out] = __float2bfloat16_rn(w4_activation(g, act) * u);
@@ -487,7 +510,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
 #pragma unroll
                     for (int i = 0; i < 16; i++)
                         if (feature < s.n_out && token0 + c + i < s.T)
-                            o[static_cast<size_t>(i) * s.n_out] = __float2bfloat16_rn(kW4Unit * __uint_as_float(v[i]));
+                            o[static_cast<size_t>(i) * s.n_out] = __float2bfloat16_rn(kTcUnit * __uint_as_float(v[i]));
                 }
             }
         }
@@ -516,7 +539,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                 if (GATED)
                     u += ld_cluster_f32(red + (c * kTcRows + row + 16) * 4, r);
             }
-            out[static_cast<size_t>(token) * s.n_out + feature] = __float2bfloat16_rn(GATED ? w4_activation(kW4Unit * v, act) * (kW4Unit * u) : kW4Unit * v);
+            out[static_cast<size_t>(token) * s.n_out + feature] = __float2bfloat16_rn(GATED ? w4_activation(kTcUnit * v, act) * (kTcUnit * u) : kTcUnit * v);
         }
     }
     if (*abort_flag)
