@@ -327,8 +327,58 @@ int launch_w4(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void 
     return gated ? launch_tc<true>(w, xb, T, ob, act, di.sms, status, st) : launch_tc<false>(w, xb, T, ob, act, di.sms, status, st);
 }
 
+template <int GROUP, int ITER, bool ALIGNED>
+int launch_norm_t(const xs::NormResidualArgs &a, int sms, cudaStream_t st)
+{
+    constexpr int threads = GROUP < 256 ? 256 : GROUP, per_block = threads / GROUP;
+    const int blocks = (a.rows + per_block - 1) / per_block, slots = sms * (2048 / threads);
+    XS_CUDA(launch_pdl(xs::norm_residual_kernel<GROUP, ITER, ALIGNED>, blocks < slots ? blocks : slots, threads, 0, st, a));
+    note_launch();
+    return 0;
+}
+
+template <bool ALIGNED>
+int launch_norm_rows(const xs::NormResidualArgs &a, int sms, cudaStream_t st)
+{
+    const int pieces = (a.H + 7) / 8 + (ALIGNED ? 0 : 1); // an unaligned row may touch one more
+    if (pieces <= 32)
+        return launch_norm_t<32, 1, ALIGNED>(a, sms, st);
+    if (pieces <= 64)
+        return launch_norm_t<32, 2, ALIGNED>(a, sms, st);
+    if (pieces <= 128)
+        return launch_norm_t<128, 1, ALIGNED>(a, sms, st);
+    // few rows: as many threads as the row has pieces, since only latency counts; many rows: more work a thread and more
+    // blocks on an SM, which hide one another's sums
+    if (a.rows <= 2 * sms) {
+        if (pieces <= 256)
+            return launch_norm_t<256, 1, ALIGNED>(a, sms, st);
+        if (pieces <= 512)
+            return launch_norm_t<512, 1, ALIGNED>(a, sms, st);
+        if (pieces <= 1024)
+            return launch_norm_t<1024, 1, ALIGNED>(a, sms, st);
+    }
+    if (pieces <= 256)
+        return launch_norm_t<256, 1, ALIGNED>(a, sms, st);
+    if (pieces <= 512)
+        return launch_norm_t<256, 2, ALIGNED>(a, sms, st);
+    if (pieces <= 1024)
+        return launch_norm_t<512, 2, ALIGNED>(a, sms, st);
+    return launch_norm_t<1024, 2, ALIGNED>(a, sms, st);
+}
+
 int launch_norm_residual(const xs::NormResidualArgs &a, cudaStream_t st)
 {
+    DeviceInfo di;
+    if (int rc = device_info(&di))
+        return rc;
+    uintptr_t low = 0;
+    for (const void *p : {static_cast<const void *>(a.y), static_cast<const void *>(a.r), static_cast<const void *>(a.w_post), static_cast<const void *>(a.gate),
+                          static_cast<const void *>(a.w_next), static_cast<const void *>(a.r_out), static_cast<const void *>(a.n_out)})
+        low |= reinterpret_cast<uintptr_t>(p);
+    if (low % 16 == 0 && a.H <= 16 * 1024 - 8)
+        return a.H % 8 == 0 ? launch_norm_rows<true>(a, di.sms, st) : launch_norm_rows<false>(a, di.sms, st);
+    if (low % 16 == 0 && a.H == 16 * 1024)
+        return launch_norm_rows<true>(a, di.sms, st);
     const size_t smem = static_cast<size_t>(a.H) * 4;
     if (smem > 48 * 1024)
         XS_CUDA(cudaFuncSetAttribute(xs::norm_residual_loop_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
