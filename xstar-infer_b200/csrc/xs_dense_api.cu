@@ -347,8 +347,8 @@ int launch_norm_rows(const xs::NormResidualArgs &a, int sms, cudaStream_t st)
         return launch_norm_t<32, 2, ALIGNED>(a, sms, st);
     if (pieces <= 128)
         return launch_norm_t<128, 1, ALIGNED>(a, sms, st);
-    // few rows: as many threads as the row has pieces, since only latency counts; many rows: more work a thread and more
-    // blocks on an SM, which hide one another's sums
+    // few rows: as many threads as the row has pieces, since only latency counts; many rows: two to four pieces a thread, by
+    // what leaves the fewest threads idle
     if (a.rows <= 2 * sms) {
         if (pieces <= 256)
             return launch_norm_t<256, 1, ALIGNED>(a, sms, st);
@@ -356,14 +356,21 @@ int launch_norm_rows(const xs::NormResidualArgs &a, int sms, cudaStream_t st)
             return launch_norm_t<512, 1, ALIGNED>(a, sms, st);
         if (pieces <= 1024)
             return launch_norm_t<1024, 1, ALIGNED>(a, sms, st);
+        return launch_norm_t<1024, 2, ALIGNED>(a, sms, st);
     }
     if (pieces <= 256)
-        return launch_norm_t<256, 1, ALIGNED>(a, sms, st);
+        return launch_norm_t<128, 2, ALIGNED>(a, sms, st);
+    if (pieces <= 384)
+        return launch_norm_t<128, 3, ALIGNED>(a, sms, st);
     if (pieces <= 512)
         return launch_norm_t<256, 2, ALIGNED>(a, sms, st);
+    if (pieces <= 768)
+        return launch_norm_t<256, 3, ALIGNED>(a, sms, st);
     if (pieces <= 1024)
         return launch_norm_t<512, 2, ALIGNED>(a, sms, st);
-    return launch_norm_t<1024, 2, ALIGNED>(a, sms, st);
+    if (pieces <= 1536)
+        return launch_norm_t<512, 3, ALIGNED>(a, sms, st);
+    return launch_norm_t<512, 4, ALIGNED>(a, sms, st);
 }
 
 int launch_norm_residual(const xs::NormResidualArgs &a, cudaStream_t st)

@@ -226,8 +226,7 @@ __global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP) norm_residual_kerne
             for (int k = 0; k < ITER; k++)
 #pragma unroll
                 for (int i = 0; i < 8; i++)
-                    if (ALIGNED || (i >= lo[k] && i < hi[k]))
-                        ss = fmaf(f[k][i], f[k][i], ss);
+                    ss = fmaf(f[k][i], f[k][i], ss); // what is not of this row was loaded as zero
             const float inv = rsqrtf(row_sum(ss) * inv_h + a.eps);
 #pragma unroll
             for (int k = 0; k < ITER; k++)
