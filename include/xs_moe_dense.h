@@ -41,7 +41,8 @@ typedef enum XsMoeActivation {
 } XsMoeActivation;
 
 /* out (tokens, rows) bf16 = x (tokens, cols) bf16 times W^T; f32 sums, one rounding at the end.  Up to 8 tokens the weights
- * enter the products exactly; larger batches round (q - z) * s to bf16 once for the tensor core (half a bf16 step per weight).
+ * enter the products exactly; larger batches go to the tensor core in f16, tokens and weight rows scaled by powers of two: a
+ * weight is rounded once to 11 bits, tokens are exact down to 2^-27 of their largest element.
  * x is 16-byte aligned and does not overlap out.  Takes the role of gemm_launch behind linear
  * (xstar_cpp/include/ops/gemm.h:165-176). */
 int xs_moe_linear_w4_workspace_bytes(const XsMoeW4 *w, int32_t tokens, size_t *bytes);
@@ -56,7 +57,7 @@ int xs_moe_gated_w4(const XsMoeW4 *gate_up, int32_t activation, const void *x_de
 
 /* out (tokens, H) bf16 = (act(x Wg^T) * (x Wu^T)) Wd^T, gate_up (2I, H), down (H, I): the reference's
  * mlp(x, gate_up_weight, down_weight) (xstar_cpp/include/ops/mlp.h:51) with 4-bit weights.  The product of the first half is
- * rounded to bf16 once, as everywhere in this library. */
+ * rounded once: to bf16 up to 8 tokens, beyond to f16, scaled by a power of two that a bound of the row gives. */
 int xs_moe_mlp_w4_workspace_bytes(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t tokens, size_t *bytes);
 int xs_moe_mlp_w4(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t activation, const void *x_dev, int32_t tokens,
                   void *out_dev, void *workspace_dev, size_t workspace_bytes, void *stream);

@@ -128,16 +128,24 @@ def ref_norm_residual(y, r, post=None, gate=None, nxt=None, eps=1e-6, scale=1.0,
 
 # ---- how far off ----------------------------------------------------------------------------------------------------
 # A sum of K products in f32, in any order, is off by at most K * 2^-23 * sum |product| (2^-23 a step: additions that cut off
-# instead of rounding).  A weight that was rounded to bf16 is off by HALF of itself, so its products are, too.
-def _sum_error(K, magnitude, tokens):
-    return (K * 2.0**-23 + (HALF if tokens > EXACT_WEIGHT_TOKENS else 0.0)) * magnitude
+# instead of rounding).  Beyond EXACT_WEIGHT_TOKENS the operands are f16: a weight is off by half a step, 2^-11 of itself, and a
+# token, scaled to a largest element of 2^13 at least, by 2^-25 in that unit: 2^-38 of its largest element.
+F16 = 2.0**-11
+
+
+def _sum_error(X, W, tokens):
+    magnitude = X.abs() @ W.abs().T
+    err = X.shape[1] * 2.0**-23 * magnitude
+    if tokens > EXACT_WEIGHT_TOKENS:
+        err = err + F16 * magnitude + 2.0**-38 * X.abs().amax(-1, keepdim=True) * W.abs().sum(-1)
+    return err
 
 
 def linear_reference(w, x):
     """out in 64 bits and the largest error of each of its elements"""
     W, X = matrix(w), x.to(F)
     ref = X @ W.T
-    err = _sum_error(W.shape[1], X.abs() @ W.abs().T, x.shape[0])
+    err = _sum_error(X, W, x.shape[0])
     return ref, HALF * ref.abs() + err * (1 + HALF) + 1e-37
 
 
@@ -146,7 +154,7 @@ def _gated(w, X, act, tokens, dx=None):
     W = matrix(w)
     I = W.shape[0] // 2
     gu = X @ W.T
-    err = _sum_error(W.shape[1], X.abs() @ W.abs().T, tokens)
+    err = _sum_error(X, W, tokens)
     if dx is not None:
         err = err + dx @ W.abs().T * (1 + HALF)
     g, u, dg, du = gu[:, :I], gu[:, I:], err[:, :I], err[:, I:]
@@ -164,10 +172,16 @@ def gated_reference(w, x, act):
 def mlp_reference(gu, dn, x, act, dx=None):
     X = x.to(F)
     h, dh = _gated(gu, X, act, x.shape[0], dx)
-    dh = HALF * h.abs() + dh * (1 + HALF)
+    if x.shape[0] > EXACT_WEIGHT_TOKENS:
+        # h in f16, scaled by a bound of its row: 2^15 of |x|^2 K max(s_gate s_up) at most, of which f16 keeps 2^-40
+        s = gu["s"].to(F).abs().amax(-1)
+        bound = 2.0**15 * X.square().sum(-1, keepdim=True) * X.shape[1] * (s[: h.shape[1]] * s[h.shape[1]:]).amax()
+        dh = F16 * h.abs() + 2.0**-40 * bound + dh * (1 + F16)
+    else:
+        dh = HALF * h.abs() + dh * (1 + HALF)
     D = matrix(dn)
     ref = h @ D.T
-    err = _sum_error(D.shape[1], (h.abs() + dh) @ D.abs().T, x.shape[0]) + dh @ D.abs().T
+    err = _sum_error(h.abs() + dh, D, x.shape[0]) + dh @ D.abs().T
     return ref, HALF * ref.abs() + err * (1 + HALF) + 1e-37
 
 

@@ -1,9 +1,9 @@
 """4-bit dense operators and the step between two blocks: refusals (no GPU needed) and results against 64-bit definitions.
 
 Tolerances: element by element from the roundings the operators are documented to make (dense_util), and in the norm: the
-roundings to bf16 (output, weights beyond 8 tokens, the gated product, the intermediate rows of a block) are off by at most
-half a step each, 2^-8, spread evenly, so each adds at most 2^-8 / sqrt(3) of the result in the root mean square, and no chain
-here has more than six: sqrt(6 / 3) * 2^-8 < 2^-7."""
+roundings to bf16 (output, the gated product, the intermediate rows of a block) are off by at most half a step each, 2^-8,
+spread evenly, so each adds at most 2^-8 / sqrt(3) of the result in the root mean square, and no chain here has more than six:
+sqrt(6 / 3) * 2^-8 < 2^-7."""
 import ctypes as C
 
 import pytest
@@ -302,8 +302,8 @@ def test_mlp_and_its_first_half_match_their_definitions(H, I, group, zeros, act)
         du.assert_close(out, ref, tol)
         assert du.rel_l2(out, ref) < L2
         assert (buf[T * H:] == 77.0).all()
-        # the whole is its two halves
-        assert torch.equal(out, du.linear(dn, h)[0])
+        if T <= du.EXACT_WEIGHT_TOKENS:  # the whole is its two halves; larger batches hand h on in f16
+            assert torch.equal(out, du.linear(dn, h)[0])
 
 
 @pytest.mark.gpu

@@ -3,6 +3,7 @@
 
 #include "xs_api_common.cuh"
 #include "xs_norm_residual.cuh"
+#include "xs_w4_prepare.cuh"
 #include "xs_w4_small.cuh"
 #include "xs_w4_tc.cuh"
 
@@ -224,7 +225,7 @@ int launch_small(const XsMoeW4 *w, bool gated, const __nv_bfloat16 *x, int T, __
                  : launch_small_t<false, SUB, false>(w, p, x, T, out, act, early, status, st);
 }
 
-// A batch of bf16 rows read in boxes of 64 columns x box_rows, 128-byte swizzle; past the end of rows and columns there are zeros.
+// A batch of f16 rows read in boxes of 64 columns x box_rows, 128-byte swizzle; past the end of rows and columns there are zeros.
 int make_tmap_rows(CUtensorMap *m, const void *x, int T, int K, uint32_t box_rows)
 {
     EncodeTiledFn fn = get_encode_fn();
@@ -232,7 +233,7 @@ int make_tmap_rows(CUtensorMap *m, const void *x, int T, int K, uint32_t box_row
         return fail(XS_MOE_ERR_CUDA, "CUDA error: cuTensorMapEncodeTiled entry point not available");
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(T)}, strides[1] = {static_cast<cuuint64_t>(K) * 2};
     const cuuint32_t box[2] = {64, box_rows}, one[2] = {1, 1};
-    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(x), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(x), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
         return fail(XS_MOE_ERR_CUDA, "CUDA error: cuTensorMapEncodeTiled failed with code %d (rows=%d cols=%d)", (int)r, T, K);
@@ -280,7 +281,7 @@ TcPlan plan_tc(const XsMoeW4 *w, bool gated, int T, int sms)
 }
 
 template <int CG, int N_TILE, bool GATED>
-int launch_tc_t(const XsMoeW4 *w, const TcPlan &p, const __nv_bfloat16 *x, __nv_bfloat16 *out, int act, int32_t *status, cudaStream_t st)
+int launch_tc_t(const XsMoeW4 *w, const TcPlan &p, const void *x16, void *out, const xs::TcOperands &ops, int act, int32_t *status, cudaStream_t st)
 {
     auto kern = xs::w4_tc_kernel<CG, N_TILE, GATED>;
     constexpr int smem = xs::tc_smem_bytes(CG, N_TILE);
@@ -288,43 +289,201 @@ int launch_tc_t(const XsMoeW4 *w, const TcPlan &p, const __nv_bfloat16 *x, __nv_
     CUtensorMap mw, mx;
     if (int rc = make_tmap_codes(&mw, w, GATED ? 2 : 1, GATED ? xs::kTcRows / 2 : xs::kTcRows))
         return rc;
-    if (int rc = make_tmap_rows(&mx, x, p.shape.T, p.shape.K, N_TILE / CG))
+    if (int rc = make_tmap_rows(&mx, x16, p.shape.T, p.shape.K, N_TILE / CG))
         return rc;
-    XS_CUDA(launch_pdl_cluster(kern, p.grid, xs::kTcThreads, CG * p.shape.split, smem, st, mw, mx, matrix_of(w), out, p.shape, act, status));
+    XS_CUDA(launch_pdl_cluster(kern, p.grid, xs::kTcThreads, CG * p.shape.split, smem, st, mw, mx, ops, out, p.shape, act, status));
     note_launch();
     return 0;
 }
 
 template <bool GATED>
-int launch_tc(const XsMoeW4 *w, const __nv_bfloat16 *x, int T, __nv_bfloat16 *out, int act, int sms, int32_t *status, cudaStream_t st)
-{
-    const TcPlan p = plan_tc(w, GATED, T, sms);
-    if (p.cg == 2)
-        return launch_tc_t<2, 256, GATED>(w, p, x, out, act, status, st);
-    if (p.n_tile == 128)
-        return launch_tc_t<1, 128, GATED>(w, p, x, out, act, status, st);
-    if (p.n_tile == 64)
-        return launch_tc_t<1, 64, GATED>(w, p, x, out, act, status, st);
-    return launch_tc_t<1, 32, GATED>(w, p, x, out, act, status, st);
-}
-
-// early: nothing that may still be running when the kernel starts writes the weights (the second product of one call)
-int launch_w4(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void *out, bool early, int32_t *status, cudaStream_t st)
+int launch_tc(const XsMoeW4 *w, const void *x16, int T, void *out, const xs::TcOperands &ops, int act, int32_t *status, cudaStream_t st)
 {
     DeviceInfo di;
     if (int rc = device_info(&di))
         return rc;
-    const int K = w->cols;
+    const TcPlan p = plan_tc(w, GATED, T, di.sms);
+    if (p.cg == 2)
+        return launch_tc_t<2, 256, GATED>(w, p, x16, out, ops, act, status, st);
+    if (p.n_tile == 128)
+        return launch_tc_t<1, 128, GATED>(w, p, x16, out, ops, act, status, st);
+    if (p.n_tile == 64)
+        return launch_tc_t<1, 64, GATED>(w, p, x16, out, ops, act, status, st);
+    return launch_tc_t<1, 32, GATED>(w, p, x16, out, ops, act, status, st);
+}
+
+// Which kernel: up to eight tokens the one that streams weights past the tokens, if a cluster's shared memory holds them.
+constexpr int kBlockSmem = 227 * 1024;
+bool small_batch(int T, int K)
+{
+    return T <= xs::kSwTokens && xs::sw_smem_bytes(T, ((K + xs::kSwChunk - 1) / xs::kSwChunk + 7) / 8, 2) <= kBlockSmem;
+}
+
+// Scratch of the tensor-core kernel: tokens and scales in f16, zero points, factors.
+struct TcScratch {
+    size_t x16 = 0, token = 0, l = 0, h_factor = 0, h_inverse = 0, part = 0, scales[2] = {}, zeros[2] = {}, row[2] = {}, bytes = 0;
+};
+constexpr size_t kOffTicket = 224; // status block: blocks of w4_prepare_kernel that are done (zero between calls)
+
+int groups_pitch(const XsMoeW4 *w)
+{
+    return (w->cols / w->group + 7) / 8 * 8;
+}
+
+TcScratch plan_scratch(const XsMoeW4 *first, const XsMoeW4 *second, int T, size_t at)
+{
+    TcScratch p;
+    auto take = [&](size_t bytes) {
+        const size_t o = at;
+        at = align_up(at + bytes, 256);
+        return o;
+    };
+    p.x16 = take(static_cast<size_t>(T) * first->cols * 2);
+    for (size_t *o : {&p.token, &p.l, &p.h_factor, &p.h_inverse})
+        *o = take(static_cast<size_t>(T) * 4);
+    p.part = take(static_cast<size_t>(first->rows) * 4);
+    const XsMoeW4 *w[2] = {first, second};
+    for (int i = 0; i < 2; i++) {
+        if (!w[i])
+            continue;
+        const size_t n = static_cast<size_t>(w[i]->rows) * groups_pitch(w[i]);
+        p.scales[i] = take(n * 2);
+        p.zeros[i] = take(w[i]->zeros_dev ? n : 0);
+        p.row[i] = take(static_cast<size_t>(w[i]->rows) * 4);
+    }
+    p.bytes = at;
+    return p;
+}
+
+// What a product of `cols` columns adds to the exponent of its bound: |g| |u| <= 2^(2 l) cols 2^(2 * 4) max s(gate) max s(up), brought
+// to 2^15 at most.
+int bound_exponent(int cols)
+{
+    int log = 0;
+    while ((1 << log) < cols)
+        log++;
+    return log + 8 - 15;
+}
+
+// Tokens (normed by `norm` where it is given) and the scales of up to two matrices.
+int launch_prepare(const XsMoeW4 *first, bool pair, const XsMoeW4 *second, const XsMoeBlockNorms *norm, const void *x, int T, uint8_t *ws,
+                   const TcScratch &p, cudaStream_t st)
+{
+    xs::PrepareArgs a{};
+    a.x = static_cast<const __nv_bfloat16 *>(x);
+    if (norm) {
+        a.norm_w = static_cast<const __nv_bfloat16 *>(norm->pre_weight_dev);
+        a.eps = norm->eps;
+        a.offset = norm->weight_offset;
+    }
+    a.x16 = reinterpret_cast<__half *>(ws + p.x16);
+    a.factor = reinterpret_cast<float *>(ws + p.token);
+    a.l = reinterpret_cast<int *>(ws + p.l);
+    a.T = T;
+    a.K = first->cols;
+    const XsMoeW4 *w[2] = {first, second};
+    int blocks = T;
+    for (int i = 0; i < 2; i++) {
+        if (!w[i])
+            continue;
+        xs::PrepareScales &m = a.m[i];
+        m.scales = static_cast<const uint16_t *>(w[i]->scales_dev);
+        m.zeros = w[i]->zeros_dev;
+        m.scales16 = reinterpret_cast<uint16_t *>(ws + p.scales[i]);
+        m.zeros8 = ws + p.zeros[i];
+        m.factor = reinterpret_cast<float *>(ws + p.row[i]);
+        m.rows = w[i]->rows;
+        m.groups = w[i]->cols / w[i]->group;
+        m.pitch = groups_pitch(w[i]);
+        m.vec = m.groups % 8 == 0 && !misaligned(m.scales, 16);
+        m.lanes = 1;
+        while (m.lanes < 32 && m.lanes * 8 < m.groups)
+            m.lanes *= 2;
+        const int at_once = xs::kPrepThreads / m.lanes;
+        m.per_block = at_once < xs::kPrepRows ? at_once : xs::kPrepRows;
+        const int rows = i == 0 && pair ? m.rows / 2 : m.rows, per = i == 0 && pair ? m.per_block / 2 : m.per_block;
+        m.blocks = (rows + per - 1) / per;
+        blocks += m.blocks;
+    }
+    a.pair = pair ? 1 : 0;
+    a.bound_add = bound_exponent(first->cols);
+    a.pair_part = reinterpret_cast<int *>(ws + p.part);
+    a.h_factor = reinterpret_cast<float *>(ws + p.h_factor);
+    a.h_inverse = reinterpret_cast<float *>(ws + p.h_inverse);
+    a.ticket = reinterpret_cast<unsigned int *>(ws + kOffTicket);
+    XS_CUDA(launch_pdl(xs::w4_prepare_kernel, blocks, xs::kPrepThreads, 0, st, a));
+    note_launch();
+    return 0;
+}
+
+xs::TcOperands operands(const XsMoeW4 *w, const uint8_t *ws, const TcScratch &p, int i, size_t token)
+{
+    xs::TcOperands o{};
+    o.scales = reinterpret_cast<const uint16_t *>(ws + p.scales[i]);
+    o.zeros = w->zeros_dev ? ws + p.zeros[i] : nullptr;
+    o.row = reinterpret_cast<const float *>(ws + p.row[i]);
+    o.token = reinterpret_cast<const float *>(ws + token);
+    o.pitch = groups_pitch(w);
+    return o;
+}
+
+// early: nothing that may still be running when the kernel starts writes the weights (the second product of one call)
+int run_small(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void *out, bool early, int32_t *status, cudaStream_t st)
+{
+    DeviceInfo di;
+    if (int rc = device_info(&di))
+        return rc;
     const __nv_bfloat16 *xb = static_cast<const __nv_bfloat16 *>(x);
     __nv_bfloat16 *ob = static_cast<__nv_bfloat16 *>(out);
-    if (T <= xs::kSwTokens && xs::sw_smem_bytes(T, ((K + xs::kSwChunk - 1) / xs::kSwChunk + 7) / 8, 2) <= di.max_smem) {
-        if (w->group == 32)
-            return launch_small<1>(w, gated, xb, T, ob, act, early, di, status, st);
-        if (w->group == 64)
-            return launch_small<2>(w, gated, xb, T, ob, act, early, di, status, st);
-        return launch_small<4>(w, gated, xb, T, ob, act, early, di, status, st);
+    if (w->group == 32)
+        return launch_small<1>(w, gated, xb, T, ob, act, early, di, status, st);
+    if (w->group == 64)
+        return launch_small<2>(w, gated, xb, T, ob, act, early, di, status, st);
+    return launch_small<4>(w, gated, xb, T, ob, act, early, di, status, st);
+}
+
+size_t linear_bytes(const XsMoeW4 *w, int T)
+{
+    return small_batch(T, w->cols) ? kStatusBytes : plan_scratch(w, nullptr, T, kStatusBytes).bytes;
+}
+
+int run_linear(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void *out, uint8_t *ws, cudaStream_t st)
+{
+    int32_t *status = reinterpret_cast<int32_t *>(ws);
+    if (small_batch(T, w->cols))
+        return run_small(w, gated, act, x, T, out, false, status, st);
+    const TcScratch p = plan_scratch(w, nullptr, T, kStatusBytes);
+    if (int rc = launch_prepare(w, gated, nullptr, nullptr, x, T, ws, p, st))
+        return rc;
+    const xs::TcOperands ops = operands(w, ws, p, 0, p.token);
+    return gated ? launch_tc<true>(w, ws + p.x16, T, out, ops, act, status, st) : launch_tc<false>(w, ws + p.x16, T, out, ops, 0, status, st);
+}
+
+// The gated product and the down product share one scratch: h behind the status block, then what the tensor-core kernel needs.
+size_t mlp_bytes(const XsMoeW4 *gu, const XsMoeW4 *dn, int T)
+{
+    const size_t at = kStatusBytes + bf16_bytes(T, gu->rows / 2);
+    return small_batch(T, gu->cols) && small_batch(T, dn->cols) ? at : plan_scratch(gu, dn, T, at).bytes;
+}
+
+// norm: the rows of x are normed on the way to the tensor core (null for small batches, and where there is no norm)
+int run_mlp(const XsMoeW4 *gu, const XsMoeW4 *dn, int32_t act, const XsMoeBlockNorms *norm, const void *x, int32_t T, void *out, uint8_t *ws, cudaStream_t st)
+{
+    int32_t *status = reinterpret_cast<int32_t *>(ws);
+    uint8_t *h = ws + kStatusBytes;
+    if (small_batch(T, gu->cols) && small_batch(T, dn->cols)) {
+        if (int rc = run_small(gu, true, act, x, T, h, false, status, st))
+            return rc;
+        return run_small(dn, false, 0, h, T, out, true, status, st);
     }
-    return gated ? launch_tc<true>(w, xb, T, ob, act, di.sms, status, st) : launch_tc<false>(w, xb, T, ob, act, di.sms, status, st);
+    const TcScratch p = plan_scratch(gu, dn, T, kStatusBytes + bf16_bytes(T, gu->rows / 2));
+    if (int rc = launch_prepare(gu, true, dn, norm, x, T, ws, p, st))
+        return rc;
+    xs::TcOperands up = operands(gu, ws, p, 0, p.token);
+    up.h_inverse = reinterpret_cast<const float *>(ws + p.h_inverse);
+    if (int rc = launch_tc<true>(gu, ws + p.x16, T, h, up, act, status, st))
+        return rc;
+    return launch_tc<false>(dn, h, T, out, operands(dn, ws, p, 1, p.h_factor), 0, status, st);
 }
 
 template <int GROUP, int ITER, bool ALIGNED>
@@ -542,13 +701,6 @@ XsMoeNormResidual block_tail(const XsMoeBlockNorms *n, const void *y, const void
     return a;
 }
 
-int run_mlp(const XsMoeW4 *gu, const XsMoeW4 *dn, int32_t act, const void *x, int32_t tokens, void *out, uint8_t *scratch, int32_t *status, cudaStream_t st)
-{
-    if (int rc = launch_w4(gu, true, act, x, tokens, scratch, false, status, st))
-        return rc;
-    return launch_w4(dn, false, 0, scratch, tokens, out, true, status, st);
-}
-
 // the fail() string may allocate: an exception of the host library becomes a status like every other failure
 template <typename F>
 int guarded(F &&f) noexcept
@@ -571,7 +723,7 @@ int xs_moe_linear_w4_workspace_bytes(const XsMoeW4 *w, int32_t tokens, size_t *b
             return rc;
         if (!bytes)
             return fail(XS_MOE_ERR_INVALID_ARG, "null out-pointer");
-        *bytes = kStatusBytes;
+        *bytes = linear_bytes(w, tokens);
         return 0;
     });
 }
@@ -583,16 +735,17 @@ int xs_moe_linear_w4(const XsMoeW4 *w, const void *x, int32_t tokens, void *out,
             return rc;
         if (tokens == 0)
             return 0;
-        if (int rc = check_workspace(ws, ws_bytes, kStatusBytes))
+        const size_t need = linear_bytes(w, tokens);
+        if (int rc = check_workspace(ws, ws_bytes, need))
             return rc;
         int dev = 0;
         if (int rc = current_device(&dev))
             return rc;
         if (int rc = check_w4_data(w, dev))
             return rc;
-        if (int rc = check_io(x, static_cast<size_t>(tokens) * w->cols, out, static_cast<size_t>(tokens) * w->rows, ws, kStatusBytes, dev))
+        if (int rc = check_io(x, static_cast<size_t>(tokens) * w->cols, out, static_cast<size_t>(tokens) * w->rows, ws, need, dev))
             return rc;
-        return launch_w4(w, false, 0, x, tokens, out, false, static_cast<int32_t *>(ws), static_cast<cudaStream_t>(stream));
+        return run_linear(w, false, 0, x, tokens, out, static_cast<uint8_t *>(ws), static_cast<cudaStream_t>(stream));
     });
 }
 
@@ -603,16 +756,17 @@ int xs_moe_gated_w4(const XsMoeW4 *gate_up, int32_t activation, const void *x, i
             return rc;
         if (tokens == 0)
             return 0;
-        if (int rc = check_workspace(ws, ws_bytes, kStatusBytes))
+        const size_t need = linear_bytes(gate_up, tokens);
+        if (int rc = check_workspace(ws, ws_bytes, need))
             return rc;
         int dev = 0;
         if (int rc = current_device(&dev))
             return rc;
         if (int rc = check_w4_data(gate_up, dev))
             return rc;
-        if (int rc = check_io(x, static_cast<size_t>(tokens) * gate_up->cols, h, static_cast<size_t>(tokens) * (gate_up->rows / 2), ws, kStatusBytes, dev))
+        if (int rc = check_io(x, static_cast<size_t>(tokens) * gate_up->cols, h, static_cast<size_t>(tokens) * (gate_up->rows / 2), ws, need, dev))
             return rc;
-        return launch_w4(gate_up, true, activation, x, tokens, h, false, static_cast<int32_t *>(ws), static_cast<cudaStream_t>(stream));
+        return run_linear(gate_up, true, activation, x, tokens, h, static_cast<uint8_t *>(ws), static_cast<cudaStream_t>(stream));
     });
 }
 
@@ -623,7 +777,7 @@ int xs_moe_mlp_w4_workspace_bytes(const XsMoeW4 *gate_up, const XsMoeW4 *down, i
             return rc;
         if (!bytes)
             return fail(XS_MOE_ERR_INVALID_ARG, "null out-pointer");
-        *bytes = kStatusBytes + bf16_bytes(tokens, gate_up->rows / 2);
+        *bytes = mlp_bytes(gate_up, down, tokens);
         return 0;
     });
 }
@@ -636,7 +790,7 @@ int xs_moe_mlp_w4(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t activatio
             return rc;
         if (tokens == 0)
             return 0;
-        const size_t need = kStatusBytes + bf16_bytes(tokens, gate_up->rows / 2);
+        const size_t need = mlp_bytes(gate_up, down, tokens);
         if (int rc = check_workspace(ws, ws_bytes, need))
             return rc;
         int dev = 0;
@@ -649,8 +803,7 @@ int xs_moe_mlp_w4(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t activatio
         const size_t n = static_cast<size_t>(tokens) * gate_up->cols;
         if (int rc = check_io(x, n, out, n, ws, need, dev))
             return rc;
-        return run_mlp(gate_up, down, activation, x, tokens, out, static_cast<uint8_t *>(ws) + kStatusBytes, static_cast<int32_t *>(ws),
-                       static_cast<cudaStream_t>(stream));
+        return run_mlp(gate_up, down, activation, nullptr, x, tokens, out, static_cast<uint8_t *>(ws), static_cast<cudaStream_t>(stream));
     });
 }
 
@@ -685,8 +838,7 @@ int xs_moe_mlp_w4_block(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t act
             return rc;
         if (tokens == 0)
             return 0;
-        const size_t act_bytes = bf16_bytes(tokens, gate_up->rows / 2), row_bytes = bf16_bytes(tokens, H);
-        const size_t need = kStatusBytes + act_bytes + 2 * row_bytes;
+        const size_t inner = mlp_bytes(gate_up, down, tokens), row_bytes = bf16_bytes(tokens, H), need = inner + 2 * row_bytes;
         if (int rc = check_workspace(ws, ws_bytes, need))
             return rc;
         if (int rc = check_w4_data(gate_up, dev))
@@ -698,13 +850,18 @@ int xs_moe_mlp_w4_block(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t act
             return rc;
         if (int rc = check_block_overlap(norms, tokens, H, out, ws, need))
             return rc;
-        uint8_t *h = static_cast<uint8_t *>(ws) + kStatusBytes, *xn = h + act_bytes, *y = xn + row_bytes;
+        uint8_t *base = static_cast<uint8_t *>(ws), *xn = base + inner, *y = xn + row_bytes;
         cudaStream_t st = static_cast<cudaStream_t>(stream);
-        const XsMoeNormResidual pre = pre_norm(norms, x, xn, tokens, H), tail = block_tail(norms, y, x, out, tokens, H);
-        if (int rc = run_norm(&pre, st))
+        // larger batches are normed where their tokens are made ready for the tensor core, small ones by a pass of their own
+        const bool small = small_batch(tokens, H) && small_batch(tokens, down->cols);
+        if (small) {
+            const XsMoeNormResidual pre = pre_norm(norms, x, xn, tokens, H);
+            if (int rc = run_norm(&pre, st))
+                return rc;
+        }
+        if (int rc = run_mlp(gate_up, down, activation, small ? nullptr : norms, small ? xn : x, tokens, y, base, st))
             return rc;
-        if (int rc = run_mlp(gate_up, down, activation, xn, tokens, y, h, static_cast<int32_t *>(ws), st))
-            return rc;
+        const XsMoeNormResidual tail = block_tail(norms, y, x, out, tokens, H);
         return run_norm(&tail, st);
     });
 }

@@ -1,0 +1,284 @@
+// What the tensor-core kernel of the 4-bit products needs before it starts: the tokens and the size of the scales.
+//
+// Its operands are f16, not bf16: (q - z) s has twelve significant bits, and f16 keeps eleven of them where bf16 keeps eight (the rounding
+// of a weight is then an eighth of the rounding of a result, instead of as large), while a bf16 token is exact in f16 once its
+// exponent fits.  So every token is scaled by a power of two that brings its largest element to 2^13 .. 2^14: elements down to
+// 2^-27 of that are exact, smaller ones are off by 2^-39 of it at most.  The scales of each weight row are brought to f16 in the
+// same way, into rows of a padded pitch (with the zero points), which the kernel reads in one piece per block whatever the
+// alignment of the originals; a row whose scales differ by less than 2^4 is marked, and takes a shorter conversion there.  The powers of
+// two come back in the kernel's epilogue.
+//
+// The gated product's own result becomes the next product's token, and must be scaled before the largest of a row is known: by
+// a bound, |act(g) u| <= |g| |u| <= (|x| |w_g|) (|x| |w_u|) with |w| <= sqrt(K) 15 max s (2-norms).  The bound lies some 2^15 above
+// what occurs, of the 2^39 that f16 spans; the products of a row smaller than that again lose bits.
+//
+// Bytes decide: tokens are read once and written once; the scales are a fiftieth of the weights.  With `norm_w` the tokens are
+// normed on the way (the first norm of a block): v / sqrt(mean v^2 + eps) * (offset + w), rounded once, to f16.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "xs_ptx.cuh"
+
+namespace xs {
+
+struct PrepareScales {
+    const uint16_t *scales; // bf16 (rows, groups)
+    const uint8_t *zeros;   // (rows, groups) or null
+    uint16_t *scales16;     // f16 (rows, pitch): scale = scales16 * 2^c
+    uint8_t *zeros8;        // (rows, pitch)
+    float *factor;          // 2^(c + 9) of a row: what its sums are multiplied by; negative for a row of wide range
+    int rows, groups, pitch;
+    int per_block, blocks; // rows of a block (half gate, half up rows where they go together)
+    int lanes;             // lanes on a row: a power of two; 8 groups each at a time if `vec`
+    int vec;
+};
+struct PrepareArgs {
+    const __nv_bfloat16 *x, *norm_w;
+    __half *x16;
+    float *factor; // token = x16 * factor
+    int *l;        // 2-norm of the token <= 2^l
+    int T, K;
+    float eps, offset;
+    PrepareScales m[2];   // the second may be empty (blocks = 0)
+    int pair;             // m[0] is gate and up: rows i and i + rows / 2 go together
+    int bound_add;        // what the number of columns adds to the exponent of the gated product's bound
+    int *pair_part;       // for each block of m[0]: its largest exponent(gate) + exponent(up)
+    float *h_factor, *h_inverse; // of each token's gated product, by its bound
+    unsigned int *ticket; // zero between calls
+};
+
+constexpr int kPrepThreads = 256;
+constexpr int kPrepRows = 64;      // weight rows of a block at most
+constexpr int kPrepKeep = 4;       // pieces of eight columns a thread keeps in registers
+constexpr int kExpMin = -112, kExpMax = 112;
+constexpr int kTcUnitExp = 9; // the codes enter as (q - z) 2^-9
+
+__device__ __forceinline__ float pow2f(int e) // -126 <= e <= 127
+{
+    return __int_as_float((e + 127) << 23);
+}
+// floor(log2 v) of a positive normal v; subnormal numbers count as 2^-127
+__device__ __forceinline__ int log2_floor(float v)
+{
+    return ((__float_as_int(v) >> 23) & 255) - 127;
+}
+__device__ __forceinline__ float prep_get(const uint4 &v, int i)
+{
+    const uint32_t u = i / 2 == 0 ? v.x : i / 2 == 1 ? v.y : i / 2 == 2 ? v.z : v.w;
+    return __uint_as_float(i % 2 ? u & 0xffff0000u : u << 16);
+}
+__device__ __forceinline__ float finite_abs(float v)
+{
+    const float a = fabsf(v);
+    return a <= 3.4e38f ? a : 0.0f; // infinities and NaN do not count
+}
+
+__global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareArgs a)
+{
+    constexpr int WARPS = kPrepThreads / 32;
+    __shared__ float part[3][WARPS];
+    __shared__ int ipart[WARPS], row_exp[kPrepRows], last;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (static_cast<int>(blockIdx.x) < a.T) {
+        const int t = blockIdx.x, pieces = a.K / 8;
+        const uint4 *x = reinterpret_cast<const uint4 *>(a.x + static_cast<size_t>(t) * a.K);
+        uint4 keep[kPrepKeep];
+#pragma unroll
+        for (int i = 0; i < kPrepKeep; i++) {
+            keep[i] = make_uint4(0, 0, 0, 0);
+            if (threadIdx.x + i * kPrepThreads < pieces)
+                keep[i] = x[threadIdx.x + i * kPrepThreads];
+        }
+        // f(piece, its columns) over this thread's pieces: those kept, then the rest of a long row from memory again
+        auto each = [&](auto &&f) {
+#pragma unroll
+            for (int i = 0; i < kPrepKeep; i++)
+                if (threadIdx.x + i * kPrepThreads < pieces)
+                    f(threadIdx.x + i * kPrepThreads, keep[i]);
+            for (int p = threadIdx.x + kPrepKeep * kPrepThreads; p < pieces; p += kPrepThreads)
+                f(p, x[p]);
+        };
+        auto block_reduce = [&](float v, int slot, bool maximum) {
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+                const float u = __shfl_xor_sync(0xffffffffu, v, o);
+                v = maximum ? fmaxf(v, u) : v + u;
+            }
+            if (lane == 0)
+                part[slot][warp] = v;
+            __syncthreads();
+            v = part[slot][0];
+#pragma unroll
+            for (int i = 1; i < WARPS; i++)
+                v = maximum ? fmaxf(v, part[slot][i]) : v + part[slot][i];
+            return v;
+        };
+        float inv = 1.0f;
+        if (a.norm_w) {
+            float ss = 0.0f;
+            each([&](int, const uint4 &v) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    ss = fmaf(prep_get(v, i), prep_get(v, i), ss);
+            });
+            inv = rsqrtf(block_reduce(ss, 0, false) / static_cast<float>(a.K) + a.eps);
+        }
+        auto value = [&](int p, const uint4 &v, int i) {
+            float f = prep_get(v, i);
+            if (a.norm_w)
+                f = f * inv * (a.offset + __bfloat162float(a.norm_w[p * 8 + i]));
+            return f;
+        };
+        float top = 0.0f;
+        each([&](int p, const uint4 &v) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                top = fmaxf(top, finite_abs(value(p, v, i)));
+        });
+        const int e = max(kExpMin, min(kExpMax, log2_floor(block_reduce(top, 1, true)) - 13));
+        const float down = pow2f(-e);
+        float ss = 0.0f;
+        uint4 *out = reinterpret_cast<uint4 *>(a.x16 + static_cast<size_t>(t) * a.K);
+        each([&](int p, const uint4 &v) {
+            __half2 o[4];
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const float f0 = value(p, v, i) * down, f1 = value(p, v, i + 1) * down;
+                const float c0 = finite_abs(f0), c1 = finite_abs(f1);
+                ss = fmaf(c0, c0, fmaf(c1, c1, ss));
+                o[i / 2] = __floats2half2_rn(f0, f1);
+            }
+            out[p] = *reinterpret_cast<uint4 *>(o);
+        });
+        ss = block_reduce(ss, 2, false);
+        if (threadIdx.x == 0) {
+            a.factor[t] = pow2f(e);
+            // sqrt(ss) < 2^((k + 1) / 2) with k = floor(log2 ss), and one more for the roundings of the sum
+            a.l[t] = ss > 0.0f ? e + ((log2_floor(ss) + 3) >> 1) : kExpMin;
+        }
+    } else {
+        int b = blockIdx.x - a.T;
+        const int which = b >= a.m[0].blocks ? 1 : 0;
+        if (which)
+            b -= a.m[0].blocks;
+        const PrepareScales m = which ? a.m[1] : a.m[0];
+        const bool pair = which == 0 && a.pair;
+        const int half_rows = m.rows / 2, half_block = m.per_block / 2;
+        const int sub = lane & (m.lanes - 1);
+        for (int r = threadIdx.x / m.lanes; r < m.per_block; r += kPrepThreads / m.lanes) {
+            // a block's first rows are gate rows, its last the up rows of the same features
+            const int i = pair ? b * half_block + (r < half_block ? r : r - half_block) : b * m.per_block + r;
+            const bool there = i < (pair ? half_rows : m.rows);
+            const size_t row = there ? static_cast<size_t>(i) + (pair && r >= half_block ? half_rows : 0) : 0;
+            const uint16_t *s = m.scales + row * m.groups;
+            auto eight = [&](int g) { // groups g .. g + 7, zero behind the last one
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (m.vec) {
+                    v = *reinterpret_cast<const uint4 *>(s + g);
+                } else {
+                    uint32_t u[4] = {};
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (g + j < m.groups)
+                            u[j / 2] |= static_cast<uint32_t>(s[g + j]) << (j % 2 * 16);
+                    v = make_uint4(u[0], u[1], u[2], u[3]);
+                }
+                return v;
+            };
+            float top = 0.0f, low = 3.4e38f;
+            bool odd = false; // an infinity or NaN
+            for (int g = sub * 8; g < m.groups; g += m.lanes * 8) {
+                const uint4 v = eight(g);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float f = fabsf(prep_get(v, j)), c = finite_abs(f);
+                    odd |= !(f <= 3.4e38f);
+                    top = fmaxf(top, c);
+                    low = c > 0.0f ? fminf(low, c) : low;
+                }
+            }
+            for (int o = m.lanes / 2; o; o >>= 1) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+                odd |= __shfl_xor_sync(0xffffffffu, odd ? 1 : 0, o) != 0;
+            }
+            // narrow: scales below 1 and not below 2^-4, so that (q - 8) scale 2^-9 is a normal f16 and the scale times 2^15 one as well;
+            // wide: below 2^15, which leaves 2^20 down to the first lost bit
+            const int top_exp = log2_floor(top);
+            const bool narrow = !odd && top_exp < 100 && top_exp - log2_floor(fminf(low, top)) < 4;
+            const int c = max(kExpMin, min(kExpMax, narrow ? top_exp + 1 : top_exp - 14));
+            const float down = pow2f(-c);
+            if (there) {
+                for (int g = sub * 8; g < m.groups; g += m.lanes * 8) {
+                    const uint4 v = eight(g);
+                    __half2 o[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        o[j] = __floats2half2_rn(prep_get(v, 2 * j) * down, prep_get(v, 2 * j + 1) * down);
+                    *reinterpret_cast<uint4 *>(m.scales16 + row * m.pitch + g) = *reinterpret_cast<uint4 *>(o);
+                    if (m.zeros) {
+                        const uint8_t *z = m.zeros + row * m.groups + g;
+                        uint32_t u[2] = {};
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            if (g + j < m.groups)
+                                u[j / 4] |= static_cast<uint32_t>(z[j]) << (j % 4 * 8);
+                        *reinterpret_cast<uint2 *>(m.zeros8 + row * m.pitch + g) = make_uint2(u[0], u[1]);
+                    }
+                }
+                if (sub == 0)
+                    m.factor[row] = narrow ? pow2f(c + kTcUnitExp) : -pow2f(c + kTcUnitExp);
+            }
+            if (pair && sub == 0)
+                row_exp[r] = there ? top_exp + 1 : -1000; // the row's scales are below 2^row_exp
+        }
+        if (pair) {
+            __syncthreads();
+            int top = -4000;
+            for (int r = threadIdx.x; r < half_block; r += kPrepThreads)
+                top = max(top, row_exp[r] + row_exp[r + half_block]);
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0)
+                ipart[warp] = top;
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                for (int i = 0; i < WARPS; i++)
+                    top = max(top, ipart[i]);
+                a.pair_part[b] = top;
+            }
+        }
+    }
+    if (!a.pair)
+        return;
+    // the block that is done last knows the bound of every token's gated product
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last = atomicInc(a.ticket, gridDim.x - 1) == gridDim.x - 1; // and leaves the ticket at zero
+    }
+    __syncthreads();
+    if (!last)
+        return;
+    __threadfence();
+    int top = -4000;
+    for (int i = threadIdx.x; i < a.m[0].blocks; i += kPrepThreads)
+        top = max(top, __ldcg(a.pair_part + i));
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0)
+        ipart[warp] = top;
+    __syncthreads();
+    for (int i = 0; i < WARPS; i++)
+        top = max(top, ipart[i]);
+    for (int t = threadIdx.x; t < a.T; t += kPrepThreads) {
+        const int e = max(kExpMin, min(kExpMax, 2 * __ldcg(a.l + t) + top + a.bound_add));
+        a.h_factor[t] = pow2f(e);
+        a.h_inverse[t] = pow2f(-e);
+    }
+}
+
+} // namespace xs

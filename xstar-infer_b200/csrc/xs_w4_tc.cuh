@@ -1,10 +1,11 @@
 // Products with 4-bit weights on the tensor core, for batches from nine tokens up: out = x W^T (or act(x Wg^T) * (x Wu^T)).
 //
 // tcgen05.mma with the WEIGHTS as its M rows, taken from TMEM, and the tokens as its N columns, taken from shared memory.  The codes
-// arrive by TMA as they lie in memory; sixteen warps turn them into bf16, thread = weight row, and store them with tcgen05.st
+// arrive by TMA as they lie in memory; sixteen warps turn them into f16, thread = weight row, and store them with tcgen05.st
 // straight into TMEM columns, so a dequantised weight never passes through shared memory, whose bandwidth the tokens need.
-// Weights in TMEM also make the group scale a scalar of the thread.  (q - z) s is rounded to bf16 once, half a step: the price of
-// the tensor core, whose operands have one type.  Sums are f32 in TMEM, scaled by 2^-10.
+// Weights in TMEM also make the group scale a scalar of the thread.  Tokens, and the scales of a weight row, have been given a
+// common exponent (xs_w4_prepare.cuh); q - z is exact, and times its scale it is rounded once, to the eleven bits of f16.
+// Sums are f32 in TMEM; the epilogue multiplies them by the powers of two of their row and token.
 //
 // CG = 2 pairs two SMs on a 256 x 256 tile (cta_group::2): each dequantises its 128 rows and loads its 128 tokens, so the
 // traffic out of L2 and the dequantisation per product halve against two 128 x 256 tiles.  CG = 1 serves smaller batches, where
@@ -20,11 +21,13 @@
 // tile, and everybody else waited for it.
 #pragma once
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include "xs_ptx.cuh"
 #include "xs_w4_common.cuh"
+#include "xs_w4_prepare.cuh"
 
 namespace xs {
 
@@ -37,8 +40,6 @@ constexpr int kTcRawBlocks = 2;    // operand blocks in one load of codes: 256 c
 constexpr int kTcRawBytes = kTcRows * 128;
 constexpr int kTcStages = 4;       // operand blocks in flight: TMEM columns of weights, shared memory of tokens
 constexpr int kTcAccCol = kTcStages * (kTcBlockK / 2);
-
-constexpr float kTcUnit = 1024.0f; // the sums are 2^-10 of the products
 
 __host__ __device__ constexpr int tc_x_bytes(int cg, int n_tile)
 {
@@ -136,11 +137,24 @@ __device__ __forceinline__ uint32_t w4_pair(uint32_t word, int c)
     const uint32_t low = word & 0x0f0f0f0fu, high = word & 0xf0f0f0f0u;
     return prmt(low, high, c | (8 | c) << 4 | (4 + c) << 8 | (8 | c) << 12);
 }
-__device__ __forceinline__ uint32_t bf16x2_mul(uint32_t a, uint32_t b)
+__device__ __forceinline__ uint32_t f16x2_mul(uint32_t a, uint32_t b)
 {
     uint32_t r;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
+}
+__device__ __forceinline__ uint32_t f16x2_fma(uint32_t a, uint32_t b, uint32_t c)
+{
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+// An f16 whose bits are an integer below 1024 is that integer times 2^-24, so a nibble, or sixteen times one, is a number as it
+// stands; times 2^15 (2^11) it is the code times 2^-9.
+constexpr uint32_t kTcPairMul = 0x68007800u, kTcMinus8 = 0xa400a400u; // 2^11 2^15; -8 * 2^-9
+__device__ __forceinline__ uint32_t tc_minus_zero(uint32_t z)
+{
+    return f16x2_mul(z * 0x00010001u, 0xf800f800u); // -2^15
 }
 
 // Barrier 1 among the eight epilogue warps; the conjunction of their predicates.
@@ -150,6 +164,16 @@ __device__ __forceinline__ bool named_barrier_and(bool ok)
     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"(ok ? 1u : 0u) : "memory");
     return r != 0;
 }
+
+// What w4_prepare_kernel made of the scales and tokens, and how the result is written.
+struct TcOperands {
+    const uint16_t *scales; // f16 (rows, pitch)
+    const uint8_t *zeros;   // (rows, pitch) or null: 8
+    const float *row;       // factor of a weight row's sums; negative: its scales are of wide range
+    const float *token;     // factor of a token
+    const float *h_inverse; // gated: write the product in f16, times this; null: in bf16
+    int pitch;
+};
 
 struct TcShape {
     int n_out, T, K, G_log; // G_log: log2 of the group
@@ -167,15 +191,30 @@ __device__ __forceinline__ void tc_tile(const TcShape &s, int item, int &wt, int
     tt = first + r - wt * width;
 }
 
+// One element of the result: v, or act(v) u; in bf16, or scaled by its bound in f16 for the product that follows.
+template <bool GATED>
+__device__ __forceinline__ void tc_store(void *out, const TcShape &s, const TcOperands &w, int act, int t, int feature, float v, float u)
+{
+    const size_t at = static_cast<size_t>(t) * s.n_out + feature;
+    if constexpr (GATED) {
+        v = w4_activation(v, act) * u;
+        if (w.h_inverse) {
+            static_cast<__half *>(out)[at] = __float2half_rn(v * __ldg(w.h_inverse + t));
+            return;
+        }
+    }
+    static_cast<__nv_bfloat16 *>(out)[at] = __float2bfloat16_rn(v);
+}
+
 template <int CG, int N_TILE, bool GATED>
 __global__ void __launch_bounds__(kTcThreads, 1)
-w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const W4Matrix w, __nv_bfloat16 *__restrict__ out,
+w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const TcOperands w, void *__restrict__ out,
              const TcShape s, int act, int32_t *__restrict__ status)
 {
     constexpr int RAW = tc_raw_stages(CG, N_TILE), X_BYTES = tc_x_bytes(CG, N_TILE);
     constexpr int FEATURES = GATED ? kTcRows / 2 : kTcRows; // of a block
     constexpr int NBUF = N_TILE <= 128 ? 2 : 1;             // accumulators
-    constexpr uint32_t IDESC = make_idesc(1, 1, kTcRows * CG, N_TILE);
+    constexpr uint32_t IDESC = make_idesc(0, 0, kTcRows * CG, N_TILE); // f16
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -316,9 +355,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
         const int feature = GATED ? q * 16 + (lane & 15) : raw_row;
         const uint32_t raw_addr = smem_u32(smem) + raw_row * 128, swz = (raw_row & 7) << 4;
         // Groups of a block (4, 2 or 1) with their scales and zero points, loaded two of this warpgroup's blocks ahead.
-        const int groups = s.K >> s.G_log, per_block = 1 << (7 - s.G_log);
-        const bool vec = groups % per_block == 0 && reinterpret_cast<uintptr_t>(w.scales) % (2 * per_block) == 0 &&
-                         reinterpret_cast<uintptr_t>(w.zeros) % per_block == 0;
+        const int per_block = 1 << (7 - s.G_log);
         const bool zeros = w.zeros != nullptr;
         const int first = kb0 + ((wg - kb0) & 3);
         struct Scales {
@@ -327,50 +364,38 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
         };
         int ld_item = first < kb1 ? item0 : items, ld_kb = first;
         size_t ld_row = 0; // first group of the row
-        auto ld_start = [&]() {
+        auto row_at = [&](int item) {
             int wt, tt;
-            tc_tile(s, ld_item, wt, tt);
-            const int f = min(wt * FEATURES * CG + block_feature + feature, s.n_out - 1);
-            ld_row = (static_cast<size_t>(f) + (GATED && lane >= 16 ? s.n_out : 0)) * groups;
+            tc_tile(s, item, wt, tt);
+            return static_cast<size_t>(min(wt * FEATURES * CG + block_feature + feature, s.n_out - 1)) + (GATED && lane >= 16 ? s.n_out : 0);
         };
         auto load_scales = [&]() {
             Scales r;
             r.s = make_uint2(0, 0);
             r.z = 0;
             if (ld_item < items) {
-                const int g0 = ld_kb * per_block;
-                const uint16_t *sp = reinterpret_cast<const uint16_t *>(w.scales) + ld_row + g0;
-                const uint8_t *zp = w.zeros + ld_row + g0;
-                if (vec) {
-                    if (per_block == 4)
-                        r.s = __ldg(reinterpret_cast<const uint2 *>(sp));
-                    else if (per_block == 2)
-                        r.s.x = __ldg(reinterpret_cast<const uint32_t *>(sp));
-                    else
-                        r.s.x = __ldg(sp);
-                    if (zeros)
-                        r.z = per_block == 4 ? __ldg(reinterpret_cast<const uint32_t *>(zp)) : per_block == 2 ? __ldg(reinterpret_cast<const uint16_t *>(zp)) : __ldg(zp);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (i < per_block && g0 + i < groups) {
-                            (i < 2 ? r.s.x : r.s.y) |= static_cast<uint32_t>(__ldg(sp + i)) << (i % 2 * 16);
-                            if (zeros)
-                                r.z |= static_cast<uint32_t>(__ldg(zp + i)) << (i * 8);
-                        }
-                }
+                const uint16_t *sp = w.scales + ld_row + ld_kb * per_block;
+                const uint8_t *zp = w.zeros + ld_row + ld_kb * per_block;
+                if (per_block == 4)
+                    r.s = __ldg(reinterpret_cast<const uint2 *>(sp));
+                else if (per_block == 2)
+                    r.s.x = __ldg(reinterpret_cast<const uint32_t *>(sp));
+                else
+                    r.s.x = __ldg(sp);
+                if (zeros)
+                    r.z = per_block == 4 ? __ldg(reinterpret_cast<const uint32_t *>(zp)) : per_block == 2 ? __ldg(reinterpret_cast<const uint16_t *>(zp)) : __ldg(zp);
                 ld_kb += 4;
                 if (ld_kb >= kb1) {
                     ld_kb = first;
                     ld_item += item_step;
                     if (ld_item < items)
-                        ld_start();
+                        ld_row = row_at(ld_item) * w.pitch;
                 }
             }
             return r;
         };
         if (ld_item < items)
-            ld_start();
+            ld_row = row_at(ld_item) * w.pitch;
         Scales cur, next, after;
 #pragma unroll 1
         for (int i = 0; i < 2; i++) {
@@ -380,6 +405,9 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
         const uint32_t tmem_lane = tmem + (static_cast<uint32_t>(q * 32) << 16);
         uint32_t n = 0, nr = 0; // operand blocks and loads of codes before this item
         for (int item = item0; item < items && ok; item += item_step, n += n_kb, nr += raw1 - raw0) {
+            // Zero point 8 and scales of narrow range in the warp's 32 rows: one multiply-add a pair, n (2^15 s) 2^-24 - 8 s 2^-9, whose
+            // parts are exact; else (q - z) 2^-9 first, exactly, then times s.
+            const bool one_step = !zeros && __all_sync(0xffffffffu, __ldg(w.row + row_at(item)) > 0.0f);
             // up to the last load's second block, which may not be there: its codes are given back all the same
             for (int kb = first; kb < raw1 * kTcRawBlocks; kb += 4) {
                 const uint32_t rc = nr + (kb >> 1) - raw0, rs = rc % RAW;
@@ -390,10 +418,6 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                     cur = next;
                     next = after;
                     after = load_scales();
-                    // A scale below 32 and the zero point 8 need one multiply-add: s 2^123 is finite and 8 s exact, so the
-                    // difference is rounded once; else (q - z) / 64 is made first, exactly, and multiplied by s / 16.
-                    const bool one_step =
-                        !zeros && __all_sync(0xffffffffu, ((((cur.s.x & 0x7fff7fffu) + 0x3e003e00u) | ((cur.s.y & 0x7fff7fffu) + 0x3e003e00u)) & 0x80008000u) == 0);
                     if (!__all_sync(0xffffffffu, raw_there || mbar_wait(&raw_full[rs], (rc / RAW) & 1, abort_flag))) {
                         ok = false;
                         break;
@@ -402,26 +426,27 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
 #pragma unroll
                     for (int h = 0; h < 4; h++) { // 32 columns: one 16-byte piece of codes, one group
                         const int e = (h * per_block) >> 2;
+                        // past the end of K the codes read as zero, and so must the weight, whatever the zero point
                         uint32_t sv = prmt(cur.s.x, cur.s.y, 0x1010u + 0x2222u * e);
                         if (kb * kTcBlockK + h * 32 >= s.K)
-                            sv = 0; // past the end: the codes read as zero, and so must the weight, whatever the zero point
+                            sv = 0;
                         const uint4 qv = lds128(codes + ((((kb & 1) * 4 + h) << 4) ^ swz));
                         const uint32_t words[4] = {qv.x, qv.y, qv.z, qv.w};
                         uint32_t a[16];
                         if (one_step) {
-                            const uint32_t mul = bf16x2_mul(sv, 0x7b007d00u), add = bf16x2_mul(sv, 0xbc00bc00u); // 2^119 2^123, -2^-7
+                            const uint32_t mul = f16x2_mul(sv, kTcPairMul), add = f16x2_mul(sv, kTcMinus8);
 #pragma unroll
                             for (int j = 0; j < 4; j++)
 #pragma unroll
                                 for (int c = 0; c < 4; c++)
-                                    a[j * 4 + c] = w4_fma(w4_pair(words[j], c), mul, add);
+                                    a[j * 4 + c] = f16x2_fma(w4_pair(words[j], c), mul, add);
                         } else {
-                            const uint32_t mz = zeros ? w4_minus_zero((cur.z >> (8 * e)) & 15u) : kW4Minus8, ms = bf16x2_mul(sv, 0x3d803d80u); // 2^-4
+                            const uint32_t mz = zeros ? tc_minus_zero((cur.z >> (8 * e)) & 15u) : kTcMinus8;
 #pragma unroll
                             for (int j = 0; j < 4; j++)
 #pragma unroll
                                 for (int c = 0; c < 4; c++)
-                                    a[j * 4 + c] = bf16x2_mul(w4_fma(w4_pair(words[j], c), 0x7d007f00u, mz), ms); // 2^123 2^127
+                                    a[j * 4 + c] = f16x2_mul(f16x2_fma(w4_pair(words[j], c), kTcPairMul, mz), sv);
                         }
                         if (h == 0) {
                             ok = __all_sync(0xffffffffu, is_free || mbar_wait(&empty[st], free, abort_flag));
@@ -469,6 +494,8 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
             tc_fence_after();
             const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16) + kTcAccCol + buf * N_TILE + part * COLS;
             const int feature = wt * FEATURES * CG + block_feature + lane_feature, token0 = tt * N_TILE + part * COLS;
+            const int f0 = min(feature, s.n_out - 1);
+            const float row_f = fabsf(__ldg(w.row + f0)), row_u = GATED ? fabsf(__ldg(w.row + s.n_out + f0)) : 0.0f;
             if (CG == 1 && s.split > 1) {
                 // the sums of this block's slice of K, [token][lane], over the operand ring, which nothing reads or fills any more
                 float *red = reinterpret_cast<float *>(smem);
@@ -493,7 +520,6 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                     if (lane == 0)
                         tc_arrive_leader<CG>(&acc_empty[buf]);
                 }
-                __nv_bfloat16 *o = out + static_cast<size_t>(token0 + c) * s.n_out + feature;
                 if constexpr (GATED) {
                     // lanes 0..15 hold gate sums and 16..31 the up sums of the same features: of each pair of tokens the first half
                     // of the warp finishes the even one, the second half the odd one
@@ -501,16 +527,18 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
                         const float give = __uint_as_float(up ? v[i] : v[i + 1]), got = __shfl_xor_sync(0xffffffffu, give, 16);
-                        const float g = kTcUnit * (up ? got : __uint_as_float(v[i])), u = kTcUnit * (up ? __uint_as_float(v[i + 1]) : got);
-                        const int t = i + (up ? 1 : 0);
-                        if (feature < s.n_out && token0 + c + t < s.T)
-                            o[static_cast<size_t>(t) * s.n_out] = __float2bfloat16_rn(w4_activation(g, act) * u);
+                        const int t = token0 + c + i + (up ? 1 : 0);
+                        if (feature < s.n_out && t < s.T) {
+                            const float f = __ldg(w.token + t);
+                            tc_store<true>(out, s, w, act, t, feature, (up ? got : __uint_as_float(v[i])) * f * row_f,
+                                           (up ? __uint_as_float(v[i + 1]) : got) * f * row_u);
+                        }
                     }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 16; i++)
                         if (feature < s.n_out && token0 + c + i < s.T)
-                            o[static_cast<size_t>(i) * s.n_out] = __float2bfloat16_rn(kTcUnit * __uint_as_float(v[i]));
+                            tc_store<false>(out, s, w, act, token0 + c + i, feature, __uint_as_float(v[i]) * __ldg(w.token + token0 + c + i) * row_f, 0.0f);
                 }
             }
         }
@@ -539,7 +567,9 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                 if (GATED)
                     u += ld_cluster_f32(red + (c * kTcRows + row + 16) * 4, r);
             }
-            out[static_cast<size_t>(token) * s.n_out + feature] = __float2bfloat16_rn(GATED ? w4_activation(kTcUnit * v, act) * (kTcUnit * u) : kTcUnit * v);
+            const float t = __ldg(w.token + token);
+            tc_store<GATED>(out, s, w, act, token, feature, v * t * fabsf(__ldg(w.row + feature)),
+                            GATED ? u * t * fabsf(__ldg(w.row + s.n_out + feature)) : 0.0f);
         }
     }
     if (*abort_flag)
