@@ -321,9 +321,8 @@ bool small_batch(int T, int K)
 
 // Scratch of the tensor-core kernel: tokens and scales in f16, zero points, factors.
 struct TcScratch {
-    size_t x16 = 0, token = 0, l = 0, h_factor = 0, h_inverse = 0, part = 0, scales[2] = {}, zeros[2] = {}, row[2] = {}, bytes = 0;
+    size_t x16 = 0, token = 0, l = 0, part = 0, scales[2] = {}, zeros[2] = {}, row[2] = {}, bytes = 0;
 };
-constexpr size_t kOffTicket = 224; // status block: blocks of w4_prepare_kernel that are done (zero between calls)
 
 int groups_pitch(const XsMoeW4 *w)
 {
@@ -339,8 +338,8 @@ TcScratch plan_scratch(const XsMoeW4 *first, const XsMoeW4 *second, int T, size_
         return o;
     };
     p.x16 = take(static_cast<size_t>(T) * first->cols * 2);
-    for (size_t *o : {&p.token, &p.l, &p.h_factor, &p.h_inverse})
-        *o = take(static_cast<size_t>(T) * 4);
+    for (size_t *o : {&p.token, &p.l})
+        *o = take(static_cast<size_t>(T) * 4 + 1024); // a whole tile of tokens may be read
     p.part = take(static_cast<size_t>(first->rows) * 4);
     const XsMoeW4 *w[2] = {first, second};
     for (int i = 0; i < 2; i++) {
@@ -367,7 +366,7 @@ int bound_exponent(int cols)
 
 // Tokens (normed by `norm` where it is given) and the scales of up to two matrices.
 int launch_prepare(const XsMoeW4 *first, bool pair, const XsMoeW4 *second, const XsMoeBlockNorms *norm, const void *x, int T, uint8_t *ws,
-                   const TcScratch &p, cudaStream_t st)
+                   const TcScratch &p, cudaStream_t st, int *pair_parts = nullptr)
 {
     xs::PrepareArgs a{};
     a.x = static_cast<const __nv_bfloat16 *>(x);
@@ -395,7 +394,7 @@ int launch_prepare(const XsMoeW4 *first, bool pair, const XsMoeW4 *second, const
         m.rows = w[i]->rows;
         m.groups = w[i]->cols / w[i]->group;
         m.pitch = groups_pitch(w[i]);
-        m.vec = m.groups % 8 == 0 && !misaligned(m.scales, 16);
+        m.vec = m.groups % 8 == 0 && !misaligned(m.scales, 16) && !misaligned(m.zeros, 8);
         m.lanes = 1;
         while (m.lanes < 32 && m.lanes * 8 < m.groups)
             m.lanes *= 2;
@@ -406,23 +405,21 @@ int launch_prepare(const XsMoeW4 *first, bool pair, const XsMoeW4 *second, const
         blocks += m.blocks;
     }
     a.pair = pair ? 1 : 0;
-    a.bound_add = bound_exponent(first->cols);
     a.pair_part = reinterpret_cast<int *>(ws + p.part);
-    a.h_factor = reinterpret_cast<float *>(ws + p.h_factor);
-    a.h_inverse = reinterpret_cast<float *>(ws + p.h_inverse);
-    a.ticket = reinterpret_cast<unsigned int *>(ws + kOffTicket);
     XS_CUDA(launch_pdl(xs::w4_prepare_kernel, blocks, xs::kPrepThreads, 0, st, a));
     note_launch();
+    if (pair_parts)
+        *pair_parts = a.m[0].blocks;
     return 0;
 }
 
-xs::TcOperands operands(const XsMoeW4 *w, const uint8_t *ws, const TcScratch &p, int i, size_t token)
+xs::TcOperands operands(const XsMoeW4 *w, const uint8_t *ws, const TcScratch &p, int i)
 {
     xs::TcOperands o{};
     o.scales = reinterpret_cast<const uint16_t *>(ws + p.scales[i]);
     o.zeros = w->zeros_dev ? ws + p.zeros[i] : nullptr;
     o.row = reinterpret_cast<const float *>(ws + p.row[i]);
-    o.token = reinterpret_cast<const float *>(ws + token);
+    o.token = reinterpret_cast<const float *>(ws + p.token);
     o.pitch = groups_pitch(w);
     return o;
 }
@@ -455,7 +452,7 @@ int run_linear(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void
     const TcScratch p = plan_scratch(w, nullptr, T, kStatusBytes);
     if (int rc = launch_prepare(w, gated, nullptr, nullptr, x, T, ws, p, st))
         return rc;
-    const xs::TcOperands ops = operands(w, ws, p, 0, p.token);
+    const xs::TcOperands ops = operands(w, ws, p, 0);
     return gated ? launch_tc<true>(w, ws + p.x16, T, out, ops, act, status, st) : launch_tc<false>(w, ws + p.x16, T, out, ops, 0, status, st);
 }
 
@@ -477,13 +474,21 @@ int run_mlp(const XsMoeW4 *gu, const XsMoeW4 *dn, int32_t act, const XsMoeBlockN
         return run_small(dn, false, 0, h, T, out, true, status, st);
     }
     const TcScratch p = plan_scratch(gu, dn, T, kStatusBytes + bf16_bytes(T, gu->rows / 2));
-    if (int rc = launch_prepare(gu, true, dn, norm, x, T, ws, p, st))
+    int pair_parts = 0;
+    if (int rc = launch_prepare(gu, true, dn, norm, x, T, ws, p, st, &pair_parts))
         return rc;
-    xs::TcOperands up = operands(gu, ws, p, 0, p.token);
-    up.h_inverse = reinterpret_cast<const float *>(ws + p.h_inverse);
+    xs::TcOperands up = operands(gu, ws, p, 0), down = operands(dn, ws, p, 1);
+    up.out_f16 = 1;
+    down.token = nullptr;
+    for (xs::TcOperands *o : {&up, &down}) {
+        o->l = reinterpret_cast<const int *>(ws + p.l);
+        o->pair_part = reinterpret_cast<const int *>(ws + p.part);
+        o->parts = pair_parts;
+        o->bound_add = bound_exponent(gu->cols);
+    }
     if (int rc = launch_tc<true>(gu, ws + p.x16, T, h, up, act, status, st))
         return rc;
-    return launch_tc<false>(dn, h, T, out, operands(dn, ws, p, 1, p.h_factor), 0, status, st);
+    return launch_tc<false>(dn, h, T, out, down, 0, status, st);
 }
 
 template <int GROUP, int ITER, bool ALIGNED>

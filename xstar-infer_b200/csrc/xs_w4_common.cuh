@@ -44,12 +44,12 @@ __device__ __forceinline__ uint32_t w4_minus_zero(uint32_t z)
 }
 
 // silu: v / (1 + exp(-v)); gelu: v / 2 * (1 + tanh(c (v + 0.044715 v^3))), and (1 + tanh(a)) / 2 = 1 / (1 + exp(-2 a)).  The fast
-// exponential and division are off by a few f32 steps, far below the bf16 step of the result; far below zero both end at 0.
+// exponential and division are off by a few f32 steps, far below the step of the result; far below zero, where the
+// exponential leaves f32, the division gives the zero that the result is.
 __device__ __forceinline__ float w4_activation(float v, int act)
 {
-    const float a = act == 0 ? v : 1.5957691216057308f * (v + 0.044715f * v * v * v);
-    const float e = 1.0f + __expf(-a);
-    return e < 1e37f ? __fdividef(v, e) : (v != v ? v : v * 0.0f);
+    const float a = act == 0 ? v : 1.5957691216057308f * fmaf(0.044715f * v * v, v, v);
+    return __fdividef(v, 1.0f + __expf(-a));
 }
 
 // A bounded wait of a whole warp with one outcome; one lane polls for all.

@@ -44,14 +44,11 @@ struct PrepareArgs {
     float eps, offset;
     PrepareScales m[2];   // the second may be empty (blocks = 0)
     int pair;             // m[0] is gate and up: rows i and i + rows / 2 go together
-    int bound_add;        // what the number of columns adds to the exponent of the gated product's bound
     int *pair_part;       // for each block of m[0]: its largest exponent(gate) + exponent(up)
-    float *h_factor, *h_inverse; // of each token's gated product, by its bound
-    unsigned int *ticket; // zero between calls
 };
 
-constexpr int kPrepThreads = 256;
-constexpr int kPrepRows = 64;      // weight rows of a block at most
+constexpr int kPrepThreads = 128;
+constexpr int kPrepRows = 128;     // weight rows of a block at most
 constexpr int kPrepKeep = 4;       // pieces of eight columns a thread keeps in registers
 constexpr int kExpMin = -112, kExpMax = 112;
 constexpr int kTcUnitExp = 9; // the codes enter as (q - z) 2^-9
@@ -80,7 +77,7 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
 {
     constexpr int WARPS = kPrepThreads / 32;
     __shared__ float part[3][WARPS];
-    __shared__ int ipart[WARPS], row_exp[kPrepRows], last;
+    __shared__ int ipart[WARPS], row_exp[kPrepRows];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
     pdl_launch_dependents();
@@ -103,21 +100,6 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
             for (int p = threadIdx.x + kPrepKeep * kPrepThreads; p < pieces; p += kPrepThreads)
                 f(p, x[p]);
         };
-        auto block_reduce = [&](float v, int slot, bool maximum) {
-#pragma unroll
-            for (int o = 16; o; o >>= 1) {
-                const float u = __shfl_xor_sync(0xffffffffu, v, o);
-                v = maximum ? fmaxf(v, u) : v + u;
-            }
-            if (lane == 0)
-                part[slot][warp] = v;
-            __syncthreads();
-            v = part[slot][0];
-#pragma unroll
-            for (int i = 1; i < WARPS; i++)
-                v = maximum ? fmaxf(v, part[slot][i]) : v + part[slot][i];
-            return v;
-        };
         float inv = 1.0f;
         if (a.norm_w) {
             float ss = 0.0f;
@@ -126,40 +108,77 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
                 for (int i = 0; i < 8; i++)
                     ss = fmaf(prep_get(v, i), prep_get(v, i), ss);
             });
-            inv = rsqrtf(block_reduce(ss, 0, false) / static_cast<float>(a.K) + a.eps);
+#pragma unroll
+            for (int o = 16; o; o >>= 1)
+                ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (lane == 0)
+                part[2][warp] = ss;
+            __syncthreads();
+            ss = 0.0f;
+#pragma unroll
+            for (int i = 0; i < WARPS; i++)
+                ss += part[2][i];
+            inv = rsqrtf(ss / static_cast<float>(a.K) + a.eps);
         }
-        auto value = [&](int p, const uint4 &v, int i) {
-            float f = prep_get(v, i);
-            if (a.norm_w)
-                f = f * inv * (a.offset + __bfloat162float(a.norm_w[p * 8 + i]));
-            return f;
-        };
-        float top = 0.0f;
-        each([&](int p, const uint4 &v) {
+        // the eight columns of a piece, normed
+        auto values = [&](int p, const uint4 &v, float (&f)[8]) {
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                top = fmaxf(top, finite_abs(value(p, v, i)));
+                f[i] = prep_get(v, i);
+            if (a.norm_w) {
+                const __nv_bfloat16 *w = a.norm_w + p * 8;
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    f[i] = f[i] * inv * (a.offset + __bfloat162float(w[i]));
+            }
+        };
+        float top = 0.0f, ss = 0.0f;
+        each([&](int p, const uint4 &v) {
+            float f[8];
+            values(p, v, f);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float c = finite_abs(f[i]);
+                top = fmaxf(top, c);
+                ss = fmaf(c, c, ss);
+            }
         });
-        const int e = max(kExpMin, min(kExpMax, log2_floor(block_reduce(top, 1, true)) - 13));
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        }
+        if (lane == 0) {
+            part[0][warp] = top;
+            part[1][warp] = ss;
+        }
+        __syncthreads();
+        top = ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < WARPS; i++) {
+            top = fmaxf(top, part[0][i]);
+            ss += part[1][i];
+        }
+        const int top_exp = log2_floor(top), e = max(kExpMin, min(kExpMax, top_exp - 13));
         const float down = pow2f(-e);
-        float ss = 0.0f;
         uint4 *out = reinterpret_cast<uint4 *>(a.x16 + static_cast<size_t>(t) * a.K);
         each([&](int p, const uint4 &v) {
+            float f[8];
+            values(p, v, f);
             __half2 o[4];
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                const float f0 = value(p, v, i) * down, f1 = value(p, v, i + 1) * down;
-                const float c0 = finite_abs(f0), c1 = finite_abs(f1);
-                ss = fmaf(c0, c0, fmaf(c1, c1, ss));
-                o[i / 2] = __floats2half2_rn(f0, f1);
-            }
+            for (int i = 0; i < 4; i++)
+                o[i] = __floats2half2_rn(f[2 * i] * down, f[2 * i + 1] * down);
             out[p] = *reinterpret_cast<uint4 *>(o);
         });
-        ss = block_reduce(ss, 2, false);
         if (threadIdx.x == 0) {
             a.factor[t] = pow2f(e);
-            // sqrt(ss) < 2^((k + 1) / 2) with k = floor(log2 ss), and one more for the roundings of the sum
-            a.l[t] = ss > 0.0f ? e + ((log2_floor(ss) + 3) >> 1) : kExpMin;
+            // sqrt(ss) < 2^((k + 1) / 2) with k = floor(log2 ss), and one more for the roundings of the sum; where the squares leave
+            // the range of f32, sqrt(K) times the largest element
+            int l = (log2_floor(ss) + 3) >> 1;
+            if (top_exp > 50 || top_exp < -50)
+                l = top_exp + 1 + (32 - __clz(a.K) + 1) / 2;
+            a.l[t] = l;
         }
     } else {
         int b = blockIdx.x - a.T;
@@ -176,24 +195,38 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
             const bool there = i < (pair ? half_rows : m.rows);
             const size_t row = there ? static_cast<size_t>(i) + (pair && r >= half_block ? half_rows : 0) : 0;
             const uint16_t *s = m.scales + row * m.groups;
-            auto eight = [&](int g) { // groups g .. g + 7, zero behind the last one
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (m.vec) {
-                    v = *reinterpret_cast<const uint4 *>(s + g);
-                } else {
-                    uint32_t u[4] = {};
+            const uint8_t *z = m.zeros + row * m.groups;
+            auto scales = [&](int g) { // of groups g .. g + 7, zero behind the last one
+                if (m.vec)
+                    return *reinterpret_cast<const uint4 *>(s + g);
+                uint32_t u[4] = {};
 #pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        if (g + j < m.groups)
-                            u[j / 2] |= static_cast<uint32_t>(s[g + j]) << (j % 2 * 16);
-                    v = make_uint4(u[0], u[1], u[2], u[3]);
-                }
-                return v;
+                for (int j = 0; j < 8; j++)
+                    if (g + j < m.groups)
+                        u[j / 2] |= static_cast<uint32_t>(s[g + j]) << (j % 2 * 16);
+                return make_uint4(u[0], u[1], u[2], u[3]);
             };
+            auto zeros = [&](int g) {
+                if (m.vec)
+                    return *reinterpret_cast<const uint2 *>(z + g);
+                uint32_t u[2] = {};
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (g + j < m.groups)
+                        u[j / 4] |= static_cast<uint32_t>(z[g + j]) << (j % 4 * 8);
+                return make_uint2(u[0], u[1]);
+            };
+            uint4 s0 = make_uint4(0, 0, 0, 0); // this lane's first groups; a row of more than 256 is read again below
+            uint2 z0 = make_uint2(0, 0);
+            if (sub * 8 < m.groups) {
+                s0 = scales(sub * 8);
+                if (m.zeros)
+                    z0 = zeros(sub * 8);
+            }
             float top = 0.0f, low = 3.4e38f;
             bool odd = false; // an infinity or NaN
             for (int g = sub * 8; g < m.groups; g += m.lanes * 8) {
-                const uint4 v = eight(g);
+                const uint4 v = g == sub * 8 ? s0 : scales(g);
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const float f = fabsf(prep_get(v, j)), c = finite_abs(f);
@@ -215,21 +248,14 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
             const float down = pow2f(-c);
             if (there) {
                 for (int g = sub * 8; g < m.groups; g += m.lanes * 8) {
-                    const uint4 v = eight(g);
+                    const uint4 v = g == sub * 8 ? s0 : scales(g);
                     __half2 o[4];
 #pragma unroll
                     for (int j = 0; j < 4; j++)
                         o[j] = __floats2half2_rn(prep_get(v, 2 * j) * down, prep_get(v, 2 * j + 1) * down);
                     *reinterpret_cast<uint4 *>(m.scales16 + row * m.pitch + g) = *reinterpret_cast<uint4 *>(o);
-                    if (m.zeros) {
-                        const uint8_t *z = m.zeros + row * m.groups + g;
-                        uint32_t u[2] = {};
-#pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            if (g + j < m.groups)
-                                u[j / 4] |= static_cast<uint32_t>(z[j]) << (j % 4 * 8);
-                        *reinterpret_cast<uint2 *>(m.zeros8 + row * m.pitch + g) = make_uint2(u[0], u[1]);
-                    }
+                    if (m.zeros)
+                        *reinterpret_cast<uint2 *>(m.zeros8 + row * m.pitch + g) = g == sub * 8 ? z0 : zeros(g);
                 }
                 if (sub == 0)
                     m.factor[row] = narrow ? pow2f(c + kTcUnitExp) : -pow2f(c + kTcUnitExp);
@@ -252,32 +278,6 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
                 a.pair_part[b] = top;
             }
         }
-    }
-    if (!a.pair)
-        return;
-    // the block that is done last knows the bound of every token's gated product
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        __threadfence();
-        last = atomicInc(a.ticket, gridDim.x - 1) == gridDim.x - 1; // and leaves the ticket at zero
-    }
-    __syncthreads();
-    if (!last)
-        return;
-    __threadfence();
-    int top = -4000;
-    for (int i = threadIdx.x; i < a.m[0].blocks; i += kPrepThreads)
-        top = max(top, __ldcg(a.pair_part + i));
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0)
-        ipart[warp] = top;
-    __syncthreads();
-    for (int i = 0; i < WARPS; i++)
-        top = max(top, ipart[i]);
-    for (int t = threadIdx.x; t < a.T; t += kPrepThreads) {
-        const int e = max(kExpMin, min(kExpMax, 2 * __ldcg(a.l + t) + top + a.bound_add));
-        a.h_factor[t] = pow2f(e);
-        a.h_inverse[t] = pow2f(-e);
     }
 }
 

@@ -170,10 +170,18 @@ struct TcOperands {
     const uint16_t *scales; // f16 (rows, pitch)
     const uint8_t *zeros;   // (rows, pitch) or null: 8
     const float *row;       // factor of a weight row's sums; negative: its scales are of wide range
-    const float *token;     // factor of a token
-    const float *h_inverse; // gated: write the product in f16, times this; null: in bf16
+    const float *token;     // factor of a token; or null: the tokens are a gated product, scaled by its bound
     int pitch;
+    int out_f16;           // gated: write the product in f16, scaled by its bound
+    const int *l;          // 2-norm of the (gated product's) tokens <= 2^l
+    const int *pair_part;  // its largest is the largest exponent(gate) + exponent(up)
+    int parts, bound_add;  // what the number of columns adds to the bound
 };
+// Exponent of the scale of a token's gated product: the product is below 2^(exponent + 15).
+__device__ __forceinline__ int tc_bound(int l, int pair_and_columns)
+{
+    return max(kExpMin, min(kExpMax, 2 * l + pair_and_columns));
+}
 
 struct TcShape {
     int n_out, T, K, G_log; // G_log: log2 of the group
@@ -193,17 +201,14 @@ __device__ __forceinline__ void tc_tile(const TcShape &s, int item, int &wt, int
 
 // One element of the result: v, or act(v) u; in bf16, or scaled by its bound in f16 for the product that follows.
 template <bool GATED>
-__device__ __forceinline__ void tc_store(void *out, const TcShape &s, const TcOperands &w, int act, int t, int feature, float v, float u)
+__device__ __forceinline__ uint16_t tc_result(const TcOperands &w, int bound, int act, int t, float v, float u)
 {
-    const size_t at = static_cast<size_t>(t) * s.n_out + feature;
     if constexpr (GATED) {
         v = w4_activation(v, act) * u;
-        if (w.h_inverse) {
-            static_cast<__half *>(out)[at] = __float2half_rn(v * __ldg(w.h_inverse + t));
-            return;
-        }
+        if (w.out_f16)
+            return __half_as_ushort(__float2half_rn(v * pow2f(-tc_bound(__ldg(w.l + t), bound))));
     }
-    static_cast<__nv_bfloat16 *>(out)[at] = __float2bfloat16_rn(v);
+    return __bfloat16_as_ushort(__float2bfloat16_rn(v));
 }
 
 template <int CG, int N_TILE, bool GATED>
@@ -225,6 +230,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
     uint64_t *acc_full = empty + kTcStages, *acc_empty = acc_full + NBUF;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + NBUF);
     volatile uint32_t *abort_flag = tmem_slot + 1;
+    int *epi_max = reinterpret_cast<int *>(tmem_slot + 2); // eight
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31; // warp: known to be uniform
     const int rank = CG > 1 || s.split > 1 ? static_cast<int>(cluster_rank()) : 0;
@@ -277,6 +283,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
     const int block_feature = CG > 1 ? rank * FEATURES : 0, block_token = CG > 1 ? rank * (N_TILE / CG) : 0;
 
     bool ok = true;
+    int split_bound = 0;
     if ((warp == 0 || warp == 3) && lane == 0) {
         const uint64_t policy = policy_evict_last();
         uint32_t n = 0;
@@ -479,6 +486,21 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
         const int q = warp & 3, part = (warp - kTcEpilogueWarp) >> 2;
         constexpr int COLS = N_TILE / 2; // of this warp
         const int lane_feature = GATED ? q * 16 + (lane & 15) : q * 32 + lane;
+        const bool by_bound = GATED ? w.out_f16 != 0 : w.token == nullptr;
+        int bound = 0;
+        if (by_bound) {
+            int top = -4000;
+            for (int i = threadIdx.x - 32 * kTcEpilogueWarp; i < w.parts; i += 256)
+                top = max(top, __ldg(w.pair_part + i));
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0)
+                epi_max[warp - kTcEpilogueWarp] = top;
+            named_barrier_and(true);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                top = max(top, epi_max[i]);
+            bound = split_bound = top + w.bound_add;
+        }
         uint32_t use = 0;
         for (int item = item0; item < items; item += item_step, use++) {
             int wt, tt;
@@ -509,10 +531,24 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                 }
                 break; // one tile a block; summed below
             }
-#pragma unroll 2
+            const bool whole = token0 + COLS <= s.T && feature - lane_feature + FEATURES <= s.n_out;
+            uint16_t *o = static_cast<uint16_t *>(out) + static_cast<size_t>(token0 + (GATED && lane >= 16 ? 1 : 0)) * s.n_out + feature;
             for (int c = 0; c < COLS; c += 16) {
                 uint32_t v[16];
                 tmem_ld16(acc + c, v);
+                // the factors of sixteen tokens (the arrays are padded), one address for the warp
+                float tf[16];
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    if (GATED || !by_bound) {
+                        const float4 f = __ldg(reinterpret_cast<const float4 *>(w.token + token0 + c + i));
+                        tf[i] = f.x, tf[i + 1] = f.y, tf[i + 2] = f.z, tf[i + 3] = f.w;
+                    } else {
+                        const int4 l = __ldg(reinterpret_cast<const int4 *>(w.l + token0 + c + i));
+                        tf[i] = pow2f(tc_bound(l.x, bound)), tf[i + 1] = pow2f(tc_bound(l.y, bound));
+                        tf[i + 2] = pow2f(tc_bound(l.z, bound)), tf[i + 3] = pow2f(tc_bound(l.w, bound));
+                    }
+                }
                 tmem_ld_wait_16(v);
                 if (c + 16 == COLS) {
                     tc_fence_before();
@@ -526,19 +562,20 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                     const bool up = lane >= 16;
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
-                        const float give = __uint_as_float(up ? v[i] : v[i + 1]), got = __shfl_xor_sync(0xffffffffu, give, 16);
+                        const float even = __uint_as_float(v[i]), uneven = __uint_as_float(v[i + 1]);
+                        const float got = __shfl_xor_sync(0xffffffffu, up ? even : uneven, 16), f = up ? tf[i + 1] : tf[i];
                         const int t = token0 + c + i + (up ? 1 : 0);
-                        if (feature < s.n_out && t < s.T) {
-                            const float f = __ldg(w.token + t);
-                            tc_store<true>(out, s, w, act, t, feature, (up ? got : __uint_as_float(v[i])) * f * row_f,
-                                           (up ? __uint_as_float(v[i + 1]) : got) * f * row_u);
-                        }
+                        if (whole || (feature < s.n_out && t < s.T))
+                            *o = tc_result<true>(w, bound, act, t, (up ? got : even) * f * row_f, (up ? uneven : got) * f * row_u);
+                        o += 2 * static_cast<size_t>(s.n_out);
                     }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        if (feature < s.n_out && token0 + c + i < s.T)
-                            tc_store<false>(out, s, w, act, token0 + c + i, feature, __uint_as_float(v[i]) * __ldg(w.token + token0 + c + i) * row_f, 0.0f);
+                    for (int i = 0; i < 16; i++) {
+                        if (whole || (feature < s.n_out && token0 + c + i < s.T))
+                            *o = tc_result<false>(w, bound, act, token0 + c + i, __uint_as_float(v[i]) * tf[i] * row_f, 0.0f);
+                        o += s.n_out;
+                    }
                 }
             }
         }
@@ -567,9 +604,9 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                 if (GATED)
                     u += ld_cluster_f32(red + (c * kTcRows + row + 16) * 4, r);
             }
-            const float t = __ldg(w.token + token);
-            tc_store<GATED>(out, s, w, act, token, feature, v * t * fabsf(__ldg(w.row + feature)),
-                            GATED ? u * t * fabsf(__ldg(w.row + s.n_out + feature)) : 0.0f);
+            const float t = GATED || w.token ? __ldg(w.token + token) : pow2f(tc_bound(__ldg(w.l + token), split_bound));
+            static_cast<uint16_t *>(out)[static_cast<size_t>(token) * s.n_out + feature] =
+                tc_result<GATED>(w, split_bound, act, token, v * t * fabsf(__ldg(w.row + feature)), GATED ? u * t * fabsf(__ldg(w.row + s.n_out + feature)) : 0.0f);
         }
     }
     if (*abort_flag)
