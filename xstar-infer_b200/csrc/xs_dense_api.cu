@@ -339,7 +339,7 @@ TcScratch plan_scratch(const XsMoeW4 *first, const XsMoeW4 *second, int T, size_
     };
     p.x16 = take(static_cast<size_t>(T) * first->cols * 2);
     for (size_t *o : {&p.token, &p.l})
-        *o = take(static_cast<size_t>(T) * 4 + 1024); // a whole tile of tokens may be read
+        *o = take(static_cast<size_t>(T) * 4);
     p.part = take(static_cast<size_t>(first->rows) * 4);
     const XsMoeW4 *w[2] = {first, second};
     for (int i = 0; i < 2; i++) {

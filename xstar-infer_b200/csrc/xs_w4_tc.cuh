@@ -52,7 +52,7 @@ __host__ __device__ constexpr int tc_raw_stages(int cg, int n_tile)
 }
 __host__ __device__ constexpr int tc_smem_bytes(int cg, int n_tile)
 {
-    return 1024 + tc_raw_stages(cg, n_tile) * kTcRawBytes + kTcStages * tc_x_bytes(cg, n_tile) + 512;
+    return 1024 + tc_raw_stages(cg, n_tile) * kTcRawBytes + kTcStages * tc_x_bytes(cg, n_tile) + 512 + 4 * 256 * 4; // barriers; factors of two tiles' tokens
 }
 
 __device__ __forceinline__ bool elect_one()
@@ -201,12 +201,12 @@ __device__ __forceinline__ void tc_tile(const TcShape &s, int item, int &wt, int
 
 // One element of the result: v, or act(v) u; in bf16, or scaled by its bound in f16 for the product that follows.
 template <bool GATED>
-__device__ __forceinline__ uint16_t tc_result(const TcOperands &w, int bound, int act, int t, float v, float u)
+__device__ __forceinline__ uint16_t tc_result(const TcOperands &w, int act, float inverse, float v, float u)
 {
     if constexpr (GATED) {
         v = w4_activation(v, act) * u;
         if (w.out_f16)
-            return __half_as_ushort(__float2half_rn(v * pow2f(-tc_bound(__ldg(w.l + t), bound))));
+            return __half_as_ushort(__float2half_rn(v * inverse));
     }
     return __bfloat16_as_ushort(__float2bfloat16_rn(v));
 }
@@ -231,6 +231,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + NBUF);
     volatile uint32_t *abort_flag = tmem_slot + 1;
     int *epi_max = reinterpret_cast<int *>(tmem_slot + 2); // eight
+    float *token_smem = reinterpret_cast<float *>(bars) + 128; // [tile parity][factor, inverse of the product's factor][256]
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31; // warp: known to be uniform
     const int rank = CG > 1 || s.split > 1 ? static_cast<int>(cluster_rank()) : 0;
@@ -283,7 +284,6 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
     const int block_feature = CG > 1 ? rank * FEATURES : 0, block_token = CG > 1 ? rank * (N_TILE / CG) : 0;
 
     bool ok = true;
-    int split_bound = 0;
     if ((warp == 0 || warp == 3) && lane == 0) {
         const uint64_t policy = policy_evict_last();
         uint32_t n = 0;
@@ -499,13 +499,23 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 top = max(top, epi_max[i]);
-            bound = split_bound = top + w.bound_add;
+            bound = top + w.bound_add;
         }
         uint32_t use = 0;
         for (int item = item0; item < items; item += item_step, use++) {
             int wt, tt;
             tc_tile(s, item, wt, tt);
             const uint32_t buf = use % NBUF;
+            // the factors of this tile's tokens, into the place the tile before last has left
+            float *factor = token_smem + (use & 1) * 512, *inverse = factor + 256;
+            {
+                const int j = threadIdx.x - 32 * kTcEpilogueWarp, t = min(tt * N_TILE + j, s.T - 1);
+                if (j < N_TILE) {
+                    const int e = by_bound ? tc_bound(__ldg(w.l + t), bound) : 0;
+                    factor[j] = GATED || !by_bound ? __ldg(w.token + t) : pow2f(e);
+                    inverse[j] = pow2f(-e);
+                }
+            }
             // one warp asks, sleeping in between, and the others wait at a barrier that costs no issue slots
             if (warp == kTcEpilogueWarp)
                 ok = warp_sleep_wait(&acc_full[buf], (use / NBUF) & 1, abort_flag);
@@ -536,17 +546,14 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
             for (int c = 0; c < COLS; c += 16) {
                 uint32_t v[16];
                 tmem_ld16(acc + c, v);
-                // the factors of sixteen tokens (the arrays are padded), one address for the warp
-                float tf[16];
+                float tf[16], ti[GATED ? 16 : 1];
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
-                    if (GATED || !by_bound) {
-                        const float4 f = __ldg(reinterpret_cast<const float4 *>(w.token + token0 + c + i));
-                        tf[i] = f.x, tf[i + 1] = f.y, tf[i + 2] = f.z, tf[i + 3] = f.w;
-                    } else {
-                        const int4 l = __ldg(reinterpret_cast<const int4 *>(w.l + token0 + c + i));
-                        tf[i] = pow2f(tc_bound(l.x, bound)), tf[i + 1] = pow2f(tc_bound(l.y, bound));
-                        tf[i + 2] = pow2f(tc_bound(l.z, bound)), tf[i + 3] = pow2f(tc_bound(l.w, bound));
+                    const float4 f = *reinterpret_cast<const float4 *>(factor + part * COLS + c + i);
+                    tf[i] = f.x, tf[i + 1] = f.y, tf[i + 2] = f.z, tf[i + 3] = f.w;
+                    if constexpr (GATED) {
+                        const float4 g = *reinterpret_cast<const float4 *>(inverse + part * COLS + c + i);
+                        ti[i] = g.x, ti[i + 1] = g.y, ti[i + 2] = g.z, ti[i + 3] = g.w;
                     }
                 }
                 tmem_ld_wait_16(v);
@@ -566,14 +573,14 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                         const float got = __shfl_xor_sync(0xffffffffu, up ? even : uneven, 16), f = up ? tf[i + 1] : tf[i];
                         const int t = token0 + c + i + (up ? 1 : 0);
                         if (whole || (feature < s.n_out && t < s.T))
-                            *o = tc_result<true>(w, bound, act, t, (up ? got : even) * f * row_f, (up ? uneven : got) * f * row_u);
+                            *o = tc_result<true>(w, act, up ? ti[i + 1] : ti[i], (up ? got : even) * f * row_f, (up ? uneven : got) * f * row_u);
                         o += 2 * static_cast<size_t>(s.n_out);
                     }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
                         if (whole || (feature < s.n_out && token0 + c + i < s.T))
-                            *o = tc_result<false>(w, bound, act, token0 + c + i, __uint_as_float(v[i]) * tf[i] * row_f, 0.0f);
+                            *o = tc_result<false>(w, act, 1.0f, __uint_as_float(v[i]) * tf[i] * row_f, 0.0f);
                         o += s.n_out;
                     }
                 }
@@ -604,9 +611,9 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                 if (GATED)
                     u += ld_cluster_f32(red + (c * kTcRows + row + 16) * 4, r);
             }
-            const float t = GATED || w.token ? __ldg(w.token + token) : pow2f(tc_bound(__ldg(w.l + token), split_bound));
+            const float t = token_smem[c], inverse = token_smem[256 + c]; // the one tile's
             static_cast<uint16_t *>(out)[static_cast<size_t>(token) * s.n_out + feature] =
-                tc_result<GATED>(w, split_bound, act, token, v * t * fabsf(__ldg(w.row + feature)), GATED ? u * t * fabsf(__ldg(w.row + s.n_out + feature)) : 0.0f);
+                tc_result<GATED>(w, act, inverse, v * t * fabsf(__ldg(w.row + feature)), GATED ? u * t * fabsf(__ldg(w.row + s.n_out + feature)) : 0.0f);
         }
     }
     if (*abort_flag)
