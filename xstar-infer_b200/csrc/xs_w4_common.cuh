@@ -112,4 +112,14 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr, uint32_t rank)
     return v;
 }
 
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr, uint32_t rank)
+{
+    float4 v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr), "r"(rank)
+                 : "memory");
+    return v;
+}
+
 } // namespace xs

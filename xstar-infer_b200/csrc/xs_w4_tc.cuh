@@ -594,26 +594,40 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
     __syncwarp();
     if (CG == 1 && s.split > 1)
         cluster_barrier();
-    if (CG == 1 && s.split > 1 && warp >= kTcEpilogueWarp) {
-        // this block's tokens of the tile: the slices' sums in the order of the slices
+    if (CG == 1 && s.split > 1) {
+        // this block's tokens of the tile, four features a thread: the slices' sums in the order of the slices
         int wt, tt;
         tc_tile(s, item0, wt, tt);
         const uint32_t red = smem_u32(smem);
         const int share = N_TILE / s.split;
-        for (int i = threadIdx.x - 32 * kTcEpilogueWarp; i < share * FEATURES; i += 256) {
-            const int c = rank * share + i / FEATURES, f = i % FEATURES, feature = wt * FEATURES + f, token = tt * N_TILE + c;
+        for (int i = threadIdx.x; i < share * (FEATURES / 4); i += kTcThreads) {
+            const int c = rank * share + i / (FEATURES / 4), f = i % (FEATURES / 4) * 4, feature = wt * FEATURES + f, token = tt * N_TILE + c;
             if (feature >= s.n_out || token >= s.T)
                 continue;
-            const int row = GATED ? (f >> 4) * 32 + (f & 15) : f;
-            float v = 0.0f, u = 0.0f;
-            for (int r = 0; r < s.split; r++) {
-                v += ld_cluster_f32(red + (c * kTcRows + row) * 4, r);
-                if (GATED)
-                    u += ld_cluster_f32(red + (c * kTcRows + row + 16) * 4, r);
-            }
+            const uint32_t at = red + (c * kTcRows + (GATED ? (f >> 4) * 32 + (f & 15) : f)) * 4;
+            float4 v[8], u[GATED ? 8 : 1];
+#pragma unroll
+            for (int r = 0; r < 8; r++)
+                if (r < s.split) {
+                    v[r] = ld_cluster_f32x4(at, r);
+                    if constexpr (GATED)
+                        u[r] = ld_cluster_f32x4(at + 64, r);
+                }
+            float sv[4] = {}, su[4] = {};
+#pragma unroll
+            for (int r = 0; r < 8; r++)
+                if (r < s.split) {
+                    sv[0] += v[r].x, sv[1] += v[r].y, sv[2] += v[r].z, sv[3] += v[r].w;
+                    if constexpr (GATED)
+                        su[0] += u[r].x, su[1] += u[r].y, su[2] += u[r].z, su[3] += u[r].w;
+                }
             const float t = token_smem[c], inverse = token_smem[256 + c]; // the one tile's
-            static_cast<uint16_t *>(out)[static_cast<size_t>(token) * s.n_out + feature] =
-                tc_result<GATED>(w, act, inverse, v * t * fabsf(__ldg(w.row + feature)), GATED ? u * t * fabsf(__ldg(w.row + s.n_out + feature)) : 0.0f);
+            uint16_t *o = static_cast<uint16_t *>(out) + static_cast<size_t>(token) * s.n_out + feature;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (feature + j < s.n_out)
+                    o[j] = tc_result<GATED>(w, act, inverse, sv[j] * t * fabsf(__ldg(w.row + feature + j)),
+                                            GATED ? su[j] * t * fabsf(__ldg(w.row + s.n_out + feature + j)) : 0.0f);
         }
     }
     if (*abort_flag)
