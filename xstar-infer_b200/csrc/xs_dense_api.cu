@@ -245,8 +245,9 @@ struct TcPlan {
     xs::TcShape shape{};
 };
 
-// Tile and split by estimated cycles of the busiest block: a 64-column block of a tile takes the larger of the MMAs (2 cycles a
-// token of a 128-row tile) and of the conversion of its codes (180), a tile's start, sum and store a fixed part more.
+// Tile and split by the estimated time of the busiest block, from measurements (microseconds): a 128-column block of a tile takes
+// 0.42 with 32 tokens, 0.46 with 64, 0.6 with 128, 0.8 on a pair of SMs with 256; a tile's start, sums and store 2 and
+// 0.006 a token; meeting the other slices of K 1.6 more.
 TcPlan plan_tc(const XsMoeW4 *w, bool gated, int T, int sms)
 {
     const int n_out = gated ? w->rows / 2 : w->rows, K = w->cols;
@@ -254,7 +255,7 @@ TcPlan plan_tc(const XsMoeW4 *w, bool gated, int T, int sms)
     TcPlan best;
     float best_cost = 0.0f;
     for (int cg = 1; cg <= 2; cg++)
-        for (int n_tile = cg == 1 ? 32 : 256; n_tile <= (cg == 1 ? 128 : 256); n_tile *= 2)
+        for (int n_tile = cg == 1 ? 32 : 128; n_tile <= (cg == 1 ? 128 : 256); n_tile *= 2)
             for (int split = 1; split <= (cg == 1 ? 8 : 1); split *= 2) {
                 const int raw_per = (all_raw + split - 1) / split;
                 if (raw_per * (split - 1) >= all_raw)
@@ -265,13 +266,14 @@ TcPlan plan_tc(const XsMoeW4 *w, bool gated, int T, int sms)
                 const int features = (gated ? xs::kTcRows / 2 : xs::kTcRows) * cg;
                 p.shape = {n_out, T, K, w->group == 32 ? 5 : w->group == 64 ? 6 : 7, (n_out + features - 1) / features, (T + n_tile - 1) / n_tile, split};
                 const long items = static_cast<long>(p.shape.w_tiles) * p.shape.t_tiles;
-                const int slots = sms / (cg * split);
+                // clusters of eight whole SMs do not fit everywhere
+                const int slots = split == 8 ? sms / 8 * 3 / 4 : sms / (cg * split);
                 if (split > 1 && items > slots)
                     break; // a split block has one tile
                 const long rounds = (items + slots - 1) / slots;
                 p.grid = static_cast<int>(items < slots ? items : slots) * cg * split;
-                const float mma = 2.0f * n_tile, block = mma > 180.0f ? mma : 180.0f;
-                const float cost = rounds * (raw_per * 4 * block + 1500.0f + 8.0f * n_tile + (split > 1 ? 1500.0f : 0.0f));
+                const float block = cg == 2 ? (n_tile == 128 ? 0.48f : 0.8f) : n_tile == 128 ? 0.6f : n_tile == 64 ? 0.46f : 0.42f;
+                const float cost = rounds * (raw_per * 2 * block + 2.0f + 0.006f * n_tile) + (split > 1 ? 1.6f : 0.0f);
                 if (best.grid == 0 || cost < best_cost) {
                     best = p;
                     best_cost = cost;
@@ -303,6 +305,8 @@ int launch_tc(const XsMoeW4 *w, const void *x16, int T, void *out, const xs::TcO
     if (int rc = device_info(&di))
         return rc;
     const TcPlan p = plan_tc(w, GATED, T, di.sms);
+    if (p.cg == 2 && p.n_tile == 128)
+        return launch_tc_t<2, 128, GATED>(w, p, x16, out, ops, act, status, st);
     if (p.cg == 2)
         return launch_tc_t<2, 256, GATED>(w, p, x16, out, ops, act, status, st);
     if (p.n_tile == 128)
@@ -368,6 +372,9 @@ int bound_exponent(int cols)
 int launch_prepare(const XsMoeW4 *first, bool pair, const XsMoeW4 *second, const XsMoeBlockNorms *norm, const void *x, int T, uint8_t *ws,
                    const TcScratch &p, cudaStream_t st, int *pair_parts = nullptr)
 {
+    DeviceInfo di;
+    if (int rc = device_info(&di))
+        return rc;
     xs::PrepareArgs a{};
     a.x = static_cast<const __nv_bfloat16 *>(x);
     if (norm) {
@@ -399,7 +406,10 @@ int launch_prepare(const XsMoeW4 *first, bool pair, const XsMoeW4 *second, const
         while (m.lanes < 32 && m.lanes * 8 < m.groups)
             m.lanes *= 2;
         const int at_once = xs::kPrepThreads / m.lanes;
-        m.per_block = at_once < xs::kPrepRows ? at_once : xs::kPrepRows;
+        // four rows a thread where there are enough of them for every SM
+        m.per_block = at_once;
+        if (m.rows > 8 * di.sms * at_once)
+            m.per_block = 4 * at_once < xs::kPrepRows ? 4 * at_once : xs::kPrepRows;
         const int rows = i == 0 && pair ? m.rows / 2 : m.rows, per = i == 0 && pair ? m.per_block / 2 : m.per_block;
         m.blocks = (rows + per - 1) / per;
         blocks += m.blocks;

@@ -189,44 +189,55 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
         const bool pair = which == 0 && a.pair;
         const int half_rows = m.rows / 2, half_block = m.per_block / 2;
         const int sub = lane & (m.lanes - 1);
-        for (int r = threadIdx.x / m.lanes; r < m.per_block; r += kPrepThreads / m.lanes) {
+        const int stride = kPrepThreads / m.lanes;
+        struct Row {
+            bool there;
+            size_t row;
+            uint4 s0; // scales of this lane's first groups; a row of more than 256 groups is read again below
+            uint2 z0;
+        };
+        auto scales = [&](const Row &w, int g) { // of groups g .. g + 7, zero behind the last one
+            const uint16_t *s = m.scales + w.row * m.groups;
+            if (m.vec)
+                return *reinterpret_cast<const uint4 *>(s + g);
+            uint32_t u[4] = {};
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (g + j < m.groups)
+                    u[j / 2] |= static_cast<uint32_t>(s[g + j]) << (j % 2 * 16);
+            return make_uint4(u[0], u[1], u[2], u[3]);
+        };
+        auto zeros = [&](const Row &w, int g) {
+            const uint8_t *z = m.zeros + w.row * m.groups;
+            if (m.vec)
+                return *reinterpret_cast<const uint2 *>(z + g);
+            uint32_t u[2] = {};
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (g + j < m.groups)
+                    u[j / 4] |= static_cast<uint32_t>(z[g + j]) << (j % 4 * 8);
+            return make_uint2(u[0], u[1]);
+        };
+        auto load = [&](int r) {
+            Row w;
             // a block's first rows are gate rows, its last the up rows of the same features
             const int i = pair ? b * half_block + (r < half_block ? r : r - half_block) : b * m.per_block + r;
-            const bool there = i < (pair ? half_rows : m.rows);
-            const size_t row = there ? static_cast<size_t>(i) + (pair && r >= half_block ? half_rows : 0) : 0;
-            const uint16_t *s = m.scales + row * m.groups;
-            const uint8_t *z = m.zeros + row * m.groups;
-            auto scales = [&](int g) { // of groups g .. g + 7, zero behind the last one
-                if (m.vec)
-                    return *reinterpret_cast<const uint4 *>(s + g);
-                uint32_t u[4] = {};
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    if (g + j < m.groups)
-                        u[j / 2] |= static_cast<uint32_t>(s[g + j]) << (j % 2 * 16);
-                return make_uint4(u[0], u[1], u[2], u[3]);
-            };
-            auto zeros = [&](int g) {
-                if (m.vec)
-                    return *reinterpret_cast<const uint2 *>(z + g);
-                uint32_t u[2] = {};
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    if (g + j < m.groups)
-                        u[j / 4] |= static_cast<uint32_t>(z[g + j]) << (j % 4 * 8);
-                return make_uint2(u[0], u[1]);
-            };
-            uint4 s0 = make_uint4(0, 0, 0, 0); // this lane's first groups; a row of more than 256 is read again below
-            uint2 z0 = make_uint2(0, 0);
-            if (sub * 8 < m.groups) {
-                s0 = scales(sub * 8);
+            w.there = r < m.per_block && i < (pair ? half_rows : m.rows);
+            w.row = w.there ? static_cast<size_t>(i) + (pair && r >= half_block ? half_rows : 0) : 0;
+            w.s0 = make_uint4(0, 0, 0, 0);
+            w.z0 = make_uint2(0, 0);
+            if (w.there && sub * 8 < m.groups) {
+                w.s0 = scales(w, sub * 8);
                 if (m.zeros)
-                    z0 = zeros(sub * 8);
+                    w.z0 = zeros(w, sub * 8);
             }
+            return w;
+        };
+        auto finish = [&](const Row &w, int r) {
             float top = 0.0f, low = 3.4e38f;
             bool odd = false; // an infinity or NaN
             for (int g = sub * 8; g < m.groups; g += m.lanes * 8) {
-                const uint4 v = g == sub * 8 ? s0 : scales(g);
+                const uint4 v = g == sub * 8 ? w.s0 : scales(w, g);
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const float f = fabsf(prep_get(v, j)), c = finite_abs(f);
@@ -246,22 +257,33 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
             const bool narrow = !odd && top_exp < 100 && top_exp - log2_floor(fminf(low, top)) < 4;
             const int c = max(kExpMin, min(kExpMax, narrow ? top_exp + 1 : top_exp - 14));
             const float down = pow2f(-c);
-            if (there) {
+            if (w.there) {
                 for (int g = sub * 8; g < m.groups; g += m.lanes * 8) {
-                    const uint4 v = g == sub * 8 ? s0 : scales(g);
+                    const uint4 v = g == sub * 8 ? w.s0 : scales(w, g);
                     __half2 o[4];
 #pragma unroll
                     for (int j = 0; j < 4; j++)
                         o[j] = __floats2half2_rn(prep_get(v, 2 * j) * down, prep_get(v, 2 * j + 1) * down);
-                    *reinterpret_cast<uint4 *>(m.scales16 + row * m.pitch + g) = *reinterpret_cast<uint4 *>(o);
+                    *reinterpret_cast<uint4 *>(m.scales16 + w.row * m.pitch + g) = *reinterpret_cast<uint4 *>(o);
                     if (m.zeros)
-                        *reinterpret_cast<uint2 *>(m.zeros8 + row * m.pitch + g) = g == sub * 8 ? z0 : zeros(g);
+                        *reinterpret_cast<uint2 *>(m.zeros8 + w.row * m.pitch + g) = g == sub * 8 ? w.z0 : zeros(w, g);
                 }
                 if (sub == 0)
-                    m.factor[row] = narrow ? pow2f(c + kTcUnitExp) : -pow2f(c + kTcUnitExp);
+                    m.factor[w.row] = narrow ? pow2f(c + kTcUnitExp) : -pow2f(c + kTcUnitExp);
             }
-            if (pair && sub == 0)
-                row_exp[r] = there ? top_exp + 1 : -1000; // the row's scales are below 2^row_exp
+            if (pair && sub == 0 && r < m.per_block)
+                row_exp[r] = w.there ? top_exp + 1 : -1000; // the row's scales are below 2^row_exp
+        };
+        // four rows' loads on their way before the first is worked on
+        for (int r = static_cast<int>(threadIdx.x) / m.lanes; r - static_cast<int>(threadIdx.x) / m.lanes < m.per_block; r += 4 * stride) {
+            Row w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                w[i] = load(r + i * stride);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (i * stride + r - static_cast<int>(threadIdx.x) / m.lanes < m.per_block)
+                    finish(w[i], r + i * stride);
         }
         if (pair) {
             __syncthreads();

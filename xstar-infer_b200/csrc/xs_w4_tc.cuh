@@ -271,7 +271,10 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
         __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    pdl_wait(); // everything above touches only shared memory and TMEM
+    // Everything above touches only shared memory and TMEM.  The codes may be loaded at once: what runs before this kernel in its
+    // stream is the preparation of the tokens (or the product that made them), and the codes were there before that began.
+    if (warp != 2)
+        pdl_wait();
 
     const int all_raw = (s.K + kTcRawBlocks * kTcBlockK - 1) / (kTcRawBlocks * kTcBlockK);
     const int raw_per = (all_raw + s.split - 1) / s.split;
@@ -592,6 +595,8 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
         atomicOr(status, kStatusWaitTimeout);
     }
     __syncwarp();
+    if (warp == 2)
+        pdl_wait();
     if (CG == 1 && s.split > 1)
         cluster_barrier();
     if (CG == 1 && s.split > 1) {
