@@ -242,44 +242,74 @@ int make_tmap_rows(CUtensorMap *m, const void *x, int T, int K, uint32_t box_row
 
 struct TcPlan {
     int cg = 1, n_tile = 32, grid = 0;
+    float cost = 0.0f;
     xs::TcShape shape{};
 };
 
 // Tile and split by the estimated time of the busiest block, from measurements (microseconds): a 128-column block of a tile takes
-// 0.42 with 32 tokens, 0.46 with 64, 0.6 with 128, 0.8 on a pair of SMs with 256; a tile's start, sums and store 2 and
-// 0.006 a token; meeting the other slices of K 1.6 more.
-TcPlan plan_tc(const XsMoeW4 *w, bool gated, int T, int sms)
+// 0.42 with 32 tokens, 0.46 with 64, 0.6 with 128; on a pair of SMs 0.48 with 128 and 0.8 with 256; a tile's start, sums and
+// store 2 and 0.006 a token; meeting the other slices of K 1.6 more.
+constexpr struct {
+    int cg, n_tile;
+    float block;
+} kTcTiles[] = {{1, 32, 0.42f}, {1, 64, 0.46f}, {1, 128, 0.6f}, {2, 128, 0.48f}, {2, 256, 0.8f}};
+
+// `features` features from f0 on, with one launch; `tile`: one of kTcTiles, or -1 for the best
+TcPlan plan_tc_part(const XsMoeW4 *w, bool gated, int T, int sms, int f0, int features, int tile)
 {
-    const int n_out = gated ? w->rows / 2 : w->rows, K = w->cols;
-    const int all_raw = (K + 255) / 256;
+    const int n_out = gated ? w->rows / 2 : w->rows, K = w->cols, all_raw = (K + 255) / 256;
     TcPlan best;
-    float best_cost = 0.0f;
-    for (int cg = 1; cg <= 2; cg++)
-        for (int n_tile = cg == 1 ? 32 : 128; n_tile <= (cg == 1 ? 128 : 256); n_tile *= 2)
-            for (int split = 1; split <= (cg == 1 ? 8 : 1); split *= 2) {
-                const int raw_per = (all_raw + split - 1) / split;
-                if (raw_per * (split - 1) >= all_raw)
-                    break;
-                TcPlan p;
-                p.cg = cg;
-                p.n_tile = n_tile;
-                const int features = (gated ? xs::kTcRows / 2 : xs::kTcRows) * cg;
-                p.shape = {n_out, T, K, w->group == 32 ? 5 : w->group == 64 ? 6 : 7, (n_out + features - 1) / features, (T + n_tile - 1) / n_tile, split};
-                const long items = static_cast<long>(p.shape.w_tiles) * p.shape.t_tiles;
-                // clusters of eight whole SMs do not fit everywhere
-                const int slots = split == 8 ? sms / 8 * 3 / 4 : sms / (cg * split);
-                if (split > 1 && items > slots)
-                    break; // a split block has one tile
-                const long rounds = (items + slots - 1) / slots;
-                p.grid = static_cast<int>(items < slots ? items : slots) * cg * split;
-                const float block = cg == 2 ? (n_tile == 128 ? 0.48f : 0.8f) : n_tile == 128 ? 0.6f : n_tile == 64 ? 0.46f : 0.42f;
-                const float cost = rounds * (raw_per * 2 * block + 2.0f + 0.006f * n_tile) + (split > 1 ? 1.6f : 0.0f);
-                if (best.grid == 0 || cost < best_cost) {
-                    best = p;
-                    best_cost = cost;
-                }
-            }
+    for (int i = 0; i < 5; i++) {
+        if (tile >= 0 && i != tile)
+            continue;
+        const int cg = kTcTiles[i].cg, n_tile = kTcTiles[i].n_tile, width = (gated ? xs::kTcRows / 2 : xs::kTcRows) * cg;
+        for (int split = 1; split <= (cg == 1 ? 8 : 1); split *= 2) {
+            const int raw_per = (all_raw + split - 1) / split;
+            if (raw_per * (split - 1) >= all_raw)
+                break;
+            TcPlan p;
+            p.cg = cg;
+            p.n_tile = n_tile;
+            p.shape = {n_out, T, K, w->group == 32 ? 5 : w->group == 64 ? 6 : 7, (features + width - 1) / width, (T + n_tile - 1) / n_tile, split, f0};
+            const long items = static_cast<long>(p.shape.w_tiles) * p.shape.t_tiles;
+            // clusters of eight whole SMs do not fit everywhere
+            const int slots = split == 8 ? sms / 8 * 3 / 4 : sms / (cg * split);
+            if (split > 1 && items > slots)
+                break; // a split block has one tile
+            const long rounds = (items + slots - 1) / slots;
+            p.grid = static_cast<int>(items < slots ? items : slots) * cg * split;
+            p.cost = rounds * (raw_per * 2 * kTcTiles[i].block + 2.0f + 0.006f * n_tile) + (split > 1 ? 1.6f : 0.0f);
+            if (best.grid == 0 || p.cost < best.cost)
+                best = p;
+        }
+    }
     return best;
+}
+
+// One launch, or two: whole rounds of tiles on every SM, and what would have been a last round of few tiles in another shape.
+// Returns the number of launches.
+int plan_tc(const XsMoeW4 *w, bool gated, int T, int sms, TcPlan (&plan)[2])
+{
+    constexpr float kLaunchCost = 6.0f, kGain = 0.9f; // a second launch starts cold; the estimate has to say that it pays
+    const int n_out = gated ? w->rows / 2 : w->rows;
+    plan[0] = plan_tc_part(w, gated, T, sms, 0, n_out, -1);
+    float cost = plan[0].cost;
+    int parts = 1;
+    for (int i = 0; i < 5; i++) {
+        const int cg = kTcTiles[i].cg, n_tile = kTcTiles[i].n_tile, width = (gated ? xs::kTcRows / 2 : xs::kTcRows) * cg, slots = sms / cg;
+        const long t_tiles = (T + n_tile - 1) / n_tile, items = (n_out + width - 1) / width * t_tiles, rounds = items / slots;
+        const int first = static_cast<int>(rounds * slots / t_tiles) * width; // features of the whole rounds
+        if (rounds == 0 || first <= 0 || first >= n_out)
+            continue;
+        const TcPlan a = plan_tc_part(w, gated, T, sms, 0, first, i), b = plan_tc_part(w, gated, T, sms, first, n_out - first, -1);
+        if (a.cost + b.cost + kLaunchCost < cost * (parts == 1 ? kGain : 1.0f)) {
+            cost = a.cost + b.cost + kLaunchCost;
+            plan[0] = a;
+            plan[1] = b;
+            parts = 2;
+        }
+    }
+    return parts;
 }
 
 template <int CG, int N_TILE, bool GATED>
@@ -304,16 +334,25 @@ int launch_tc(const XsMoeW4 *w, const void *x16, int T, void *out, const xs::TcO
     DeviceInfo di;
     if (int rc = device_info(&di))
         return rc;
-    const TcPlan p = plan_tc(w, GATED, T, di.sms);
-    if (p.cg == 2 && p.n_tile == 128)
-        return launch_tc_t<2, 128, GATED>(w, p, x16, out, ops, act, status, st);
-    if (p.cg == 2)
-        return launch_tc_t<2, 256, GATED>(w, p, x16, out, ops, act, status, st);
-    if (p.n_tile == 128)
-        return launch_tc_t<1, 128, GATED>(w, p, x16, out, ops, act, status, st);
-    if (p.n_tile == 64)
-        return launch_tc_t<1, 64, GATED>(w, p, x16, out, ops, act, status, st);
-    return launch_tc_t<1, 32, GATED>(w, p, x16, out, ops, act, status, st);
+    TcPlan plan[2];
+    const int parts = plan_tc(w, GATED, T, di.sms, plan);
+    for (int i = 0; i < parts; i++) {
+        const TcPlan &p = plan[i];
+        int rc = 0;
+        if (p.cg == 2 && p.n_tile == 128)
+            rc = launch_tc_t<2, 128, GATED>(w, p, x16, out, ops, act, status, st);
+        else if (p.cg == 2)
+            rc = launch_tc_t<2, 256, GATED>(w, p, x16, out, ops, act, status, st);
+        else if (p.n_tile == 128)
+            rc = launch_tc_t<1, 128, GATED>(w, p, x16, out, ops, act, status, st);
+        else if (p.n_tile == 64)
+            rc = launch_tc_t<1, 64, GATED>(w, p, x16, out, ops, act, status, st);
+        else
+            rc = launch_tc_t<1, 32, GATED>(w, p, x16, out, ops, act, status, st);
+        if (rc)
+            return rc;
+    }
+    return 0;
 }
 
 // Which kernel: up to eight tokens the one that streams weights past the tokens, if a cluster's shared memory holds them.

@@ -187,6 +187,7 @@ struct TcShape {
     int n_out, T, K, G_log; // G_log: log2 of the group
     int w_tiles, t_tiles;   // tiles along the features and along the tokens
     int split;              // blocks that share a tile (CG = 1)
+    int f0;                 // first feature of this launch
 };
 
 // Work item -> tile.  Eight token tiles go with each weight tile before the next one, so that what runs at one time shares both.
@@ -321,7 +322,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                     break;
                 }
                 mbar_arrive_expect_tx(&raw_full[st], kTcRawBytes);
-                tma_load_3d(smem + st * kTcRawBytes, &tmap_w, &raw_full[st], r * 128, wt * FEATURES * CG + block_feature, 0, policy);
+                tma_load_3d(smem + st * kTcRawBytes, &tmap_w, &raw_full[st], r * 128, s.f0 + wt * FEATURES * CG + block_feature, 0, policy);
             }
         }
     } else if (warp == 1 && leader) {
@@ -377,7 +378,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
         auto row_at = [&](int item) {
             int wt, tt;
             tc_tile(s, item, wt, tt);
-            return static_cast<size_t>(min(wt * FEATURES * CG + block_feature + feature, s.n_out - 1)) + (GATED && lane >= 16 ? s.n_out : 0);
+            return static_cast<size_t>(min(s.f0 + wt * FEATURES * CG + block_feature + feature, s.n_out - 1)) + (GATED && lane >= 16 ? s.n_out : 0);
         };
         auto load_scales = [&]() {
             Scales r;
@@ -528,7 +529,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
             }
             tc_fence_after();
             const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16) + kTcAccCol + buf * N_TILE + part * COLS;
-            const int feature = wt * FEATURES * CG + block_feature + lane_feature, token0 = tt * N_TILE + part * COLS;
+            const int feature = s.f0 + wt * FEATURES * CG + block_feature + lane_feature, token0 = tt * N_TILE + part * COLS;
             const int f0 = min(feature, s.n_out - 1);
             const float row_f = fabsf(__ldg(w.row + f0)), row_u = GATED ? fabsf(__ldg(w.row + s.n_out + f0)) : 0.0f;
             if (CG == 1 && s.split > 1) {
@@ -606,7 +607,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
         const uint32_t red = smem_u32(smem);
         const int share = N_TILE / s.split;
         for (int i = threadIdx.x; i < share * (FEATURES / 4); i += kTcThreads) {
-            const int c = rank * share + i / (FEATURES / 4), f = i % (FEATURES / 4) * 4, feature = wt * FEATURES + f, token = tt * N_TILE + c;
+            const int c = rank * share + i / (FEATURES / 4), f = i % (FEATURES / 4) * 4, feature = s.f0 + wt * FEATURES + f, token = tt * N_TILE + c;
             if (feature >= s.n_out || token >= s.T)
                 continue;
             const uint32_t at = red + (c * kTcRows + (GATED ? (f >> 4) * 32 + (f & 15) : f)) * 4;
