@@ -223,6 +223,42 @@ def test_linear_with_infinities_nans_and_zero_scales(T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("T", [1, 8, 20, 150, 520])
+def test_linear_with_scales_and_tokens_of_very_different_size(T, zeros):
+    """groups of a row 2^14 apart, rows 2^60 apart, tokens 2^80 apart and their elements 2^20: the powers of two that bring them
+    into f16 are each row's and each token's own"""
+    g = du.gen(31 + T)
+    N, K, group = 200, 1024, 32
+    w, x = du.weight(g, N, K, group, zeros), du.bf16(g, (T, K))
+    power = torch.randint(-7, 8, w["s"].shape, generator=g, device="cuda") + torch.randint(-30, 31, (N, 1), generator=g, device="cuda")
+    w["s"] = (w["s"].float() * 2.0 ** power).to(torch.bfloat16)
+    w["s"][3] = 0.0
+    w["s"][5, ::2] = 0.0
+    x = (x.float() * 2.0 ** torch.randint(-10, 11, (T, K), generator=g, device="cuda") * 2.0 ** torch.randint(-40, 41, (T, 1), generator=g, device="cuda")).to(torch.bfloat16)
+    if T > 1:
+        x[T // 2] = 0.0
+    out, ws = du.linear(w, x)
+    du.flags(ws)
+    ref, tol = du.linear_reference(w, x)
+    du.assert_close(out, ref, tol)
+    assert (out[:, 3] == 0).all() and (T == 1 or (out[T // 2] == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [20, 100])
+def test_linear_with_a_few_more_tiles_than_sms(T):
+    g = du.gen(33)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    N, K = sms * 128 + 200, 4096
+    w, x = du.weight(g, N, K, 128, True), du.bf16(g, (T, K))
+    out, ws = du.linear(w, x)
+    du.flags(ws)
+    ref, tol = du.linear_reference(w, x)
+    du.assert_close(out, ref, tol)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [1, 20])
 def test_linear_with_offsets_beyond_32_bits(T):
     K, N, group = 65536, 70001, 128  # 2.3 GB of codes
@@ -304,6 +340,41 @@ def test_mlp_and_its_first_half_match_their_definitions(H, I, group, zeros, act)
         assert (buf[T * H:] == 77.0).all()
         if T <= du.EXACT_WEIGHT_TOKENS:  # the whole is its two halves; larger batches hand h on in f16
             assert torch.equal(out, du.linear(dn, h)[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [3, 40, 300])
+def test_mlp_with_tokens_of_very_different_size(T):
+    g = du.gen(35)
+    H, I = 512, 640
+    gu, dn = du.weight(g, 2 * I, H, 64, True, std=H**-0.5), du.weight(g, H, I, 64, False, std=I**-0.5)
+    gu["s"][7] *= 64.0  # a row, and its partner, much larger than the others
+    gu["s"][I + 7] *= 64.0
+    x = (du.bf16(g, (T, H)).float() * 2.0 ** torch.randint(-12, 7, (T, 1), generator=g, device="cuda")).to(torch.bfloat16)
+    x[1] = 0.0
+    for act in ("silu", "gelu"):
+        out, ws = du.mlp(gu, dn, x, act)
+        du.flags(ws)
+        ref, tol = du.mlp_reference(gu, dn, x, act)
+        du.assert_close(out, ref, tol)
+        assert (out[1] == 0).all()
+        for t in range(0, T, 7):
+            if t != 1:
+                assert du.rel_l2(out[t], ref[t]) < L2, t
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [2, 40])
+def test_mlp_keeps_infinities_and_nans_in_their_rows(T):
+    g = du.gen(36)
+    H, I = 256, 384
+    gu, dn = du.weight(g, 2 * I, H, 128, True, std=H**-0.5), du.weight(g, H, I, 128, True, std=I**-0.5)
+    x = du.bf16(g, (T, H))
+    clean, _ = du.mlp(gu, dn, x, "silu")
+    x[0, 9], x[1, 200] = float("nan"), float("inf")
+    out, _ = du.mlp(gu, dn, x, "silu")
+    assert out[0].isnan().all() and not out[1].isfinite().any()
+    assert torch.equal(out[2:], clean[2:])
 
 
 @pytest.mark.gpu
