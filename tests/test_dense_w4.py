@@ -259,6 +259,34 @@ def test_linear_with_a_few_more_tiles_than_sms(T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T, N", [(20, 50000), (60, 41000), (100, 60001), (700, 9000), (2600, 4000)])
+@pytest.mark.parametrize("K", [96, 256, 320, 576, 768, 832, 1152, 1408, 1696])
+def test_rows_of_few_blocks_over_many_tiles(T, N, K):
+    # an SM goes through several tiles, whose operand blocks are no multiple of the ring's stages
+    g = du.gen(K + T)
+    w, x = du.weight(g, N, K, 32, K % 3 == 0), du.bf16(g, (T, K))
+    out, ws = du.linear(w, x)
+    du.flags(ws)
+    ref, tol = du.linear_reference(w, x)
+    du.assert_close(out, ref, tol)
+    for _ in range(10):
+        assert torch.equal(du.linear(w, x)[0], out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T, H, I, group", [(5121, 576, 2752, 64), (1300, 1152, 4096, 128), (2000, 832, 3000 // 32 * 32, 32)])
+def test_mlp_of_short_rows_over_many_tiles(T, H, I, group):
+    g = du.gen(T)
+    gu, dn, x = du.weight(g, 2 * I, H, group, False, std=H**-0.5), du.weight(g, H, I, group, False, std=I**-0.5), du.bf16(g, (T, H))
+    out, ws = du.mlp(gu, dn, x, "gelu")
+    du.flags(ws)
+    ref, tol = du.mlp_reference(gu, dn, x, "gelu")
+    du.assert_close(out, ref, tol)
+    for _ in range(10):
+        assert torch.equal(du.mlp(gu, dn, x, "gelu")[0], out)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [1, 20])
 def test_linear_with_offsets_beyond_32_bits(T):
     K, N, group = 65536, 70001, 128  # 2.3 GB of codes

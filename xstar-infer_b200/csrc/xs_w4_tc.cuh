@@ -13,7 +13,7 @@
 // distributed shared memory when there are too few tiles for the SMs.
 //
 // Warps: 0, 3 token loads, alternate blocks (3 owns the TMEM allocation) | 1 MMA | 2 code loads | 4..19 dequantisation (four
-// warpgroups, every fourth operand block each, lane quarter = warp % 4) | 20..27 epilogue (lane quarter = warp % 4, half of the
+// warpgroups, one for each stage of operands, lane quarter = warp % 4) | 20..27 epilogue (lane quarter = warp % 4, half of the
 // token columns each).
 //
 // An operand block is 128 columns because every hand-over costs its roles a few hundred cycles (a poll of a barrier about 110, a
@@ -360,7 +360,9 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                 tc_done<CG>(&acc_full[buf]);
         }
     } else if (warp >= 4 && warp < kTcEpilogueWarp) {
-        const int wg = (warp - 4) >> 2, q = warp & 3; // this warpgroup's operand blocks: kb % 4 == wg
+        // Of the operand blocks, counted over all items, this warpgroup has every fourth, so that one warpgroup alone fills a stage.
+        // A parity tells one use of a stage from the next, not from the one after that: nobody may come to a stage two uses early.
+        const int wg = (warp - 4) >> 2, q = warp & 3;
         // the row of the codes (as the load laid them out) that this thread's TMEM lane holds; GATED: 16 gate rows, then their 16 up rows
         const int raw_row = GATED ? (lane >> 4) * 64 + q * 16 + (lane & 15) : q * 32 + lane;
         const int feature = GATED ? q * 16 + (lane & 15) : raw_row;
@@ -368,25 +370,27 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
         // Groups of a block (4, 2 or 1) with their scales and zero points, loaded two of this warpgroup's blocks ahead.
         const int per_block = 1 << (7 - s.G_log);
         const bool zeros = w.zeros != nullptr;
-        const int first = kb0 + ((wg - kb0) & 3);
         struct Scales {
             uint2 s;    // 16 bits each
             uint32_t z; // 8 bits each
         };
-        int ld_item = first < kb1 ? item0 : items, ld_kb = first;
-        size_t ld_row = 0; // first group of the row
         auto row_at = [&](int item) {
             int wt, tt;
             tc_tile(s, item, wt, tt);
             return static_cast<size_t>(min(s.f0 + wt * FEATURES * CG + block_feature + feature, s.n_out - 1)) + (GATED && lane >= 16 ? s.n_out : 0);
         };
+        int ld_item = item0, ld_kb = wg; // kb here and below: within the item
+        for (; ld_kb >= n_kb; ld_kb -= n_kb)
+            ld_item += item_step;
+        int item = ld_item, kb = ld_kb;
+        size_t ld_row = ld_item < items ? row_at(ld_item) * w.pitch : 0; // first group of the row
         auto load_scales = [&]() {
             Scales r;
             r.s = make_uint2(0, 0);
             r.z = 0;
             if (ld_item < items) {
-                const uint16_t *sp = w.scales + ld_row + ld_kb * per_block;
-                const uint8_t *zp = w.zeros + ld_row + ld_kb * per_block;
+                const uint16_t *sp = w.scales + ld_row + (kb0 + ld_kb) * per_block;
+                const uint8_t *zp = w.zeros + ld_row + (kb0 + ld_kb) * per_block;
                 if (per_block == 4)
                     r.s = __ldg(reinterpret_cast<const uint2 *>(sp));
                 else if (per_block == 2)
@@ -396,94 +400,82 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                 if (zeros)
                     r.z = per_block == 4 ? __ldg(reinterpret_cast<const uint32_t *>(zp)) : per_block == 2 ? __ldg(reinterpret_cast<const uint16_t *>(zp)) : __ldg(zp);
                 ld_kb += 4;
-                if (ld_kb >= kb1) {
-                    ld_kb = first;
-                    ld_item += item_step;
+                if (ld_kb >= n_kb) {
+                    for (; ld_kb >= n_kb; ld_kb -= n_kb)
+                        ld_item += item_step;
                     if (ld_item < items)
                         ld_row = row_at(ld_item) * w.pitch;
                 }
             }
             return r;
         };
-        if (ld_item < items)
-            ld_row = row_at(ld_item) * w.pitch;
         Scales cur, next, after;
 #pragma unroll 1
         for (int i = 0; i < 2; i++) {
             next = after;
             after = load_scales();
         }
-        const uint32_t tmem_lane = tmem + (static_cast<uint32_t>(q * 32) << 16);
-        uint32_t n = 0, nr = 0; // operand blocks and loads of codes before this item
-        for (int item = item0; item < items && ok; item += item_step, n += n_kb, nr += raw1 - raw0) {
+        const uint32_t dst = tmem + (static_cast<uint32_t>(q * 32) << 16) + wg * (kTcBlockK / 2);
+        uint32_t free = 1, nr = (item - item0) / item_step * (raw1 - raw0); // parity of the stage's release; loads of codes before this item
+        while (item < items && ok) {
             // Zero point 8 and scales of narrow range in the warp's 32 rows: one multiply-add a pair, n (2^15 s) 2^-24 - 8 s 2^-9, whose
             // parts are exact; else (q - z) 2^-9 first, exactly, then times s.
             const bool one_step = !zeros && __all_sync(0xffffffffu, __ldg(w.row + row_at(item)) > 0.0f);
-            // up to the last load's second block, which may not be there: its codes are given back all the same
-            for (int kb = first; kb < raw1 * kTcRawBlocks; kb += 4) {
-                const uint32_t rc = nr + (kb >> 1) - raw0, rs = rc % RAW;
-                const bool raw_there = mbar_test_wait(&raw_full[rs], (rc / RAW) & 1);
-                if (kb < kb1) {
-                    const uint32_t block = n + kb - kb0, st = block % kTcStages, free = ((block / kTcStages) & 1) ^ 1;
-                    const bool is_free = mbar_test_wait(&empty[st], free); // asked early, its answer is there after the arithmetic
-                    cur = next;
-                    next = after;
-                    after = load_scales();
-                    if (!__all_sync(0xffffffffu, raw_there || mbar_wait(&raw_full[rs], (rc / RAW) & 1, abort_flag))) {
-                        ok = false;
-                        break;
+            for (; kb < n_kb; kb += 4, free ^= 1) {
+                const uint32_t rc = nr + (kb >> 1), rs = rc % RAW;
+                const bool is_free = mbar_test_wait(&empty[wg], free), raw_there = mbar_test_wait(&raw_full[rs], (rc / RAW) & 1);
+                cur = next;
+                next = after;
+                after = load_scales();
+                // In this order: once the stage is free, the blocks up to four back have been multiplied, so the use of this place of
+                // the codes' ring before this one is over, and the parity cannot be that of the one before it.
+                ok = __all_sync(0xffffffffu, is_free || mbar_wait(&empty[wg], free, abort_flag));
+                if (ok)
+                    ok = __all_sync(0xffffffffu, (is_free && raw_there) || mbar_wait(&raw_full[rs], (rc / RAW) & 1, abort_flag));
+                if (!ok)
+                    break;
+                tc_fence_after();
+                const uint32_t codes = raw_addr + rs * kTcRawBytes;
+#pragma unroll
+                for (int h = 0; h < 4; h++) { // 32 columns: one 16-byte piece of codes, one group
+                    const int e = (h * per_block) >> 2;
+                    // past the end of K the codes read as zero, and so must the weight, whatever the zero point
+                    uint32_t sv = prmt(cur.s.x, cur.s.y, 0x1010u + 0x2222u * e);
+                    if ((kb0 + kb) * kTcBlockK + h * 32 >= s.K)
+                        sv = 0;
+                    const uint4 qv = lds128(codes + ((((kb & 1) * 4 + h) << 4) ^ swz));
+                    const uint32_t words[4] = {qv.x, qv.y, qv.z, qv.w};
+                    uint32_t a[16];
+                    if (one_step) {
+                        const uint32_t mul = f16x2_mul(sv, kTcPairMul), add = f16x2_mul(sv, kTcMinus8);
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+#pragma unroll
+                            for (int c = 0; c < 4; c++)
+                                a[j * 4 + c] = f16x2_fma(w4_pair(words[j], c), mul, add);
+                    } else {
+                        const uint32_t mz = zeros ? tc_minus_zero((cur.z >> (8 * e)) & 15u) : kTcMinus8;
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+#pragma unroll
+                            for (int c = 0; c < 4; c++)
+                                a[j * 4 + c] = f16x2_mul(f16x2_fma(w4_pair(words[j], c), kTcPairMul, mz), sv);
                     }
-                    const uint32_t codes = raw_addr + rs * kTcRawBytes, dst = tmem_lane + st * (kTcBlockK / 2);
-#pragma unroll
-                    for (int h = 0; h < 4; h++) { // 32 columns: one 16-byte piece of codes, one group
-                        const int e = (h * per_block) >> 2;
-                        // past the end of K the codes read as zero, and so must the weight, whatever the zero point
-                        uint32_t sv = prmt(cur.s.x, cur.s.y, 0x1010u + 0x2222u * e);
-                        if (kb * kTcBlockK + h * 32 >= s.K)
-                            sv = 0;
-                        const uint4 qv = lds128(codes + ((((kb & 1) * 4 + h) << 4) ^ swz));
-                        const uint32_t words[4] = {qv.x, qv.y, qv.z, qv.w};
-                        uint32_t a[16];
-                        if (one_step) {
-                            const uint32_t mul = f16x2_mul(sv, kTcPairMul), add = f16x2_mul(sv, kTcMinus8);
-#pragma unroll
-                            for (int j = 0; j < 4; j++)
-#pragma unroll
-                                for (int c = 0; c < 4; c++)
-                                    a[j * 4 + c] = f16x2_fma(w4_pair(words[j], c), mul, add);
-                        } else {
-                            const uint32_t mz = zeros ? tc_minus_zero((cur.z >> (8 * e)) & 15u) : kTcMinus8;
-#pragma unroll
-                            for (int j = 0; j < 4; j++)
-#pragma unroll
-                                for (int c = 0; c < 4; c++)
-                                    a[j * 4 + c] = f16x2_mul(f16x2_fma(w4_pair(words[j], c), kTcPairMul, mz), sv);
-                        }
-                        if (h == 0) {
-                            ok = __all_sync(0xffffffffu, is_free || mbar_wait(&empty[st], free, abort_flag));
-                            if (!ok)
-                                break;
-                            tc_fence_after();
-                        }
-                        tmem_st16(dst + h * 16, a);
-                    }
-                    if (!ok)
-                        break;
-                    tmem_st_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        tc_arrive_leader<CG>(&full[st]);
-                        mbar_arrive(&raw_empty[rs]);
-                    }
-                } else {
-                    if (!__all_sync(0xffffffffu, raw_there || mbar_wait(&raw_full[rs], (rc / RAW) & 1, abort_flag))) {
-                        ok = false;
-                        break;
-                    }
-                    if (lane == 0)
-                        mbar_arrive(&raw_empty[rs]);
+                    tmem_st16(dst + h * 16, a);
                 }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    tc_arrive_leader<CG>(&full[wg]);
+                    mbar_arrive(&raw_empty[rs]);
+                    if (kb + 1 == n_kb && !(kb & 1))
+                        mbar_arrive(&raw_empty[rs]); // the load's second block is not there
+                }
+            }
+            for (; kb >= n_kb; kb -= n_kb) {
+                item += item_step;
+                nr += raw1 - raw0;
             }
         }
     } else if (warp >= kTcEpilogueWarp) {
