@@ -62,7 +62,10 @@ def test_block_is_its_parts_and_its_definition(T, kind, post, act, scale, offset
     du.norm_residual(du.norm_args(None, x, nxt=p["pre"], next_out=xn, eps=1e-5, offset=offset))
     y, _ = du.mlp(p["gu"], p["dn"], xn, act)
     du.norm_residual(du.norm_args(y, x, p["post"] if post else None, gate, kind, None, r, eps=1e-5, scale=scale, offset=offset))
-    assert branch_error(out, r.to(du.F), x) < 2 * L2  # the block norms its rows inside the product
+    if T <= du.EXACT_WEIGHT_TOKENS:  # larger batches are normed on the way to the tensor core, without a rounding to bf16
+        assert torch.equal(out, r)
+    else:
+        assert branch_error(out, r.to(du.F), x) < 2 * L2
     ref = by_definition(p, x, act, post, None if gate is None else gate.expand(T, 640), scale, offset, 1e-5)
     assert branch_error(out, ref, x) < L2
     # over its own input, as a residual stream is kept

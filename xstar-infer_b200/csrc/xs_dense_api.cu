@@ -199,7 +199,7 @@ SmallPlan plan_small(int T, int K, int n_out, int band_rows, int sms, int max_sm
 }
 
 template <bool GATED, int SUB, bool ZEROS>
-int launch_small_t(const XsMoeW4 *w, const SmallPlan &p, const __nv_bfloat16 *x, const xs::SmallNorm &norm, int T, __nv_bfloat16 *out, int act, bool early, int32_t *status,
+int launch_small_t(const XsMoeW4 *w, const SmallPlan &p, const __nv_bfloat16 *x, int T, __nv_bfloat16 *out, int act, bool early, int32_t *status,
                    cudaStream_t st)
 {
     CUtensorMap map;
@@ -207,22 +207,22 @@ int launch_small_t(const XsMoeW4 *w, const SmallPlan &p, const __nv_bfloat16 *x,
         return rc;
     auto kern = xs::w4_small_kernel<GATED, SUB, ZEROS>;
     XS_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
-    XS_CUDA(launch_pdl_cluster(kern, p.grid, 32 * xs::kSwWarps, p.cluster, p.smem, st, map, matrix_of(w), x, norm, out, GATED ? w->rows / 2 : w->rows, T,
+    XS_CUDA(launch_pdl_cluster(kern, p.grid, 32 * xs::kSwWarps, p.cluster, p.smem, st, map, matrix_of(w), x, out, GATED ? w->rows / 2 : w->rows, T,
                                w->cols, act, early ? 1 : 0, p.ways, p.cluster, p.chunks_per_block, p.stages, status));
     note_launch();
     return 0;
 }
 
 template <int SUB>
-int launch_small(const XsMoeW4 *w, bool gated, const __nv_bfloat16 *x, const xs::SmallNorm &norm, int T, __nv_bfloat16 *out, int act, bool early, const DeviceInfo &di,
+int launch_small(const XsMoeW4 *w, bool gated, const __nv_bfloat16 *x, int T, __nv_bfloat16 *out, int act, bool early, const DeviceInfo &di,
                  int32_t *status, cudaStream_t st)
 {
     const SmallPlan p = plan_small(T, w->cols, gated ? w->rows / 2 : w->rows, gated ? 16 : 32, di.sms, di.max_smem);
     if (w->zeros_dev)
-        return gated ? launch_small_t<true, SUB, true>(w, p, x, norm, T, out, act, early, status, st)
-                     : launch_small_t<false, SUB, true>(w, p, x, norm, T, out, act, early, status, st);
-    return gated ? launch_small_t<true, SUB, false>(w, p, x, norm, T, out, act, early, status, st)
-                 : launch_small_t<false, SUB, false>(w, p, x, norm, T, out, act, early, status, st);
+        return gated ? launch_small_t<true, SUB, true>(w, p, x, T, out, act, early, status, st)
+                     : launch_small_t<false, SUB, true>(w, p, x, T, out, act, early, status, st);
+    return gated ? launch_small_t<true, SUB, false>(w, p, x, T, out, act, early, status, st)
+                 : launch_small_t<false, SUB, false>(w, p, x, T, out, act, early, status, st);
 }
 
 // A batch of f16 rows read in boxes of 64 columns x box_rows, 128-byte swizzle; past the end of rows and columns there are zeros.
@@ -473,9 +473,8 @@ xs::TcOperands operands(const XsMoeW4 *w, const uint8_t *ws, const TcScratch &p,
     return o;
 }
 
-// early: nothing that may still be running when the kernel starts writes the weights (the second product of one call)
-int run_small(const XsMoeW4 *w, bool gated, int act, const void *x, const xs::SmallNorm &norm, int T, void *out, bool early, int32_t *status,
-              cudaStream_t st)
+// early: nothing that may still be running when the kernel starts writes the weights (it is not the first kernel of its call)
+int run_small(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void *out, bool early, int32_t *status, cudaStream_t st)
 {
     DeviceInfo di;
     if (int rc = device_info(&di))
@@ -483,10 +482,10 @@ int run_small(const XsMoeW4 *w, bool gated, int act, const void *x, const xs::Sm
     const __nv_bfloat16 *xb = static_cast<const __nv_bfloat16 *>(x);
     __nv_bfloat16 *ob = static_cast<__nv_bfloat16 *>(out);
     if (w->group == 32)
-        return launch_small<1>(w, gated, xb, norm, T, ob, act, early, di, status, st);
+        return launch_small<1>(w, gated, xb, T, ob, act, early, di, status, st);
     if (w->group == 64)
-        return launch_small<2>(w, gated, xb, norm, T, ob, act, early, di, status, st);
-    return launch_small<4>(w, gated, xb, norm, T, ob, act, early, di, status, st);
+        return launch_small<2>(w, gated, xb, T, ob, act, early, di, status, st);
+    return launch_small<4>(w, gated, xb, T, ob, act, early, di, status, st);
 }
 
 size_t linear_bytes(const XsMoeW4 *w, int T)
@@ -498,7 +497,7 @@ int run_linear(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void
 {
     int32_t *status = reinterpret_cast<int32_t *>(ws);
     if (small_batch(T, w->cols))
-        return run_small(w, gated, act, x, {}, T, out, false, status, st);
+        return run_small(w, gated, act, x, T, out, false, status, st);
     const TcScratch p = plan_scratch(w, nullptr, T, kStatusBytes);
     if (int rc = launch_prepare(w, gated, nullptr, nullptr, x, T, ws, p, st))
         return rc;
@@ -513,18 +512,17 @@ size_t mlp_bytes(const XsMoeW4 *gu, const XsMoeW4 *dn, int T)
     return small_batch(T, gu->cols) && small_batch(T, dn->cols) ? at : plan_scratch(gu, dn, T, at).bytes;
 }
 
-// norm: the rows of x are normed where they are laid out for the product (null: no norm)
-int run_mlp(const XsMoeW4 *gu, const XsMoeW4 *dn, int32_t act, const XsMoeBlockNorms *norm, const void *x, int32_t T, void *out, uint8_t *ws, cudaStream_t st)
+// norm: the rows of x are normed on the way to the tensor core (null for small batches, and where there is no norm).
+// after_norm: a kernel of the same call made x, so the weights were complete before it began
+int run_mlp(const XsMoeW4 *gu, const XsMoeW4 *dn, int32_t act, const XsMoeBlockNorms *norm, const void *x, int32_t T, void *out, uint8_t *ws, cudaStream_t st,
+            bool after_norm = false)
 {
     int32_t *status = reinterpret_cast<int32_t *>(ws);
     uint8_t *h = ws + kStatusBytes;
     if (small_batch(T, gu->cols) && small_batch(T, dn->cols)) {
-        xs::SmallNorm first{};
-        if (norm)
-            first = {static_cast<const __nv_bfloat16 *>(norm->pre_weight_dev), norm->eps, norm->weight_offset};
-        if (int rc = run_small(gu, true, act, x, first, T, h, false, status, st))
+        if (int rc = run_small(gu, true, act, x, T, h, after_norm, status, st))
             return rc;
-        return run_small(dn, false, 0, h, {}, T, out, true, status, st);
+        return run_small(dn, false, 0, h, T, out, true, status, st);
     }
     const TcScratch p = plan_scratch(gu, dn, T, kStatusBytes + bf16_bytes(T, gu->rows / 2));
     int pair_parts = 0;
@@ -910,15 +908,16 @@ int xs_moe_mlp_w4_block(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t act
             return rc;
         uint8_t *base = static_cast<uint8_t *>(ws), *xn = base + inner, *y = xn + row_bytes;
         cudaStream_t st = static_cast<cudaStream_t>(stream);
-        // the rows are normed where the product lays them out, or makes them ready for the tensor core; the one that does it from
-        // shared memory reads the weight in 16-byte pieces
-        const bool apart = small_batch(tokens, H) && small_batch(tokens, down->cols) && misaligned(norms->pre_weight_dev, 16);
-        if (apart) {
+        // Larger batches are normed where their tokens are made ready for the tensor core.  Small ones are normed by a pass of their
+        // own, during which the gated product already fetches its weights: 12.9 us for one token of 4096 x 2048, where norming in
+        // every block of the product took 14.4.
+        const bool small = small_batch(tokens, H) && small_batch(tokens, down->cols);
+        if (small) {
             const XsMoeNormResidual pre = pre_norm(norms, x, xn, tokens, H);
             if (int rc = run_norm(&pre, st))
                 return rc;
         }
-        if (int rc = run_mlp(gate_up, down, activation, apart ? nullptr : norms, apart ? xn : x, tokens, y, base, st))
+        if (int rc = run_mlp(gate_up, down, activation, small ? nullptr : norms, small ? xn : x, tokens, y, base, st, small))
             return rc;
         const XsMoeNormResidual tail = block_tail(norms, y, x, out, tokens, H);
         return run_norm(&tail, st);

@@ -79,12 +79,6 @@ __device__ __forceinline__ bool warp_sleep_wait(uint64_t *bar, uint32_t parity, 
     }
     return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
 }
-// Column i of eight bf16.
-__device__ __forceinline__ float w4_column(const uint4 &v, int i)
-{
-    const uint32_t u = i / 2 == 0 ? v.x : i / 2 == 1 ? v.y : i / 2 == 2 ? v.z : v.w;
-    return __uint_as_float(i % 2 ? u & 0xffff0000u : u << 16);
-}
 __device__ __forceinline__ uint4 lds128(uint32_t a)
 {
     uint4 v;

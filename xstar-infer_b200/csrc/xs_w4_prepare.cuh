@@ -21,7 +21,6 @@
 #include <stdint.h>
 
 #include "xs_ptx.cuh"
-#include "xs_w4_common.cuh"
 
 namespace xs {
 
@@ -63,6 +62,11 @@ __device__ __forceinline__ int log2_floor(float v)
 {
     return ((__float_as_int(v) >> 23) & 255) - 127;
 }
+__device__ __forceinline__ float prep_get(const uint4 &v, int i)
+{
+    const uint32_t u = i / 2 == 0 ? v.x : i / 2 == 1 ? v.y : i / 2 == 2 ? v.z : v.w;
+    return __uint_as_float(i % 2 ? u & 0xffff0000u : u << 16);
+}
 __device__ __forceinline__ float finite_abs(float v)
 {
     const float a = fabsf(v);
@@ -102,7 +106,7 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
             each([&](int, const uint4 &v) {
 #pragma unroll
                 for (int i = 0; i < 8; i++)
-                    ss = fmaf(w4_column(v, i), w4_column(v, i), ss);
+                    ss = fmaf(prep_get(v, i), prep_get(v, i), ss);
             });
 #pragma unroll
             for (int o = 16; o; o >>= 1)
@@ -120,7 +124,7 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
         auto values = [&](int p, const uint4 &v, float (&f)[8]) {
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                f[i] = w4_column(v, i);
+                f[i] = prep_get(v, i);
             if (a.norm_w) {
                 const __nv_bfloat16 *w = a.norm_w + p * 8;
 #pragma unroll
@@ -236,7 +240,7 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
                 const uint4 v = g == sub * 8 ? w.s0 : scales(w, g);
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const float f = fabsf(w4_column(v, j)), c = finite_abs(f);
+                    const float f = fabsf(prep_get(v, j)), c = finite_abs(f);
                     odd |= !(f <= 3.4e38f);
                     top = fmaxf(top, c);
                     low = c > 0.0f ? fminf(low, c) : low;
@@ -259,7 +263,7 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
                     __half2 o[4];
 #pragma unroll
                     for (int j = 0; j < 4; j++)
-                        o[j] = __floats2half2_rn(w4_column(v, 2 * j) * down, w4_column(v, 2 * j + 1) * down);
+                        o[j] = __floats2half2_rn(prep_get(v, 2 * j) * down, prep_get(v, 2 * j + 1) * down);
                     *reinterpret_cast<uint4 *>(m.scales16 + w.row * m.pitch + g) = *reinterpret_cast<uint4 *>(o);
                     if (m.zeros)
                         *reinterpret_cast<uint2 *>(m.zeros8 + w.row * m.pitch + g) = g == sub * 8 ? w.z0 : zeros(w, g);

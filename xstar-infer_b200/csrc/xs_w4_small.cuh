@@ -66,18 +66,12 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr)
                  : "r"(addr)
                  : "memory");
 }
-// The first norm of a block, done where the tokens are laid out: x becomes bf16(x / sqrt(mean x^2 + eps) * (offset + w)).
-struct SmallNorm {
-    const __nv_bfloat16 *w; // null: none
-    float eps, offset;
-};
-
 // GATED: a warp's 32 rows are the 16 gate rows and the 16 up rows of 16 features.  SUB: 32-column steps in a scale group.
 // early: the weights were complete before the predecessor began.  Cluster size C, chunks_per_block: K in slices.
 template <bool GATED, int SUB, bool ZEROS>
 __global__ void __launch_bounds__(32 * kSwWarps, 1)
-w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, const __nv_bfloat16 *x, const SmallNorm norm, __nv_bfloat16 *out, int n_out,
-                int T, int K, int act, int early, int ways, int C, int chunks_per_block, int stages, int32_t *status)
+w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, const __nv_bfloat16 *x, __nv_bfloat16 *out, int n_out, int T, int K,
+                int act, int early, int ways, int C, int chunks_per_block, int stages, int32_t *status)
 {
     constexpr int G = 32 * SUB, GROUPS = kSwChunk / G, SLOTS = (GROUPS + 3) / 4; // scale slots a lane holds per row and chunk
     constexpr int ROWS = GATED ? 16 : 32; // features a warp works on
@@ -173,29 +167,6 @@ w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, cons
     pdl_launch_dependents(); // after the wait: what the next kernel may load early was complete before this one began
     // x as the MMA's second operand: [32-column step][token][t] pieces of 16 bytes, the pairs (0,4) (1,5) (2,6) (3,7) of columns 8t ..
     {
-        float inv[kSwTokens];
-        if (norm.w) {
-            // the whole row's sum of squares, whatever slice of it this block works on: two warps a token
-            const int n = warp & 7;
-            float ss = 0.0f;
-            if (n < T)
-                for (int k = (warp >> 3) * 256 + lane * 8; k < K; k += 512) {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(x + static_cast<size_t>(n) * K + k);
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        ss = fmaf(w4_column(v, i), w4_column(v, i), ss);
-                }
-#pragma unroll
-            for (int o = 16; o; o >>= 1)
-                ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if (lane == 0)
-                part[warp] = ss;
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < kSwTokens; i++)
-                inv[i] = rsqrtf((part[i] + part[i + 8]) / static_cast<float>(K) + norm.eps);
-            __syncthreads(); // `part` is used again
-        }
         const int pieces = (chunk_end - chunk0) * (kSwChunk / 8);
         for (int p = threadIdx.x; p < pieces; p += 32 * kSwWarps) {
             const int k = chunk0 * kSwChunk + p * 8;
@@ -205,19 +176,6 @@ w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, cons
                 v[n] = make_uint4(0, 0, 0, 0);
                 if (n < T && k < K)
                     v[n] = *reinterpret_cast<const uint4 *>(x + static_cast<size_t>(n) * K + k);
-            }
-            if (norm.w && k < K) {
-                const uint4 w8 = *reinterpret_cast<const uint4 *>(norm.w + k);
-#pragma unroll
-                for (int n = 0; n < kSwTokens; n++)
-                    if (n < T) {
-                        __nv_bfloat162 o[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            o[i] = __floats2bfloat162_rn(w4_column(v[n], 2 * i) * inv[n] * (norm.offset + w4_column(w8, 2 * i)),
-                                                         w4_column(v[n], 2 * i + 1) * inv[n] * (norm.offset + w4_column(w8, 2 * i + 1)));
-                        v[n] = *reinterpret_cast<uint4 *>(o);
-                    }
             }
 #pragma unroll
             for (int n = 0; n < kSwTokens; n++)
