@@ -57,7 +57,7 @@ int xs_moe_gated_w4(const XsMoeW4 *gate_up, int32_t activation, const void *x_de
 
 /* out (tokens, H) bf16 = (act(x Wg^T) * (x Wu^T)) Wd^T, gate_up (2I, H), down (H, I): the reference's
  * mlp(x, gate_up_weight, down_weight) (xstar_cpp/include/ops/mlp.h:51) with 4-bit weights.  The product of the first half is
- * rounded once: to bf16 up to 8 tokens, beyond to f16, scaled by a power of two that a bound of the row gives. */
+ * rounded once, to f16, scaled by a power of two for each token. */
 int xs_moe_mlp_w4_workspace_bytes(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t tokens, size_t *bytes);
 int xs_moe_mlp_w4(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t activation, const void *x_dev, int32_t tokens,
                   void *out_dev, void *workspace_dev, size_t workspace_bytes, void *stream);

@@ -177,8 +177,8 @@ def mlp_reference(gu, dn, x, act, dx=None):
         s = gu["s"].to(F).abs().amax(-1)
         bound = 2.0**15 * X.square().sum(-1, keepdim=True) * X.shape[1] * (s[: h.shape[1]] * s[h.shape[1]:]).amax()
         dh = F16 * h.abs() + 2.0**-40 * bound + dh * (1 + F16)
-    else:
-        dh = HALF * h.abs() + dh * (1 + HALF)
+    else:  # h in f16, each token, or its part that is summed together, scaled to a largest element of 2^13 at least
+        dh = F16 * h.abs() + 2.0**-38 * (h.abs() + dh).amax(-1, keepdim=True) + dh * (1 + F16)
     D = matrix(dn)
     ref = h @ D.T
     err = _sum_error(h.abs() + dh, D, x.shape[0]) + dh @ D.abs().T

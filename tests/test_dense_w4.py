@@ -364,10 +364,9 @@ def test_mlp_and_its_first_half_match_their_definitions(H, I, group, zeros, act)
         du.flags(ws)
         ref, tol = du.mlp_reference(gu, dn, x, act)
         du.assert_close(out, ref, tol)
-        assert du.rel_l2(out, ref) < L2
+        # a rounding to bf16 is off by 2^-7 / sqrt(12) of the leading bit's value on average; h handed on in bf16 would double its square
+        assert du.rel_l2(out, ref) < 1.05 * 2.0**-7 / 12**0.5
         assert (buf[T * H:] == 77.0).all()
-        if T <= du.EXACT_WEIGHT_TOKENS:  # the whole is its two halves; larger batches hand h on in f16
-            assert torch.equal(out, du.linear(dn, h)[0])
 
 
 @pytest.mark.gpu

@@ -198,31 +198,45 @@ SmallPlan plan_small(int T, int K, int n_out, int band_rows, int sms, int max_sm
     return best;
 }
 
-template <bool GATED, int SUB, bool ZEROS>
-int launch_small_t(const XsMoeW4 *w, const SmallPlan &p, const __nv_bfloat16 *x, int T, __nv_bfloat16 *out, int act, bool early, int32_t *status,
-                   cudaStream_t st)
+template <bool GATED, int SUB, bool ZEROS, bool HALF>
+int launch_small_t(const XsMoeW4 *w, const void *x, int T, void *out, int act, bool out_f32, bool early, int32_t *status, cudaStream_t st)
 {
+    DeviceInfo di;
+    if (int rc = device_info(&di))
+        return rc;
+    const int n_out = GATED ? w->rows / 2 : w->rows;
+    const SmallPlan p = plan_small(T, w->cols, n_out, GATED ? 16 : 32, di.sms, di.max_smem);
     CUtensorMap map;
     if (int rc = make_tmap_codes(&map, w, GATED ? 2 : 1, GATED ? 16 : 32))
         return rc;
-    auto kern = xs::w4_small_kernel<GATED, SUB, ZEROS>;
+    auto kern = xs::w4_small_kernel<GATED, SUB, ZEROS, HALF>;
     XS_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
-    XS_CUDA(launch_pdl_cluster(kern, p.grid, 32 * xs::kSwWarps, p.cluster, p.smem, st, map, matrix_of(w), x, out, GATED ? w->rows / 2 : w->rows, T,
-                               w->cols, act, early ? 1 : 0, p.ways, p.cluster, p.chunks_per_block, p.stages, status));
+    XS_CUDA(launch_pdl_cluster(kern, p.grid, 32 * xs::kSwWarps, p.cluster, p.smem, st, map, matrix_of(w), x, out, n_out, T, w->cols, act, out_f32 ? 1 : 0,
+                               early ? 1 : 0, p.ways, p.cluster, p.chunks_per_block, p.stages, status));
     note_launch();
     return 0;
 }
 
-template <int SUB>
-int launch_small(const XsMoeW4 *w, bool gated, const __nv_bfloat16 *x, int T, __nv_bfloat16 *out, int act, bool early, const DeviceInfo &di,
-                 int32_t *status, cudaStream_t st)
+template <bool GATED, bool HALF>
+int launch_small(const XsMoeW4 *w, const void *x, int T, void *out, int act, bool out_f32, bool early, int32_t *status, cudaStream_t st)
 {
-    const SmallPlan p = plan_small(T, w->cols, gated ? w->rows / 2 : w->rows, gated ? 16 : 32, di.sms, di.max_smem);
-    if (w->zeros_dev)
-        return gated ? launch_small_t<true, SUB, true>(w, p, x, T, out, act, early, status, st)
-                     : launch_small_t<false, SUB, true>(w, p, x, T, out, act, early, status, st);
-    return gated ? launch_small_t<true, SUB, false>(w, p, x, T, out, act, early, status, st)
-                 : launch_small_t<false, SUB, false>(w, p, x, T, out, act, early, status, st);
+    const bool z = w->zeros_dev != nullptr;
+    if (w->group == 32)
+        return z ? launch_small_t<GATED, 1, true, HALF>(w, x, T, out, act, out_f32, early, status, st)
+                 : launch_small_t<GATED, 1, false, HALF>(w, x, T, out, act, out_f32, early, status, st);
+    if (w->group == 64)
+        return z ? launch_small_t<GATED, 2, true, HALF>(w, x, T, out, act, out_f32, early, status, st)
+                 : launch_small_t<GATED, 2, false, HALF>(w, x, T, out, act, out_f32, early, status, st);
+    return z ? launch_small_t<GATED, 4, true, HALF>(w, x, T, out, act, out_f32, early, status, st)
+             : launch_small_t<GATED, 4, false, HALF>(w, x, T, out, act, out_f32, early, status, st);
+}
+
+// `early` above: nothing that may still be running when the kernel starts writes the weights (it is not the first kernel of its
+// call).  One product alone:
+int run_small(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void *out, int32_t *status, cudaStream_t st)
+{
+    return gated ? launch_small<true, false>(w, x, T, out, act, false, false, status, st)
+                 : launch_small<false, false>(w, x, T, out, 0, false, false, status, st);
 }
 
 // A batch of f16 rows read in boxes of 64 columns x box_rows, 128-byte swizzle; past the end of rows and columns there are zeros.
@@ -362,6 +376,11 @@ bool small_batch(int T, int K)
     return T <= xs::kSwTokens && xs::sw_smem_bytes(T, ((K + xs::kSwChunk - 1) / xs::kSwChunk + 7) / 8, 2) <= kBlockSmem;
 }
 
+bool small_mlp(const XsMoeW4 *gu, const XsMoeW4 *dn, int T)
+{
+    return small_batch(T, gu->cols) && small_batch(T, dn->cols);
+}
+
 // Scratch of the tensor-core kernel: tokens and scales in f16, zero points, factors.
 struct TcScratch {
     size_t x16 = 0, token = 0, l = 0, part = 0, scales[2] = {}, zeros[2] = {}, row[2] = {}, bytes = 0;
@@ -473,21 +492,6 @@ xs::TcOperands operands(const XsMoeW4 *w, const uint8_t *ws, const TcScratch &p,
     return o;
 }
 
-// early: nothing that may still be running when the kernel starts writes the weights (it is not the first kernel of its call)
-int run_small(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void *out, bool early, int32_t *status, cudaStream_t st)
-{
-    DeviceInfo di;
-    if (int rc = device_info(&di))
-        return rc;
-    const __nv_bfloat16 *xb = static_cast<const __nv_bfloat16 *>(x);
-    __nv_bfloat16 *ob = static_cast<__nv_bfloat16 *>(out);
-    if (w->group == 32)
-        return launch_small<1>(w, gated, xb, T, ob, act, early, di, status, st);
-    if (w->group == 64)
-        return launch_small<2>(w, gated, xb, T, ob, act, early, di, status, st);
-    return launch_small<4>(w, gated, xb, T, ob, act, early, di, status, st);
-}
-
 size_t linear_bytes(const XsMoeW4 *w, int T)
 {
     return small_batch(T, w->cols) ? kStatusBytes : plan_scratch(w, nullptr, T, kStatusBytes).bytes;
@@ -497,7 +501,7 @@ int run_linear(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void
 {
     int32_t *status = reinterpret_cast<int32_t *>(ws);
     if (small_batch(T, w->cols))
-        return run_small(w, gated, act, x, T, out, false, status, st);
+        return run_small(w, gated, act, x, T, out, status, st);
     const TcScratch p = plan_scratch(w, nullptr, T, kStatusBytes);
     if (int rc = launch_prepare(w, gated, nullptr, nullptr, x, T, ws, p, st))
         return rc;
@@ -508,8 +512,9 @@ int run_linear(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void
 // The gated product and the down product share one scratch: h behind the status block, then what the tensor-core kernel needs.
 size_t mlp_bytes(const XsMoeW4 *gu, const XsMoeW4 *dn, int T)
 {
-    const size_t at = kStatusBytes + bf16_bytes(T, gu->rows / 2);
-    return small_batch(T, gu->cols) && small_batch(T, dn->cols) ? at : plan_scratch(gu, dn, T, at).bytes;
+    if (small_mlp(gu, dn, T))
+        return kStatusBytes + static_cast<size_t>(T) * (gu->rows / 2) * 4;
+    return plan_scratch(gu, dn, T, kStatusBytes + bf16_bytes(T, gu->rows / 2)).bytes;
 }
 
 // norm: the rows of x are normed on the way to the tensor core (null for small batches, and where there is no norm).
@@ -519,10 +524,10 @@ int run_mlp(const XsMoeW4 *gu, const XsMoeW4 *dn, int32_t act, const XsMoeBlockN
 {
     int32_t *status = reinterpret_cast<int32_t *>(ws);
     uint8_t *h = ws + kStatusBytes;
-    if (small_batch(T, gu->cols) && small_batch(T, dn->cols)) {
-        if (int rc = run_small(gu, true, act, x, T, h, after_norm, status, st))
+    if (small_mlp(gu, dn, T)) {
+        if (int rc = launch_small<true, false>(gu, x, T, h, act, true, after_norm, status, st))
             return rc;
-        return run_small(dn, false, 0, h, T, out, true, status, st);
+        return launch_small<false, true>(dn, h, T, out, 0, false, true, status, st);
     }
     const TcScratch p = plan_scratch(gu, dn, T, kStatusBytes + bf16_bytes(T, gu->rows / 2));
     int pair_parts = 0;
@@ -911,7 +916,7 @@ int xs_moe_mlp_w4_block(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t act
         // Larger batches are normed where their tokens are made ready for the tensor core.  Small ones are normed by a pass of their
         // own, during which the gated product already fetches its weights: 12.9 us for one token of 4096 x 2048, where norming in
         // every block of the product took 14.4.
-        const bool small = small_batch(tokens, H) && small_batch(tokens, down->cols);
+        const bool small = small_mlp(gate_up, down, tokens);
         if (small) {
             const XsMoeNormResidual pre = pre_norm(norms, x, xn, tokens, H);
             if (int rc = run_norm(&pre, st))

@@ -1,6 +1,7 @@
 // What the kernels with 4-bit integer weights share: the matrix, the conversion of codes, the activations.
 #pragma once
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -41,6 +42,53 @@ __device__ __forceinline__ void w4_unpack(uint32_t (&a)[4], uint32_t q, uint32_t
 __device__ __forceinline__ uint32_t w4_minus_zero(uint32_t z)
 {
     return w4_fma(z * 0x00010001u, 0xff00ff00u, 0u); // times -2^127
+}
+
+__device__ __forceinline__ uint32_t f16x2_mul(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t f16x2_fma(uint32_t a, uint32_t b, uint32_t c)
+{
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+// The same in f16, whose bits are an integer below 1024 times 2^-24: 2^15 brings a nibble, and 2^11 sixteen times one, to the code
+// times 2^-9.  kW4PairMul: for a pair of both kinds.
+constexpr uint32_t kW4HalfMulLow = 0x78007800u, kW4HalfMulHigh = 0x68006800u, kW4PairMul = 0x68007800u;
+constexpr uint32_t kW4HalfMinus8 = 0xa400a400u; // -8 * 2^-9
+constexpr float kW4HalfUnit = 512.0f;
+__device__ __forceinline__ uint32_t w4_half_minus_zero(uint32_t z)
+{
+    return f16x2_mul(z * 0x00010001u, 0xf800f800u); // -2^15
+}
+__device__ __forceinline__ void w4_unpack_half(uint32_t (&a)[4], uint32_t q, uint32_t mz)
+{
+    const uint32_t h = q >> 8;
+    a[0] = f16x2_fma(q & 0x000f000fu, kW4HalfMulLow, mz);
+    a[1] = f16x2_fma(q & 0x00f000f0u, kW4HalfMulHigh, mz);
+    a[2] = f16x2_fma(h & 0x000f000fu, kW4HalfMulLow, mz);
+    a[3] = f16x2_fma(h & 0x00f000f0u, kW4HalfMulHigh, mz);
+}
+
+// Powers of two that bring tokens and scales into the range of f16.
+constexpr int kExpMin = -112, kExpMax = 112;
+__device__ __forceinline__ float pow2f(int e) // -126 <= e <= 127
+{
+    return __int_as_float((e + 127) << 23);
+}
+// floor(log2 v) of a positive normal v; subnormal numbers count as 2^-127
+__device__ __forceinline__ int log2_floor(float v)
+{
+    return ((__float_as_int(v) >> 23) & 255) - 127;
+}
+__device__ __forceinline__ float finite_abs(float v)
+{
+    const float a = fabsf(v);
+    return a <= 3.4e38f ? a : 0.0f; // infinities and NaN do not count
 }
 
 // silu: v / (1 + exp(-v)); gelu: v / 2 * (1 + tanh(c (v + 0.044715 v^3))), and (1 + tanh(a)) / 2 = 1 / (1 + exp(-2 a)).  The fast

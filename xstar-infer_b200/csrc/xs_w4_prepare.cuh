@@ -21,6 +21,7 @@
 #include <stdint.h>
 
 #include "xs_ptx.cuh"
+#include "xs_w4_common.cuh"
 
 namespace xs {
 
@@ -50,29 +51,13 @@ struct PrepareArgs {
 constexpr int kPrepThreads = 128;
 constexpr int kPrepRows = 128;     // weight rows of a block at most
 constexpr int kPrepKeep = 4;       // pieces of eight columns a thread keeps in registers
-constexpr int kExpMin = -112, kExpMax = 112;
 constexpr int kTcUnitExp = 9; // the codes enter as (q - z) 2^-9
 
-__device__ __forceinline__ float pow2f(int e) // -126 <= e <= 127
-{
-    return __int_as_float((e + 127) << 23);
-}
-// floor(log2 v) of a positive normal v; subnormal numbers count as 2^-127
-__device__ __forceinline__ int log2_floor(float v)
-{
-    return ((__float_as_int(v) >> 23) & 255) - 127;
-}
 __device__ __forceinline__ float prep_get(const uint4 &v, int i)
 {
     const uint32_t u = i / 2 == 0 ? v.x : i / 2 == 1 ? v.y : i / 2 == 2 ? v.z : v.w;
     return __uint_as_float(i % 2 ? u & 0xffff0000u : u << 16);
 }
-__device__ __forceinline__ float finite_abs(float v)
-{
-    const float a = fabsf(v);
-    return a <= 3.4e38f ? a : 0.0f; // infinities and NaN do not count
-}
-
 __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareArgs a)
 {
     constexpr int WARPS = kPrepThreads / 32;

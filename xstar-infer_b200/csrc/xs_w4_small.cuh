@@ -14,8 +14,15 @@
 // long as both operands agree: a lane's 32-bit word holds columns 8t .. 8t+7, which come out as the pairs (0,4) (1,5) (2,6)
 // (3,7), and x is laid out in the same pairs.  ldmatrix hands word t of row g to lane (g, t), which is the fragment layout.  The
 // MMA sums (q - z) x in f32; the scale multiplies the f32 sum of a group, so the weights are never rounded.
+//
+// An MLP hands its gated product on in f32 (HALF): rounded to bf16 it would add as much error as the result's own rounding.  The
+// second product brings each token, or its slice of one, to a largest element of 2^13 .. 2^14 by a power of two, rounds it once to
+// the eleven bits of f16, and multiplies with f16 codes, which are as exact as those in bf16.  Against bf16 rows that costs 0.3 to 0.5 us
+// (one token of 4096 x 2048: 10.2 us for 9.7, with an error of 0.0017 for 0.0025); as a second bf16 row of what the first leaves it
+// cost 0.7, and half as much K fits.
 #pragma once
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -44,18 +51,17 @@ __host__ __device__ constexpr int sw_smem_bytes(int T, int chunks_per_block, int
     return 1024 + kSwWarps * stages * (kSwStageBytes + 8) + sw_x_bytes(T, chunks_per_block) + sw_part_bytes(T) + 16;
 }
 
-// the same onto zero
-__device__ __forceinline__ void mma_16816_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
-{
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
-}
+template <bool HALF>
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    if constexpr (HALF)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // Four 8 x 8 matrices of 16-bit elements: lane (g, t) receives the 32-bit word t of row g of each.  Lane l gives the address of row l % 8 of
 // matrix l / 8.
@@ -67,16 +73,19 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr)
                  : "memory");
 }
 // GATED: a warp's 32 rows are the 16 gate rows and the 16 up rows of 16 features.  SUB: 32-column steps in a scale group.
-// early: the weights were complete before the predecessor began.  Cluster size C, chunks_per_block: K in slices.
-template <bool GATED, int SUB, bool ZEROS>
+// early: the weights were complete before the predecessor began.  Cluster size C, chunks_per_block: K in slices.  HALF: x is
+// f32 and enters as f16; out_f32 (GATED): out is written so.
+template <bool GATED, int SUB, bool ZEROS, bool HALF>
 __global__ void __launch_bounds__(32 * kSwWarps, 1)
-w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, const __nv_bfloat16 *x, __nv_bfloat16 *out, int n_out, int T, int K,
-                int act, int early, int ways, int C, int chunks_per_block, int stages, int32_t *status)
+w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, const void *x, void *out, int n_out, int T, int K,
+                int act, int out_f32, int early, int ways, int C, int chunks_per_block, int stages, int32_t *status)
 {
     constexpr int G = 32 * SUB, GROUPS = kSwChunk / G, SLOTS = (GROUPS + 3) / 4; // scale slots a lane holds per row and chunk
     constexpr int ROWS = GATED ? 16 : 32; // features a warp works on
+    constexpr float UNIT = HALF ? kW4HalfUnit : kW4Unit;
 
     extern __shared__ uint8_t smem_raw[];
+    __shared__ float factor[kSwTokens]; // HALF: of each token
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int bands = kSwWarps / ways, band = warp % bands, way = warp / bands; // 32-row bands of a tile
@@ -167,22 +176,81 @@ w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, cons
     pdl_launch_dependents(); // after the wait: what the next kernel may load early was complete before this one began
     // x as the MMA's second operand: [32-column step][token][t] pieces of 16 bytes, the pairs (0,4) (1,5) (2,6) (3,7) of columns 8t ..
     {
-        const int pieces = (chunk_end - chunk0) * (kSwChunk / 8);
-        for (int p = threadIdx.x; p < pieces; p += 32 * kSwWarps) {
-            const int k = chunk0 * kSwChunk + p * 8;
-            uint4 v[kSwTokens];
+        // the warps of a token: two for each of eight, all for a single one; a thread has BATCH pieces of eight columns on their way
+        constexpr int BATCH = 4;
+        const int spread = T > 4 ? 2 : T > 2 ? 4 : T > 1 ? 8 : 16, n = warp / spread, step = spread * 32, first_p = (warp & (spread - 1)) * 32 + lane;
+        const int pieces = n < T ? (chunk_end - chunk0) * (kSwChunk / 8) : 0;
+        const int there = min(pieces, K / 8 - chunk0 * (kSwChunk / 8)); // the last slice may end inside a chunk
+        const size_t row = static_cast<size_t>(n) * K + chunk0 * kSwChunk;
+        auto place = [&](int p) { return reinterpret_cast<uint4 *>(x_smem + (((p >> 2) * T + n) * 4 + (p & 3)) * 16); };
+        if constexpr (HALF) {
+            auto load = [&](int p, float4 (&v)[BATCH][2]) {
 #pragma unroll
-            for (int n = 0; n < kSwTokens; n++) {
-                v[n] = make_uint4(0, 0, 0, 0);
-                if (n < T && k < K)
-                    v[n] = *reinterpret_cast<const uint4 *>(x + static_cast<size_t>(n) * K + k);
+                for (int j = 0; j < BATCH; j++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+                        v[j][i] = p + j * step < there ? reinterpret_cast<const float4 *>(static_cast<const float *>(x) + row)[(p + j * step) * 2 + i]
+                                                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            };
+            // the first batch is kept, the rest of a long slice loaded twice
+            float4 kept[BATCH][2];
+            load(first_p, kept);
+            float top = 0.0f;
+            auto most = [&](const float4 (&v)[BATCH][2]) {
+#pragma unroll
+                for (int j = 0; j < BATCH; j++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+                        top = fmaxf(top, fmaxf(fmaxf(finite_abs(v[j][i].x), finite_abs(v[j][i].y)), fmaxf(finite_abs(v[j][i].z), finite_abs(v[j][i].w))));
+            };
+            most(kept);
+#pragma unroll 1
+            for (int p = first_p + BATCH * step; p < there; p += BATCH * step) {
+                float4 v[BATCH][2];
+                load(p, v);
+                most(v);
             }
+            // floats that are not negative are ordered like their bits
+            const uint32_t of_warp = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+            if (lane == 0)
+                part[warp] = __uint_as_float(of_warp);
+            __syncthreads();
+            const uint32_t of_token = __reduce_max_sync(0xffffffffu, __float_as_uint(part[n * spread + (lane & (spread - 1))]));
+            const int e = max(kExpMin, min(kExpMax, log2_floor(__uint_as_float(of_token)) - 13));
+            const float down = pow2f(-e);
+            if (lane == 0 && n < T)
+                factor[n] = pow2f(e);
+            auto store = [&](int p, const float4 (&v)[BATCH][2]) {
 #pragma unroll
-            for (int n = 0; n < kSwTokens; n++)
-                if (n < T)
-                    *reinterpret_cast<uint4 *>(x_smem + (((p >> 2) * T + n) * 4 + (p & 3)) * 16) =
-                        make_uint4(__byte_perm(v[n].x, v[n].z, 0x5410), __byte_perm(v[n].x, v[n].z, 0x7632), __byte_perm(v[n].y, v[n].w, 0x5410),
-                                   __byte_perm(v[n].y, v[n].w, 0x7632));
+                for (int j = 0; j < BATCH; j++) {
+                    const float4 &a = v[j][0], &b = v[j][1];
+                    const __half2 o[4] = {__floats2half2_rn(a.x * down, b.x * down), __floats2half2_rn(a.y * down, b.y * down),
+                                          __floats2half2_rn(a.z * down, b.z * down), __floats2half2_rn(a.w * down, b.w * down)};
+                    if (p + j * step < pieces)
+                        *place(p + j * step) = *reinterpret_cast<const uint4 *>(o);
+                }
+            };
+            store(first_p, kept);
+#pragma unroll 1
+            for (int p = first_p + BATCH * step; p < pieces; p += BATCH * step) {
+                float4 v[BATCH][2];
+                load(p, v);
+                store(p, v);
+            }
+        } else {
+#pragma unroll 1
+            for (int p = first_p; p < pieces; p += BATCH * step) {
+                uint4 v[BATCH];
+#pragma unroll
+                for (int j = 0; j < BATCH; j++)
+                    v[j] = p + j * step < there ? reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(x) + row)[p + j * step]
+                                                : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < BATCH; j++)
+                    if (p + j * step < pieces)
+                        *place(p + j * step) = make_uint4(__byte_perm(v[j].x, v[j].z, 0x5410), __byte_perm(v[j].x, v[j].z, 0x7632),
+                                                          __byte_perm(v[j].y, v[j].w, 0x5410), __byte_perm(v[j].y, v[j].w, 0x7632));
+            }
         }
     }
     __syncthreads();
@@ -193,6 +261,7 @@ w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, cons
     // lanes of tokens that are not there read the last one: a column of its own, which is not stored
     const uint32_t x_lane = smem_u32(x_smem) + ((g < T ? g : T - 1) * 4 + t) * 16;
     const int x_step = T * 64;
+    const float factor_even = HALF && 2 * t < T ? factor[2 * t] : 1.0f, factor_odd = HALF && 2 * t + 1 < T ? factor[2 * t + 1] : 1.0f;
     const int share = features / C, share_log = 31 - __clz(share); // features of a tile that this block finishes: a power of two
     int stage = 0, parity = 0;
     uint32_t phase = 0;
@@ -223,18 +292,21 @@ w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, cons
                         for (int h = 0; h < 2; h++) {
                             const uint32_t v = __shfl_sync(0xffffffffu, sc[m * 2 + h][(j / SUB) / 4], (lane & ~3) | ((j / SUB) & 3));
                             s[m][h] = __uint_as_float(ZEROS ? v & 0xffff0000u : v);
-                            z[m][h] = ZEROS ? w4_minus_zero(v & 15u) : kW4Minus8;
+                            z[m][h] = HALF ? ZEROS ? w4_half_minus_zero(v & 15u) : kW4HalfMinus8 : ZEROS ? w4_minus_zero(v & 15u) : kW4Minus8;
                         }
                     }
                     uint32_t a[2][4];
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        w4_unpack(a[h], q[m * 2 + h], z[m][h]);
+                    for (int h = 0; h < 2; h++) {
+                        if constexpr (HALF)
+                            w4_unpack_half(a[h], q[m * 2 + h], z[m][h]);
+                        else
+                            w4_unpack(a[h], q[m * 2 + h], z[m][h]);
+                    }
                     if (j % SUB == 0)
-                        mma_16816_first(c[m], a[0][0], a[1][0], a[0][1], a[1][1], b.x, b.y);
-                    else
-                        mma_16816(c[m], a[0][0], a[1][0], a[0][1], a[1][1], b.x, b.y);
-                    mma_16816(c[m], a[0][2], a[1][2], a[0][3], a[1][3], b.z, b.w);
+                        c[m][0] = c[m][1] = c[m][2] = c[m][3] = 0.0f;
+                    mma_16816<HALF>(c[m], a[0][0], a[1][0], a[0][1], a[1][1], b.x, b.y);
+                    mma_16816<HALF>(c[m], a[0][2], a[1][2], a[0][3], a[1][3], b.z, b.w);
                     if (j % SUB == SUB - 1) {
                         acc[m][0] = fmaf(s[m][0], c[m][0], acc[m][0]);
                         acc[m][1] = fmaf(s[m][0], c[m][1], acc[m][1]);
@@ -262,7 +334,7 @@ w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, cons
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 if (2 * t + (e & 1) < T)
-                    mine[(2 * t + (e & 1)) * kSwPartStride + m * 16 + (e >> 1) * 8 + g] = acc[m][e];
+                    mine[(2 * t + (e & 1)) * kSwPartStride + m * 16 + (e >> 1) * 8 + g] = HALF ? acc[m][e] * (e & 1 ? factor_odd : factor_even) : acc[m][e];
         // one barrier a tile: the next tile's sums go to the other half of `part`
         if (C > 1)
             cluster_barrier();
@@ -279,8 +351,14 @@ w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, cons
                     if (GATED)
                         u += C > 1 ? ld_cluster_f32(smem_u32(pk + 16), r) : pk[16];
                 }
-            if (feature < n_out)
-                out[static_cast<size_t>(token) * n_out + feature] = __float2bfloat16_rn(GATED ? w4_activation(kW4Unit * v, act) * (kW4Unit * u) : kW4Unit * v);
+            if (feature < n_out) {
+                const float r = GATED ? w4_activation(UNIT * v, act) * (UNIT * u) : UNIT * v;
+                const size_t o = static_cast<size_t>(token) * n_out + feature;
+                if (GATED && out_f32)
+                    static_cast<float *>(out)[o] = r;
+                else
+                    static_cast<__nv_bfloat16 *>(out)[o] = __float2bfloat16_rn(r);
+            }
         }
     }
     if (C > 1)

@@ -137,26 +137,6 @@ __device__ __forceinline__ uint32_t w4_pair(uint32_t word, int c)
     const uint32_t low = word & 0x0f0f0f0fu, high = word & 0xf0f0f0f0u;
     return prmt(low, high, c | (8 | c) << 4 | (4 + c) << 8 | (8 | c) << 12);
 }
-__device__ __forceinline__ uint32_t f16x2_mul(uint32_t a, uint32_t b)
-{
-    uint32_t r;
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t f16x2_fma(uint32_t a, uint32_t b, uint32_t c)
-{
-    uint32_t r;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-    return r;
-}
-// An f16 whose bits are an integer below 1024 is that integer times 2^-24, so a nibble, or sixteen times one, is a number as it
-// stands; times 2^15 (2^11) it is the code times 2^-9.
-constexpr uint32_t kTcPairMul = 0x68007800u, kTcMinus8 = 0xa400a400u; // 2^11 2^15; -8 * 2^-9
-__device__ __forceinline__ uint32_t tc_minus_zero(uint32_t z)
-{
-    return f16x2_mul(z * 0x00010001u, 0xf800f800u); // -2^15
-}
-
 // Barrier 1 among the eight epilogue warps; the conjunction of their predicates.
 __device__ __forceinline__ bool named_barrier_and(bool ok)
 {
@@ -447,19 +427,19 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                     const uint32_t words[4] = {qv.x, qv.y, qv.z, qv.w};
                     uint32_t a[16];
                     if (one_step) {
-                        const uint32_t mul = f16x2_mul(sv, kTcPairMul), add = f16x2_mul(sv, kTcMinus8);
+                        const uint32_t mul = f16x2_mul(sv, kW4PairMul), add = f16x2_mul(sv, kW4HalfMinus8);
 #pragma unroll
                         for (int j = 0; j < 4; j++)
 #pragma unroll
                             for (int c = 0; c < 4; c++)
                                 a[j * 4 + c] = f16x2_fma(w4_pair(words[j], c), mul, add);
                     } else {
-                        const uint32_t mz = zeros ? tc_minus_zero((cur.z >> (8 * e)) & 15u) : kTcMinus8;
+                        const uint32_t mz = zeros ? w4_half_minus_zero((cur.z >> (8 * e)) & 15u) : kW4HalfMinus8;
 #pragma unroll
                         for (int j = 0; j < 4; j++)
 #pragma unroll
                             for (int c = 0; c < 4; c++)
-                                a[j * 4 + c] = f16x2_mul(f16x2_fma(w4_pair(words[j], c), kTcPairMul, mz), sv);
+                                a[j * 4 + c] = f16x2_mul(f16x2_fma(w4_pair(words[j], c), kW4PairMul, mz), sv);
                     }
                     tmem_st16(dst + h * 16, a);
                 }
