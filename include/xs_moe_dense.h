@@ -22,7 +22,7 @@ extern "C" {
  *   codes  (rows, cols / 2) bytes   q in 0..15, the even column in the low nibble (the byte order of XS_MOE_FP4_MX32)
  *   scales (rows, cols / group)     bf16, any value
  *   zeros  (rows, cols / group)     bytes, the low four bits are the zero point; NULL: 8 everywhere
- * group is 32, 64 or 128; cols is a multiple of group; rows is any positive number.  codes are 16-byte aligned, scales 2-byte.
+ * group is 32, 64 or 128; cols is a multiple of group; rows is any positive number; none is above 2^30.  codes are 16-byte aligned, scales 2-byte.
  * The reference has no quantised weights (xstar_cpp/include/dtype.h:8-12); the matrix takes the place of `weight` in its
  * linear op, x * W^T (xstar_cpp/src/ops/linear.cpp:20-31). */
 typedef struct XsMoeW4 {
@@ -43,7 +43,7 @@ typedef enum XsMoeActivation {
 /* out (tokens, rows) bf16 = x (tokens, cols) bf16 times W^T; f32 sums, one rounding at the end.  Up to 8 tokens the weights
  * enter the products exactly; larger batches go to the tensor core in f16, tokens and weight rows scaled by powers of two: a
  * weight is rounded once to 11 bits, tokens are exact down to 2^-27 of their largest element.
- * x is 16-byte aligned and does not overlap out.  Takes the role of gemm_launch behind linear
+ * x is 16-byte aligned; what a call writes may not overlap what it reads.  Takes the role of gemm_launch behind linear
  * (xstar_cpp/include/ops/gemm.h:165-176). */
 int xs_moe_linear_w4_workspace_bytes(const XsMoeW4 *w, int32_t tokens, size_t *bytes);
 int xs_moe_linear_w4(const XsMoeW4 *w, const void *x_dev, int32_t tokens, void *out_dev, void *workspace_dev,
@@ -77,7 +77,7 @@ typedef enum XsMoeGate {
  * only r'.  y_dev NULL (then post_weight, gate and residual_out are NULL too): r' = residual, only n is written -- a block's
  * first norm.  All tensors bf16; sums of squares and r' are held in f32, n is computed from r' before its rounding.
  * residual_out may be residual or y itself, next_out may be y or residual itself (same address); other overlaps are refused.
- * hidden is any positive number.  Takes the role of rmsnorm_launch and add_launch (xstar_cpp/include/ops/rmsnorm.h:46-52,
+ * hidden is at most 57344, rows 2^30.  Takes the role of rmsnorm_launch and add_launch (xstar_cpp/include/ops/rmsnorm.h:46-52,
  * xstar_cpp/include/ops/add.h:38) in the tail of the reference's block (xstar_cpp/src/ops/transformer_block.cpp:353). */
 typedef struct XsMoeNormResidual {
     const void *y_dev;
@@ -110,7 +110,8 @@ typedef struct XsMoeBlockNorms {
     int32_t reserved[2]; /* must be zero */
 } XsMoeBlockNorms;
 
-/* F = the 4-bit gated MLP. */
+/* F = the 4-bit gated MLP.  Its input, the normed rows, is rounded once, to bf16 up to 8 tokens and to f16 beyond, and its result
+ * once, to bf16. */
 int xs_moe_mlp_w4_block_workspace_bytes(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t tokens, size_t *bytes);
 int xs_moe_mlp_w4_block(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t activation, const XsMoeBlockNorms *norms,
                         const void *x_dev, int32_t tokens, void *out_dev, void *workspace_dev, size_t workspace_bytes,

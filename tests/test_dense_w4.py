@@ -28,6 +28,7 @@ def _w4(rows=8, cols=256, group=64, codes=4096, scales=4096, zeros=None, reserve
     (dict(rows=0), 1, -1, "non-positive"), (dict(cols=-64), 1, -1, "non-positive"), (dict(), -1, -1, "non-positive"),
     (dict(group=16), 1, -2, "group must be"), (dict(group=0), 1, -2, "group must be"), (dict(group=256), 1, -2, "group must be"),
     (dict(cols=288, group=64), 1, -1, "multiple of the group"), (dict(reserved=1), 1, -1, "reserved"),
+    (dict(rows=2**30 + 1), 1, -2, "at most 2"), (dict(cols=2**31 - 64), 1, -2, "at most 2"), (dict(), 2**31 - 1, -2, "at most 2"),
 ])
 def test_matrix_shapes_are_checked(kw, tokens, code, text):
     L, n = capi.lib(), C.c_size_t(0)
@@ -65,6 +66,7 @@ def test_workspaces_and_null_pointers_are_refused_before_any_device_work():
 @pytest.mark.parametrize("kw, code, text", [
     (dict(gate_kind=9), -1, "gate kind"), (dict(gate_kind=1), -1, "disagree"), (dict(gate_dev=4096), -1, "disagree"),
     (dict(rows=-1), -1, "non-positive"), (dict(hidden=0), -1, "non-positive"), (dict(hidden=60000), -2, "at most"),
+    (dict(rows=2**30 + 1), -2, "at most"),
     (dict(residual_dev=None), -1, "null"), (dict(next_weight_dev=4096), -1, "go together"), (dict(next_out_dev=4096), -1, "go together"),
     (dict(residual_out_dev=None), -1, "go together"), (dict(y_dev=None), -1, "go together"),
 ])
@@ -308,6 +310,20 @@ def test_linear_with_offsets_beyond_32_bits(T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T, K", [(8, 32768), (8, 33024), (6, 65536 + 128), (1, 300032)])
+def test_linear_with_few_tokens_and_long_rows(T, K):
+    # tokens that no longer fit into shared memory go the way of larger batches
+    g = du.gen(K)
+    w, x = du.weight(g, 300, K, 64, True), du.bf16(g, (T, K))
+    out, ws = du.linear(w, x)
+    du.flags(ws)
+    ref, _ = du.linear_reference(w, x)
+    many, tol = du.linear_reference(w, torch.cat([x, x.new_zeros(9, K)]))
+    assert torch.equal(many[:T], ref)
+    du.assert_close(out, ref, tol[:T])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [1, 16, 90, 520])
 def test_linear_gives_the_same_bits_each_time_and_for_each_token(T):
     g = du.gen(21)
@@ -336,6 +352,8 @@ def test_overlaps_host_memory_and_bad_alignment_are_refused():
 
     assert call() == 0
     assert call(out=x) == -1 and b"overlap" in L.xs_moe_last_error()
+    assert call(out=w["s"]) == -1 and b"a weight overlaps" in L.xs_moe_last_error()
+    assert call(ws=w["q"].view(-1)) == -1 and b"a weight overlaps" in L.xs_moe_last_error()
     assert call(x=torch.empty(4 * 256 + 8, dtype=torch.bfloat16, device="cuda")[1:]) == -1
     assert call(out=torch.empty(4 * 64 * 2 + 8, dtype=torch.uint8, device="cuda")[1:]) == -1
     for bad in (dict(x=x.cpu()), dict(out=out.cpu()), dict(m=with_(q=w["q"].cpu())), dict(m=with_(s=w["s"].cpu())), dict(m=with_(z=w["z"].cpu()))):

@@ -75,7 +75,7 @@ __device__ __forceinline__ void w4_unpack_half(uint32_t (&a)[4], uint32_t q, uin
 }
 
 // Powers of two that bring tokens and scales into the range of f16.
-constexpr int kExpMin = -112, kExpMax = 112;
+constexpr int kExpMin = -112, kExpMax = 114;
 __device__ __forceinline__ float pow2f(int e) // -126 <= e <= 127
 {
     return __int_as_float((e + 127) << 23);

@@ -13,7 +13,8 @@
 // what occurs, of the 2^39 that f16 spans; the products of a row smaller than that again lose bits.
 //
 // Bytes decide: tokens are read once and written once; the scales are a fiftieth of the weights.  With `norm_w` the tokens are
-// normed on the way (the first norm of a block): v / sqrt(mean v^2 + eps) * (offset + w), rounded once, to f16.
+// normed on the way (the first norm of a block): v / sqrt(mean v^2 + eps) * (offset + w), rounded once, to f16.  8192 tokens of
+// 4096 and the scales of 24576 x 4096 and 4096 x 12288: 22 us (6.3 TB/s); with a few tokens 3 to 4 us, most of them latency.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -19,6 +19,10 @@
 // An operand block is 128 columns because every hand-over costs its roles a few hundred cycles (a poll of a barrier about 110, a
 // parked wait about 300, an expect or a load 100 each): with 64 columns one loading thread took 600 cycles a block, whatever the
 // tile, and everybody else waited for it.
+//
+// Measured: 4096 x 4096 x 8192 190 to 197 us with the preparation, 1.40 to 1.45 PFLOP/s of the 1.66 that the library reaches on this part; 8192 x
+// 8192 x 8192 770 us (1.43).  With few tokens an MMA of 128 rows takes its 110 cycles whatever N, so a block of 128 x 128 weights takes
+// 0.42 to 0.46 us and the weights stream at 2.7 TB/s at most: 45 x 4096 x 20480 39 us, 83 x 11264 x 4096 27 us, where the bytes would take 7 and 5.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
