@@ -40,9 +40,10 @@ typedef enum XsMoeActivation {
     XS_MOE_GELU_TANH = 1 /* v / 2 * (1 + tanh(sqrt(2 / pi) * (v + 0.044715 v^3))) */
 } XsMoeActivation;
 
-/* out (tokens, rows) bf16 = x (tokens, cols) bf16 times W^T; f32 sums, one rounding at the end.  Up to 8 tokens the weights
- * enter the products exactly; larger batches go to the tensor core in f16, tokens and weight rows scaled by powers of two: a
- * weight is rounded once to 11 bits, tokens are exact down to 2^-27 of their largest element.
+/* out (tokens, rows) bf16 = x (tokens, cols) bf16 times W^T; f32 sums, one rounding at the end.  Small
+ * batches (up to 8 tokens of 32768 columns, up to 16 of 8192) multiply with the exact weights; larger ones go to the tensor core
+ * in f16, tokens and weight rows scaled by powers of two: a weight is rounded once to 11 bits, tokens are exact down to 2^-27 of
+ * their largest element.
  * x is 16-byte aligned; what a call writes may not overlap what it reads.  Takes the role of gemm_launch behind linear
  * (xstar_cpp/include/ops/gemm.h:165-176). */
 int xs_moe_linear_w4_workspace_bytes(const XsMoeW4 *w, int32_t tokens, size_t *bytes);
@@ -110,7 +111,7 @@ typedef struct XsMoeBlockNorms {
     int32_t reserved[2]; /* must be zero */
 } XsMoeBlockNorms;
 
-/* F = the 4-bit gated MLP.  Its input, the normed rows, is rounded once, to bf16 up to 8 tokens and to f16 beyond, and its result
+/* F = the 4-bit gated MLP.  Its input, the normed rows, is rounded once, to bf16 in small batches and to f16 in larger ones, and its result
  * once, to bf16. */
 int xs_moe_mlp_w4_block_workspace_bytes(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t tokens, size_t *bytes);
 int xs_moe_mlp_w4_block(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t activation, const XsMoeBlockNorms *norms,

@@ -12,7 +12,7 @@ F = torch.float64
 HALF = 2.0**-8  # half a bf16 step, relative to the value
 ACT = {"silu": capi.SILU, "gelu": capi.GELU_TANH}
 GATE = {"none": capi.GATE_NONE, "channel": capi.GATE_CHANNEL, "row": capi.GATE_ROW, "full": capi.GATE_FULL}
-EXACT_WEIGHT_TOKENS = 8  # up to here the weights enter the products unrounded
+EXACT_WEIGHT_TOKENS = 16  # up to here the weights of matrices of up to 8192 columns enter the products unrounded
 
 
 def workspace(nbytes):
@@ -136,7 +136,7 @@ F16 = 2.0**-11
 def _sum_error(X, W, tokens):
     magnitude = X.abs() @ W.abs().T
     err = X.shape[1] * 2.0**-23 * magnitude
-    if tokens > EXACT_WEIGHT_TOKENS:
+    if tokens > EXACT_WEIGHT_TOKENS or (tokens > 8 and X.shape[1] > 8192):
         err = err + F16 * magnitude + 2.0**-38 * X.abs().amax(-1, keepdim=True) * W.abs().sum(-1)
     return err
 

@@ -209,7 +209,7 @@ SmallPlan plan_small(int T, int K, int n_out, int band_rows, int sms, int max_sm
     return best;
 }
 
-template <bool GATED, int SUB, bool ZEROS, bool HALF>
+template <bool GATED, int SUB, bool ZEROS, bool HALF, int NT>
 int launch_small_t(const XsMoeW4 *w, const void *x, int T, void *out, int act, bool out_f32, bool early, int32_t *status, cudaStream_t st)
 {
     DeviceInfo di;
@@ -220,7 +220,7 @@ int launch_small_t(const XsMoeW4 *w, const void *x, int T, void *out, int act, b
     CUtensorMap map;
     if (int rc = make_tmap_codes(&map, w, GATED ? 2 : 1, GATED ? 16 : 32))
         return rc;
-    auto kern = xs::w4_small_kernel<GATED, SUB, ZEROS, HALF>;
+    auto kern = xs::w4_small_kernel<GATED, SUB, ZEROS, HALF, NT>;
     XS_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
     XS_CUDA(launch_pdl_cluster(kern, p.grid, 32 * xs::kSwWarps, p.cluster, p.smem, st, map, matrix_of(w), x, out, n_out, T, w->cols, act, out_f32 ? 1 : 0,
                                early ? 1 : 0, p.ways, p.cluster, p.chunks_per_block, p.stages, status));
@@ -228,18 +228,25 @@ int launch_small_t(const XsMoeW4 *w, const void *x, int T, void *out, int act, b
     return 0;
 }
 
-template <bool GATED, bool HALF>
-int launch_small(const XsMoeW4 *w, const void *x, int T, void *out, int act, bool out_f32, bool early, int32_t *status, cudaStream_t st)
+template <bool GATED, bool HALF, int NT>
+int launch_small_n(const XsMoeW4 *w, const void *x, int T, void *out, int act, bool out_f32, bool early, int32_t *status, cudaStream_t st)
 {
     const bool z = w->zeros_dev != nullptr;
     if (w->group == 32)
-        return z ? launch_small_t<GATED, 1, true, HALF>(w, x, T, out, act, out_f32, early, status, st)
-                 : launch_small_t<GATED, 1, false, HALF>(w, x, T, out, act, out_f32, early, status, st);
+        return z ? launch_small_t<GATED, 1, true, HALF, NT>(w, x, T, out, act, out_f32, early, status, st)
+                 : launch_small_t<GATED, 1, false, HALF, NT>(w, x, T, out, act, out_f32, early, status, st);
     if (w->group == 64)
-        return z ? launch_small_t<GATED, 2, true, HALF>(w, x, T, out, act, out_f32, early, status, st)
-                 : launch_small_t<GATED, 2, false, HALF>(w, x, T, out, act, out_f32, early, status, st);
-    return z ? launch_small_t<GATED, 4, true, HALF>(w, x, T, out, act, out_f32, early, status, st)
-             : launch_small_t<GATED, 4, false, HALF>(w, x, T, out, act, out_f32, early, status, st);
+        return z ? launch_small_t<GATED, 2, true, HALF, NT>(w, x, T, out, act, out_f32, early, status, st)
+                 : launch_small_t<GATED, 2, false, HALF, NT>(w, x, T, out, act, out_f32, early, status, st);
+    return z ? launch_small_t<GATED, 4, true, HALF, NT>(w, x, T, out, act, out_f32, early, status, st)
+             : launch_small_t<GATED, 4, false, HALF, NT>(w, x, T, out, act, out_f32, early, status, st);
+}
+
+template <bool GATED, bool HALF>
+int launch_small(const XsMoeW4 *w, const void *x, int T, void *out, int act, bool out_f32, bool early, int32_t *status, cudaStream_t st)
+{
+    return T <= 8 ? launch_small_n<GATED, HALF, 1>(w, x, T, out, act, out_f32, early, status, st)
+                  : launch_small_n<GATED, HALF, 2>(w, x, T, out, act, out_f32, early, status, st);
 }
 
 // `early` above: nothing that may still be running when the kernel starts writes the weights (it is not the first kernel of its
@@ -381,12 +388,16 @@ int launch_tc(const XsMoeW4 *w, const void *x16, int T, void *out, const xs::TcO
     return 0;
 }
 
-// Which kernel: up to eight tokens the one that streams weights past the tokens, if a cluster's shared memory holds them.  4096 x
-// 4096 with 1, 4, 8 tokens: 5.5, 5.8, 6.5 us against 11.3, 11.3, 11.4 on the tensor core; 8 x 4096 x 32003: 24 us against 40.
+// Which kernel: up to sixteen tokens the one that streams weights past the tokens, if a cluster's shared memory holds them.  4096 x
+// 4096 with 1, 8, 9, 16 tokens: 5.5, 6.5, 7.7, 8.8 us against 11.3, 11.4, 11.5, 11.8 on the tensor core; 8 x 4096 x 32003 with
+// zero points 24 us against 40, 16 tokens 34 against 40.  Clusters of eight do not fill the SMs: more than eight tokens go to the tensor
+// core before they take one (16 x 11264 x 4096: 22 us against 41); up to eight they gain more than they lose (8 x 20480 x 16384 66 us
+// against 82, 1 x 262144 x 4096 230 against 340, but 8 x 20480 x 4096 with zero points 42 against 31).
 constexpr int kBlockSmem = 227 * 1024;
 bool small_batch(int T, int K)
 {
-    return T <= xs::kSwTokens && xs::sw_smem_bytes(T, ((K + xs::kSwChunk - 1) / xs::kSwChunk + 7) / 8, 2) <= kBlockSmem;
+    const int cluster = T > 8 ? 4 : 8, chunks = (K + xs::kSwChunk - 1) / xs::kSwChunk;
+    return T <= xs::kSwTokens && xs::sw_smem_bytes(T, (chunks + cluster - 1) / cluster, 2) <= kBlockSmem;
 }
 
 bool small_mlp(const XsMoeW4 *gu, const XsMoeW4 *dn, int T)

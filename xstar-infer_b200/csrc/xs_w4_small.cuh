@@ -1,4 +1,4 @@
-// Products with 4-bit weights for up to eight tokens: out[t][n] = sum_k (q[n][k] - z[n][k/G]) * s[n][k/G] * x[t][k].
+// Products with 4-bit weights for up to sixteen tokens: out[t][n] = sum_k (q[n][k] - z[n][k/G]) * s[n][k/G] * x[t][k].
 //
 // The weights are read once and nothing else is large, so the kernel is a stream.  A warp works on 32 weight rows in chunks of
 // 256 columns, and owns a ring of such chunks (32 rows x 128 bytes) that TMA fills ahead, across tiles.  Scales come from memory as
@@ -10,10 +10,14 @@
 //
 // The arithmetic must stay below the rate that the stream allows: at 6.5 TB/s an SM receives 46 weights a cycle, and its
 // schedulers issue 128 lanes a cycle.  So the products go to mma.m16n8k16 with the weights as the 16 rows and the tokens as the 8
-// columns, and eight codes become (q - z) / 64 with nine instructions (w4_unpack).  The order of k inside an MMA is free as
-// long as both operands agree: a lane's 32-bit word holds columns 8t .. 8t+7, which come out as the pairs (0,4) (1,5) (2,6)
-// (3,7), and x is laid out in the same pairs.  ldmatrix hands word t of row g to lane (g, t), which is the fragment layout.  The
-// MMA sums (q - z) x in f32; the scale multiplies the f32 sum of a group, so the weights are never rounded.
+// columns (from the ninth token on: of a second MMA over the same converted weights), and eight codes become (q - z) / 64 with
+// nine instructions (w4_unpack).  The order of k inside an MMA is free as long as both operands agree: a lane's 32-bit word holds
+// columns 8t .. 8t+7, which come out as the pairs (0,4) (1,5) (2,6) (3,7), and x is laid out in the same pairs.  ldmatrix hands
+// word t of row g to lane (g, t), which is the fragment layout.  The MMA sums (q - z) x in f32; the scale multiplies the f32 sum of
+// a group, so the weights are never rounded.
+//
+// Measured: 1 x 4096 x 4096 5.5 us, of which some 4 are launch, first load and sums; 7 x 4096 x 32003 with zero points 24 us, 3.0
+// TB/s, half of the issue slots used: registers hold sixteen warps an SM, with chains of conversion and MMA between their loads.
 //
 // An MLP hands its gated product on in f32 (HALF): rounded to bf16 it would add as much error as the result's own rounding.  The
 // second product brings each token, or its slice of one, to a largest element of 2^13 .. 2^14 by a power of two, rounds it once to
@@ -31,7 +35,7 @@
 
 namespace xs {
 
-constexpr int kSwTokens = 8;
+constexpr int kSwTokens = 16; // at most: two MMAs' columns
 constexpr int kSwWarps = 16;
 constexpr int kSwChunk = 256;               // columns of one stage: 128 bytes a row
 constexpr int kSwStageBytes = 32 * 128;     // 32 rows
@@ -42,13 +46,14 @@ __host__ __device__ constexpr int sw_x_bytes(int T, int chunks_per_block)
 {
     return T * chunks_per_block * kSwChunk * 2;
 }
+// two halves, for alternate tiles, as long as they leave room for the tokens
 __host__ __device__ constexpr int sw_part_bytes(int T)
 {
-    return 2 * kSwWarps * T * kSwPartStride * 4;
+    return (T > 8 ? 1 : 2) * kSwWarps * T * kSwPartStride * 4;
 }
 __host__ __device__ constexpr int sw_smem_bytes(int T, int chunks_per_block, int stages)
 {
-    return 1024 + kSwWarps * stages * (kSwStageBytes + 8) + sw_x_bytes(T, chunks_per_block) + sw_part_bytes(T) + 16;
+    return 1024 + kSwWarps * stages * (kSwStageBytes + 8) + sw_x_bytes(T, chunks_per_block) + sw_part_bytes(T) + 16 + kSwTokens * 4;
 }
 
 template <bool HALF>
@@ -75,7 +80,8 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr)
 // GATED: a warp's 32 rows are the 16 gate rows and the 16 up rows of 16 features.  SUB: 32-column steps in a scale group.
 // early: the weights were complete before the predecessor began.  Cluster size C, chunks_per_block: K in slices.  HALF: x is
 // f32 and enters as f16; out_f32 (GATED): out is written so.
-template <bool GATED, int SUB, bool ZEROS, bool HALF>
+// NT: MMAs' columns, of eight tokens each.
+template <bool GATED, int SUB, bool ZEROS, bool HALF, int NT>
 __global__ void __launch_bounds__(32 * kSwWarps, 1)
 w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, const void *x, void *out, int n_out, int T, int K,
                 int act, int out_f32, int early, int ways, int C, int chunks_per_block, int stages, int32_t *status)
@@ -85,7 +91,6 @@ w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, cons
     constexpr float UNIT = HALF ? kW4HalfUnit : kW4Unit;
 
     extern __shared__ uint8_t smem_raw[];
-    __shared__ float factor[kSwTokens]; // HALF: of each token
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int bands = kSwWarps / ways, band = warp % bands, way = warp / bands; // 32-row bands of a tile
@@ -94,6 +99,7 @@ w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, cons
     float *part = reinterpret_cast<float *>(x_smem + sw_x_bytes(T, chunks_per_block));
     uint64_t *bars = reinterpret_cast<uint64_t *>(reinterpret_cast<uint8_t *>(part) + (sw_part_bytes(T) + 7) / 8 * 8);
     volatile uint32_t *abort_flag = reinterpret_cast<uint32_t *>(bars + kSwWarps * stages);
+    float *factor = reinterpret_cast<float *>(bars + kSwWarps * stages) + 4; // HALF: of each token
     const uint32_t ring = smem_u32(smem) + warp * stages * kSwStageBytes;
     uint64_t *full = bars + warp * stages;
 
@@ -178,7 +184,7 @@ w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, cons
     {
         // the warps of a token: two for each of eight, all for a single one; a thread has BATCH pieces of eight columns on their way
         constexpr int BATCH = 4;
-        const int spread = T > 4 ? 2 : T > 2 ? 4 : T > 1 ? 8 : 16, n = warp / spread, step = spread * 32, first_p = (warp & (spread - 1)) * 32 + lane;
+        const int spread = NT > 1 ? 1 : T > 4 ? 2 : T > 2 ? 4 : T > 1 ? 8 : 16, n = warp / spread, step = spread * 32, first_p = (warp & (spread - 1)) * 32 + lane;
         const int pieces = n < T ? (chunk_end - chunk0) * (kSwChunk / 8) : 0;
         const int there = min(pieces, K / 8 - chunk0 * (kSwChunk / 8)); // the last slice may end inside a chunk
         const size_t row = static_cast<size_t>(n) * K + chunk0 * kSwChunk;
@@ -259,14 +265,16 @@ w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, cons
     // multiple of 1024, so piece j is one XOR away
     const uint32_t frag = lane * 128 + ((lane & 7) << 4);
     // lanes of tokens that are not there read the last one: a column of its own, which is not stored
-    const uint32_t x_lane = smem_u32(x_smem) + ((g < T ? g : T - 1) * 4 + t) * 16;
+    uint32_t x_lane[NT];
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+        x_lane[i] = smem_u32(x_smem) + (min(i * 8 + g, T - 1) * 4 + t) * 16;
     const int x_step = T * 64;
-    const float factor_even = HALF && 2 * t < T ? factor[2 * t] : 1.0f, factor_odd = HALF && 2 * t + 1 < T ? factor[2 * t + 1] : 1.0f;
     const int share = features / C, share_log = 31 - __clz(share); // features of a tile that this block finishes: a power of two
     int stage = 0, parity = 0;
     uint32_t phase = 0;
-    for (int tile = tile0; tile < tiles; tile += tile_step, parity ^= 1) {
-        float acc[2][4] = {};
+    for (int tile = tile0; tile < tiles; tile += tile_step, parity ^= NT == 1 ? 1 : 0) {
+        float acc[2][NT][4] = {};
         for (int chunk = first; chunk < chunk_end; chunk += ways) {
             fetch(stage == 0 ? stages - 1 : stage - 1);
             uint32_t sc_after[4][SLOTS];
@@ -276,12 +284,15 @@ w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, cons
                 atomicOr(status, kStatusWaitTimeout);
             }
             const uint32_t st = ring + stage * kSwStageBytes + frag;
-            uint32_t xa = x_lane + (chunk - chunk0) * (kSwChunk / 32) * x_step;
-            float c[2][4], s[2][2];
+            uint32_t xa = (chunk - chunk0) * (kSwChunk / 32) * x_step;
+            float c[2][NT][4], s[2][2];
             uint32_t z[2][2];
 #pragma unroll
             for (int j = 0; j < kSwChunk / 32; j++) {
-                const uint4 b = lds128(xa);
+                uint4 b[NT];
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+                    b[i] = lds128(x_lane[i] + xa);
                 xa += x_step;
                 uint32_t q[4];
                 ldmatrix_x4(q, st ^ (j << 4));
@@ -303,15 +314,19 @@ w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, cons
                         else
                             w4_unpack(a[h], q[m * 2 + h], z[m][h]);
                     }
-                    if (j % SUB == 0)
-                        c[m][0] = c[m][1] = c[m][2] = c[m][3] = 0.0f;
-                    mma_16816<HALF>(c[m], a[0][0], a[1][0], a[0][1], a[1][1], b.x, b.y);
-                    mma_16816<HALF>(c[m], a[0][2], a[1][2], a[0][3], a[1][3], b.z, b.w);
-                    if (j % SUB == SUB - 1) {
-                        acc[m][0] = fmaf(s[m][0], c[m][0], acc[m][0]);
-                        acc[m][1] = fmaf(s[m][0], c[m][1], acc[m][1]);
-                        acc[m][2] = fmaf(s[m][1], c[m][2], acc[m][2]);
-                        acc[m][3] = fmaf(s[m][1], c[m][3], acc[m][3]);
+#pragma unroll
+                    for (int i = 0; i < NT; i++) {
+                        float (&sum)[4] = c[m][i], (&total)[4] = acc[m][i];
+                        if (j % SUB == 0)
+                            sum[0] = sum[1] = sum[2] = sum[3] = 0.0f;
+                        mma_16816<HALF>(sum, a[0][0], a[1][0], a[0][1], a[1][1], b[i].x, b[i].y);
+                        mma_16816<HALF>(sum, a[0][2], a[1][2], a[0][3], a[1][3], b[i].z, b[i].w);
+                        if (j % SUB == SUB - 1) {
+                            total[0] = fmaf(s[m][0], sum[0], total[0]);
+                            total[1] = fmaf(s[m][0], sum[1], total[1]);
+                            total[2] = fmaf(s[m][1], sum[2], total[2]);
+                            total[3] = fmaf(s[m][1], sum[3], total[3]);
+                        }
                     }
                 }
             }
@@ -330,12 +345,20 @@ w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, cons
         }
         float *mine = part + (parity * kSwWarps + warp) * part_floats;
 #pragma unroll
-        for (int m = 0; m < 2; m++)
+        for (int i = 0; i < NT; i++)
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (2 * t + (e & 1) < T)
-                    mine[(2 * t + (e & 1)) * kSwPartStride + m * 16 + (e >> 1) * 8 + g] = HALF ? acc[m][e] * (e & 1 ? factor_odd : factor_even) : acc[m][e];
-        // one barrier a tile: the next tile's sums go to the other half of `part`
+            for (int e = 0; e < 2; e++) {
+                const int token = i * 8 + 2 * t + e;
+                if (token < T) {
+                    const float f = HALF ? factor[token] : 1.0f;
+#pragma unroll
+                    for (int m = 0; m < 2; m++) {
+                        mine[token * kSwPartStride + m * 16 + g] = acc[m][i][e] * f;
+                        mine[token * kSwPartStride + m * 16 + 8 + g] = acc[m][i][2 + e] * f;
+                    }
+                }
+            }
+        // one barrier a tile: the next tile's sums go to the other half of `part`, if it has two
         if (C > 1)
             cluster_barrier();
         else
@@ -359,6 +382,12 @@ w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, cons
                 else
                     static_cast<__nv_bfloat16 *>(out)[o] = __float2bfloat16_rn(r);
             }
+        }
+        if (NT > 1 && tile + tile_step < tiles) {
+            if (C > 1)
+                cluster_barrier();
+            else
+                __syncthreads();
         }
     }
     if (C > 1)

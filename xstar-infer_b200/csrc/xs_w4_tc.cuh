@@ -1,4 +1,4 @@
-// Products with 4-bit weights on the tensor core, for batches from nine tokens up: out = x W^T (or act(x Wg^T) * (x Wu^T)).
+// Products with 4-bit weights on the tensor core, for larger batches: out = x W^T (or act(x Wg^T) * (x Wu^T)).
 //
 // tcgen05.mma with the WEIGHTS as its M rows, taken from TMEM, and the tokens as its N columns, taken from shared memory.  The codes
 // arrive by TMA as they lie in memory; sixteen warps turn them into f16, thread = weight row, and store them with tcgen05.st
