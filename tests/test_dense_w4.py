@@ -5,6 +5,7 @@ roundings to bf16 (output, the gated product, the intermediate rows of a block) 
 spread evenly, so each adds at most 2^-8 / sqrt(3) of the result in the root mean square, and no chain here has more than six:
 sqrt(6 / 3) * 2^-8 < 2^-7."""
 import ctypes as C
+import threading
 
 import pytest
 import torch
@@ -321,6 +322,34 @@ def test_linear_with_few_tokens_and_long_rows(T, K):
     many, tol = du.linear_reference(w, torch.cat([x, x.new_zeros(17, K)]))
     assert torch.equal(many[:T], ref)
     du.assert_close(out, ref, tol[:T])
+
+
+@pytest.mark.gpu
+def test_threads_with_calls_of_different_size():
+    # the same kernel with little and with much shared memory, from two threads on two streams
+    g = du.gen(44)
+    cases = [(du.weight(g, 256, K, 64, False), du.bf16(g, (T, K))) for T, K in ((1, 256), (8, 16384), (3, 4096))]
+    want = [du.linear(w, x)[0] for w, x in cases]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(w, x, ref):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                out, ws = du.linear(w, x)
+                for _ in range(300):
+                    du.linear(w, x, out, ws)
+                torch.cuda.current_stream().synchronize()
+                assert torch.equal(out, ref)
+        except Exception as e:  # noqa: BLE001
+            failed.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(*c, r)) for c, r in zip(cases, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
 
 
 @pytest.mark.gpu

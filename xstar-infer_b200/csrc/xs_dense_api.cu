@@ -1,6 +1,8 @@
 // C ABI of include/xs_moe_dense.h: argument checks, workspace plans and launches.  No exception leaves this file.
 #include "xs_moe_dense.h"
 
+#include <atomic>
+
 #include "xs_api_common.cuh"
 #include "xs_norm_residual.cuh"
 #include "xs_w4_prepare.cuh"
@@ -150,6 +152,24 @@ int make_tmap_codes(CUtensorMap *m, const XsMoeW4 *w, int parts, uint32_t box_ro
     return 0;
 }
 
+// The shared memory that a kernel may ask for, set once for each device, to the most that any of its launches takes: two threads
+// that set it to what their own call needs would undo one another's.
+struct SmemLimit {
+    std::atomic<uint64_t> done{0};
+    template <typename Kernel>
+    int set(Kernel *kern, int bytes)
+    {
+        int dev = 0;
+        XS_CUDA(cudaGetDevice(&dev));
+        const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+        if (!(done.load(std::memory_order_acquire) & bit)) {
+            XS_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+            done.fetch_or(bit, std::memory_order_release);
+        }
+        return 0;
+    }
+};
+
 // A programmatic dependent launch in clusters of `cluster` blocks.
 template <typename... KArgs, typename... Args>
 cudaError_t launch_pdl_cluster(void (*kern)(KArgs...), int grid, int block, int cluster, size_t smem, cudaStream_t st, Args &&...args)
@@ -221,7 +241,9 @@ int launch_small_t(const XsMoeW4 *w, const void *x, int T, void *out, int act, b
     if (int rc = make_tmap_codes(&map, w, GATED ? 2 : 1, GATED ? 16 : 32))
         return rc;
     auto kern = xs::w4_small_kernel<GATED, SUB, ZEROS, HALF, NT>;
-    XS_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
+    static SmemLimit limit;
+    if (int rc = limit.set(kern, di.max_smem))
+        return rc;
     XS_CUDA(launch_pdl_cluster(kern, p.grid, 32 * xs::kSwWarps, p.cluster, p.smem, st, map, matrix_of(w), x, out, n_out, T, w->cols, act, out_f32 ? 1 : 0,
                                early ? 1 : 0, p.ways, p.cluster, p.chunks_per_block, p.stages, status));
     note_launch();
@@ -350,7 +372,9 @@ int launch_tc_t(const XsMoeW4 *w, const TcPlan &p, const void *x16, void *out, c
 {
     auto kern = xs::w4_tc_kernel<CG, N_TILE, GATED>;
     constexpr int smem = xs::tc_smem_bytes(CG, N_TILE);
-    XS_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static SmemLimit limit;
+    if (int rc = limit.set(kern, smem))
+        return rc;
     CUtensorMap mw, mx;
     if (int rc = make_tmap_codes(&mw, w, GATED ? 2 : 1, GATED ? xs::kTcRows / 2 : xs::kTcRows))
         return rc;
@@ -619,6 +643,8 @@ int launch_norm_rows(const xs::NormResidualArgs &a, int sms, cudaStream_t st)
     return launch_norm_t<512, 4, ALIGNED>(a, sms, st);
 }
 
+constexpr int kNormMaxHidden = 56 * 1024; // a row in shared memory as f32
+
 int launch_norm_residual(const xs::NormResidualArgs &a, cudaStream_t st)
 {
     DeviceInfo di;
@@ -633,14 +659,13 @@ int launch_norm_residual(const xs::NormResidualArgs &a, cudaStream_t st)
     if (low % 16 == 0 && a.H == 16 * 1024)
         return launch_norm_rows<true>(a, di.sms, st);
     const size_t smem = static_cast<size_t>(a.H) * 4;
-    if (smem > 48 * 1024)
-        XS_CUDA(cudaFuncSetAttribute(xs::norm_residual_loop_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    static SmemLimit limit;
+    if (int rc = limit.set(xs::norm_residual_loop_kernel, kNormMaxHidden * 4))
+        return rc;
     XS_CUDA(launch_pdl(xs::norm_residual_loop_kernel, a.rows, xs::kNrLoopThreads, smem, st, a));
     note_launch();
     return 0;
 }
-
-constexpr int kNormMaxHidden = 56 * 1024; // a row in shared memory as f32
 
 int check_norm_shape(int gate_kind, const void *gate, int32_t rows, int32_t hidden)
 {
