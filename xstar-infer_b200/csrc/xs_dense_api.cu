@@ -190,6 +190,48 @@ cudaError_t launch_pdl_cluster(void (*kern)(KArgs...), int grid, int block, int 
     return cudaLaunchKernelEx(&cfg, kern, KArgs(std::forward<Args>(args))...);
 }
 
+// How many clusters of 1, 2, 4 and 8 blocks, each block with an SM to itself, run at one time.  A cluster lies within a GPC, so this is
+// less than the SMs would give: the grid of a plan with one cluster more than that takes twice as long (294 x 2816 x 1516
+// with 36 clusters of four: 22.8 us; planned with what fits: 14.3).
+struct ClusterSlots {
+    int of[4];
+    int operator()(int cluster) const
+    {
+        return of[cluster == 1 ? 0 : cluster == 2 ? 1 : cluster == 4 ? 2 : 3];
+    }
+};
+
+int cluster_slots(const DeviceInfo &di, ClusterSlots *out)
+{
+    static std::atomic<int> known[64][4];
+    int dev = 0;
+    XS_CUDA(cudaGetDevice(&dev));
+    out->of[0] = di.sms;
+    auto kern = xs::w4_small_kernel<false, 4, false, false, 1>;
+    for (int i = 1; i < 4; i++) {
+        int n = dev < 64 ? known[dev][i].load(std::memory_order_relaxed) : 0;
+        if (n == 0) {
+            XS_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, di.max_smem));
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = di.sms / (1 << i) * (1 << i);
+            cfg.blockDim = 32 * xs::kSwWarps;
+            cfg.dynamicSmemBytes = di.max_smem;
+            cudaLaunchAttribute attr;
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = 1 << i;
+            attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+            cfg.attrs = &attr;
+            cfg.numAttrs = 1;
+            XS_CUDA(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+            n = n < 1 ? 1 : n;
+            if (dev < 64)
+                known[dev][i].store(n, std::memory_order_relaxed);
+        }
+        out->of[i] = n;
+    }
+    return 0;
+}
+
 struct SmallPlan {
     int ways = 1, cluster = 1, chunks_per_block = 0, stages = 2, grid = 0, smem = 0;
 };
@@ -197,7 +239,7 @@ struct SmallPlan {
 // How the warps share the work: `ways` warps of a block on the same rows, `cluster` blocks on the same tile.  Taken is what gives
 // the busiest block the least work, counted in chunks of a warp; a tile's sum, barrier and store take about as long as
 // kTileCost of them, a cluster's kClusterCost more.
-SmallPlan plan_small(int T, int K, int n_out, int band_rows, int sms, int max_smem)
+SmallPlan plan_small(int T, int K, int n_out, int band_rows, const ClusterSlots &slots, int max_smem)
 {
     constexpr float kTileCost = 0.4f, kClusterCost = 0.6f;
     const int chunks = (K + xs::kSwChunk - 1) / xs::kSwChunk;
@@ -216,7 +258,7 @@ SmallPlan plan_small(int T, int K, int n_out, int band_rows, int sms, int max_sm
         p.smem = xs::sw_smem_bytes(T, p.chunks_per_block, p.stages);
         for (p.ways = xs::kSwWarps; p.ways >= 1; p.ways /= 2) {
             const int tiles = (n_out + xs::kSwWarps / p.ways * band_rows - 1) / (xs::kSwWarps / p.ways * band_rows);
-            const int clusters = tiles < sms / c ? tiles : sms / c, rounds = (tiles + clusters - 1) / clusters;
+            const int clusters = tiles < slots(c) ? tiles : slots(c), rounds = (tiles + clusters - 1) / clusters;
             const int per_warp = (p.chunks_per_block + p.ways - 1) / p.ways;
             const float cost = rounds * (per_warp + kTileCost + (c > 1 ? kClusterCost : 0.0f));
             if (best.grid == 0 || cost < best_cost) {
@@ -236,7 +278,10 @@ int launch_small_t(const XsMoeW4 *w, const void *x, int T, void *out, int act, b
     if (int rc = device_info(&di))
         return rc;
     const int n_out = GATED ? w->rows / 2 : w->rows;
-    const SmallPlan p = plan_small(T, w->cols, n_out, GATED ? 16 : 32, di.sms, di.max_smem);
+    ClusterSlots slots;
+    if (int rc = cluster_slots(di, &slots))
+        return rc;
+    const SmallPlan p = plan_small(T, w->cols, n_out, GATED ? 16 : 32, slots, di.max_smem);
     CUtensorMap map;
     if (int rc = make_tmap_codes(&map, w, GATED ? 2 : 1, GATED ? 16 : 32))
         return rc;
@@ -309,7 +354,7 @@ constexpr struct {
 } kTcTiles[] = {{1, 32, 0.42f}, {1, 64, 0.46f}, {1, 128, 0.6f}, {2, 128, 0.48f}, {2, 256, 0.8f}};
 
 // `features` features from f0 on, with one launch; `tile`: one of kTcTiles, or -1 for the best
-TcPlan plan_tc_part(const XsMoeW4 *w, bool gated, int T, int sms, int f0, int features, int tile)
+TcPlan plan_tc_part(const XsMoeW4 *w, bool gated, int T, const ClusterSlots &all, int f0, int features, int tile)
 {
     const int n_out = gated ? w->rows / 2 : w->rows, K = w->cols, all_raw = (K + 255) / 256;
     TcPlan best;
@@ -326,8 +371,7 @@ TcPlan plan_tc_part(const XsMoeW4 *w, bool gated, int T, int sms, int f0, int fe
             p.n_tile = n_tile;
             p.shape = {n_out, T, K, w->group == 32 ? 5 : w->group == 64 ? 6 : 7, (features + width - 1) / width, (T + n_tile - 1) / n_tile, split, f0};
             const long items = static_cast<long>(p.shape.w_tiles) * p.shape.t_tiles;
-            // clusters of eight whole SMs do not fit everywhere
-            const int slots = split == 8 ? sms / 8 * 3 / 4 : sms / (cg * split);
+            const int slots = all(cg * split);
             if (split > 1 && items > slots)
                 break; // a split block has one tile
             const long rounds = (items + slots - 1) / slots;
@@ -342,21 +386,21 @@ TcPlan plan_tc_part(const XsMoeW4 *w, bool gated, int T, int sms, int f0, int fe
 
 // One launch, or two: whole rounds of tiles on every SM, and what would have been a last round of few tiles in another shape.
 // Returns the number of launches.
-int plan_tc(const XsMoeW4 *w, bool gated, int T, int sms, TcPlan (&plan)[2])
+int plan_tc(const XsMoeW4 *w, bool gated, int T, const ClusterSlots &all, TcPlan (&plan)[2])
 {
     // A second launch starts cold; the estimate has to say that it pays (45 x 4096 x 20480: 38.8 us with it, 42.3 without).
     constexpr float kLaunchCost = 6.0f, kGain = 0.9f;
     const int n_out = gated ? w->rows / 2 : w->rows;
-    plan[0] = plan_tc_part(w, gated, T, sms, 0, n_out, -1);
+    plan[0] = plan_tc_part(w, gated, T, all, 0, n_out, -1);
     float cost = plan[0].cost;
     int parts = 1;
     for (int i = 0; i < 5; i++) {
-        const int cg = kTcTiles[i].cg, n_tile = kTcTiles[i].n_tile, width = (gated ? xs::kTcRows / 2 : xs::kTcRows) * cg, slots = sms / cg;
+        const int cg = kTcTiles[i].cg, n_tile = kTcTiles[i].n_tile, width = (gated ? xs::kTcRows / 2 : xs::kTcRows) * cg, slots = all(cg);
         const long t_tiles = (T + n_tile - 1) / n_tile, items = (n_out + width - 1) / width * t_tiles, rounds = items / slots;
         const int first = static_cast<int>(rounds * slots / t_tiles) * width; // features of the whole rounds
         if (rounds == 0 || first <= 0 || first >= n_out)
             continue;
-        const TcPlan a = plan_tc_part(w, gated, T, sms, 0, first, i), b = plan_tc_part(w, gated, T, sms, first, n_out - first, -1);
+        const TcPlan a = plan_tc_part(w, gated, T, all, 0, first, i), b = plan_tc_part(w, gated, T, all, first, n_out - first, -1);
         if (a.cost + b.cost + kLaunchCost < cost * (parts == 1 ? kGain : 1.0f)) {
             cost = a.cost + b.cost + kLaunchCost;
             plan[0] = a;
@@ -392,7 +436,10 @@ int launch_tc(const XsMoeW4 *w, const void *x16, int T, void *out, const xs::TcO
     if (int rc = device_info(&di))
         return rc;
     TcPlan plan[2];
-    const int parts = plan_tc(w, GATED, T, di.sms, plan);
+    ClusterSlots slots;
+    if (int rc = cluster_slots(di, &slots))
+        return rc;
+    const int parts = plan_tc(w, GATED, T, slots, plan);
     for (int i = 0; i < parts; i++) {
         const TcPlan &p = plan[i];
         int rc = 0;
@@ -415,8 +462,9 @@ int launch_tc(const XsMoeW4 *w, const void *x16, int T, void *out, const xs::TcO
 // Which kernel: up to sixteen tokens the one that streams weights past the tokens, if a cluster's shared memory holds them.  4096 x
 // 4096 with 1, 8, 9, 16 tokens: 5.5, 6.5, 7.7, 8.8 us against 11.3, 11.4, 11.5, 11.8 on the tensor core; 8 x 4096 x 32003 with
 // zero points 24 us against 40, 16 tokens 34 against 40.  Clusters of eight do not fill the SMs: more than eight tokens go to the tensor
-// core before they take one (16 x 11264 x 4096: 22 us against 41); up to eight they gain more than they lose (8 x 20480 x 16384 66 us
-// against 82, 1 x 262144 x 4096 230 against 340, but 8 x 20480 x 4096 with zero points 42 against 31).
+// core before they take one (16 x 11264 x 4096 with zero points: 22 us against 34; 13 x 16384 x 16384: 65 against 76); up to eight they
+// gain more than they lose (8 x 20480 x 16384 63 us against 83, 1 x 262144 x 4096 185 against 332, but 8 x 20480 x 4096 with
+// zero points 34 against 31).
 constexpr int kBlockSmem = 227 * 1024;
 bool small_batch(int T, int K)
 {
