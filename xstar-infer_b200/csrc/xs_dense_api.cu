@@ -255,7 +255,7 @@ SmallPlan plan_small(int T, int K, int n_out, int band_rows, const ClusterSlots 
             continue;
         for (p.stages = xs::kSwMaxStages; xs::sw_smem_bytes(T, p.chunks_per_block, p.stages) > max_smem; p.stages--) {
         }
-        p.smem = xs::sw_smem_bytes(T, p.chunks_per_block, p.stages);
+        p.smem = static_cast<int>(xs::sw_smem_bytes(T, p.chunks_per_block, p.stages));
         for (p.ways = xs::kSwWarps; p.ways >= 1; p.ways /= 2) {
             const int tiles = (n_out + xs::kSwWarps / p.ways * band_rows - 1) / (xs::kSwWarps / p.ways * band_rows);
             const int clusters = tiles < slots(c) ? tiles : slots(c), rounds = (tiles + clusters - 1) / clusters;
@@ -282,6 +282,8 @@ int launch_small_t(const XsMoeW4 *w, const void *x, int T, void *out, int act, b
     if (int rc = cluster_slots(di, &slots))
         return rc;
     const SmallPlan p = plan_small(T, w->cols, n_out, GATED ? 16 : 32, slots, di.max_smem);
+    if (p.grid == 0)
+        return fail(XS_MOE_ERR_UNSUPPORTED, "internal: no plan for %d tokens of %d columns", T, w->cols);
     CUtensorMap map;
     if (int rc = make_tmap_codes(&map, w, GATED ? 2 : 1, GATED ? 16 : 32))
         return rc;

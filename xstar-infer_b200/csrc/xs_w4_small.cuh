@@ -42,16 +42,17 @@ constexpr int kSwStageBytes = 32 * 128;     // 32 rows
 constexpr int kSwPartStride = 33;           // floats between tokens in the partial sums of a warp
 constexpr int kSwMaxStages = 4;
 
-__host__ __device__ constexpr int sw_x_bytes(int T, int chunks_per_block)
+// in 64 bits: the host asks for rows of any length, most of which do not fit
+__host__ __device__ constexpr int64_t sw_x_bytes(int T, int chunks_per_block)
 {
-    return T * chunks_per_block * kSwChunk * 2;
+    return static_cast<int64_t>(T) * chunks_per_block * kSwChunk * 2;
 }
 // two halves, for alternate tiles, as long as they leave room for the tokens
 __host__ __device__ constexpr int sw_part_bytes(int T)
 {
     return (T > 8 ? 1 : 2) * kSwWarps * T * kSwPartStride * 4;
 }
-__host__ __device__ constexpr int sw_smem_bytes(int T, int chunks_per_block, int stages)
+__host__ __device__ constexpr int64_t sw_smem_bytes(int T, int chunks_per_block, int stages)
 {
     return 1024 + kSwWarps * stages * (kSwStageBytes + 8) + sw_x_bytes(T, chunks_per_block) + sw_part_bytes(T) + 16 + kSwTokens * 4;
 }
