@@ -413,10 +413,10 @@ int plan_tc(const XsMoeW4 *w, bool gated, int T, const ClusterSlots &all, TcPlan
     return parts;
 }
 
-template <int CG, int N_TILE, bool GATED>
-int launch_tc_t(const XsMoeW4 *w, const TcPlan &p, const void *x16, void *out, const xs::TcOperands &ops, int act, int32_t *status, cudaStream_t st)
+template <int CG, int N_TILE, bool GATED, typename Out>
+int launch_tc_t(const XsMoeW4 *w, const TcPlan &p, const void *x16, Out *out, const xs::TcOperands &ops, int act, int32_t *status, cudaStream_t st)
 {
-    auto kern = xs::w4_tc_kernel<CG, N_TILE, GATED>;
+    auto kern = xs::w4_tc_kernel<CG, N_TILE, GATED, Out>;
     constexpr int smem = xs::tc_smem_bytes(CG, N_TILE);
     static SmemLimit limit;
     if (int rc = limit.set(kern, smem))
@@ -431,8 +431,8 @@ int launch_tc_t(const XsMoeW4 *w, const TcPlan &p, const void *x16, void *out, c
     return 0;
 }
 
-template <bool GATED>
-int launch_tc(const XsMoeW4 *w, const void *x16, int T, void *out, const xs::TcOperands &ops, int act, int32_t *status, cudaStream_t st)
+template <bool GATED, typename Out>
+int launch_tc(const XsMoeW4 *w, const void *x16, int T, Out *out, const xs::TcOperands &ops, int act, int32_t *status, cudaStream_t st)
 {
     DeviceInfo di;
     if (int rc = device_info(&di))
@@ -446,15 +446,15 @@ int launch_tc(const XsMoeW4 *w, const void *x16, int T, void *out, const xs::TcO
         const TcPlan &p = plan[i];
         int rc = 0;
         if (p.cg == 2 && p.n_tile == 128)
-            rc = launch_tc_t<2, 128, GATED>(w, p, x16, out, ops, act, status, st);
+            rc = launch_tc_t<2, 128, GATED, Out>(w, p, x16, out, ops, act, status, st);
         else if (p.cg == 2)
-            rc = launch_tc_t<2, 256, GATED>(w, p, x16, out, ops, act, status, st);
+            rc = launch_tc_t<2, 256, GATED, Out>(w, p, x16, out, ops, act, status, st);
         else if (p.n_tile == 128)
-            rc = launch_tc_t<1, 128, GATED>(w, p, x16, out, ops, act, status, st);
+            rc = launch_tc_t<1, 128, GATED, Out>(w, p, x16, out, ops, act, status, st);
         else if (p.n_tile == 64)
-            rc = launch_tc_t<1, 64, GATED>(w, p, x16, out, ops, act, status, st);
+            rc = launch_tc_t<1, 64, GATED, Out>(w, p, x16, out, ops, act, status, st);
         else
-            rc = launch_tc_t<1, 32, GATED>(w, p, x16, out, ops, act, status, st);
+            rc = launch_tc_t<1, 32, GATED, Out>(w, p, x16, out, ops, act, status, st);
         if (rc)
             return rc;
     }
@@ -479,9 +479,9 @@ bool small_mlp(const XsMoeW4 *gu, const XsMoeW4 *dn, int T)
     return small_batch(T, gu->cols) && small_batch(T, dn->cols);
 }
 
-// Scratch of the tensor-core kernel: tokens and scales in f16, zero points, factors.
+// Scratch of the tensor-core kernel: tokens and scales in f16, zero points, factors; of an MLP also its gated product.
 struct TcScratch {
-    size_t x16 = 0, token = 0, l = 0, part = 0, scales[2] = {}, zeros[2] = {}, row[2] = {}, bytes = 0;
+    size_t x16 = 0, token = 0, h = 0, scales[2] = {}, zeros[2] = {}, row[2] = {}, bytes = 0;
 };
 
 int groups_pitch(const XsMoeW4 *w)
@@ -489,18 +489,20 @@ int groups_pitch(const XsMoeW4 *w)
     return (w->cols / w->group + 7) / 8 * 8;
 }
 
-TcScratch plan_scratch(const XsMoeW4 *first, const XsMoeW4 *second, int T, size_t at)
+TcScratch plan_scratch(const XsMoeW4 *first, const XsMoeW4 *second, int T)
 {
     TcScratch p;
+    size_t at = kStatusBytes;
     auto take = [&](size_t bytes) {
         const size_t o = at;
         at = align_up(at + bytes, 256);
         return o;
     };
-    p.x16 = take(static_cast<size_t>(T) * first->cols * 2);
-    for (size_t *o : {&p.token, &p.l})
-        *o = take(static_cast<size_t>(T) * 4);
-    p.part = take(static_cast<size_t>(first->rows) * 4);
+    // the second product's tokens take the place of the first one's
+    p.x16 = take(static_cast<size_t>(T) * (second && second->cols > first->cols ? second->cols : first->cols) * 2);
+    p.token = take(static_cast<size_t>(T) * 4);
+    if (second)
+        p.h = take(static_cast<size_t>(T) * second->cols * 4);
     const XsMoeW4 *w[2] = {first, second};
     for (int i = 0; i < 2; i++) {
         if (!w[i])
@@ -514,19 +516,9 @@ TcScratch plan_scratch(const XsMoeW4 *first, const XsMoeW4 *second, int T, size_
     return p;
 }
 
-// What a product of `cols` columns adds to the exponent of its bound: |g| |u| <= 2^(2 l) cols 2^(2 * 4) max s(gate) max s(up), brought
-// to 2^15 at most.
-int bound_exponent(int cols)
-{
-    int log = 0;
-    while ((1 << log) < cols)
-        log++;
-    return log + 8 - 15;
-}
-
 // Tokens (normed by `norm` where it is given) and the scales of up to two matrices.
-int launch_prepare(const XsMoeW4 *first, bool pair, const XsMoeW4 *second, const XsMoeBlockNorms *norm, const void *x, int T, uint8_t *ws,
-                   const TcScratch &p, cudaStream_t st, int *pair_parts = nullptr)
+int launch_prepare(const XsMoeW4 *first, const XsMoeW4 *second, const XsMoeBlockNorms *norm, const void *x, int T, uint8_t *ws, const TcScratch &p,
+                   cudaStream_t st)
 {
     DeviceInfo di;
     if (int rc = device_info(&di))
@@ -540,7 +532,6 @@ int launch_prepare(const XsMoeW4 *first, bool pair, const XsMoeW4 *second, const
     }
     a.x16 = reinterpret_cast<__half *>(ws + p.x16);
     a.factor = reinterpret_cast<float *>(ws + p.token);
-    a.l = reinterpret_cast<int *>(ws + p.l);
     a.T = T;
     a.K = first->cols;
     const XsMoeW4 *w[2] = {first, second};
@@ -567,16 +558,11 @@ int launch_prepare(const XsMoeW4 *first, bool pair, const XsMoeW4 *second, const
         m.per_block = at_once;
         if (m.rows > 8 * di.sms * at_once)
             m.per_block = 4 * at_once < xs::kPrepRows ? 4 * at_once : xs::kPrepRows;
-        const int rows = i == 0 && pair ? m.rows / 2 : m.rows, per = i == 0 && pair ? m.per_block / 2 : m.per_block;
-        m.blocks = (rows + per - 1) / per;
+        m.blocks = (m.rows + m.per_block - 1) / m.per_block;
         blocks += m.blocks;
     }
-    a.pair = pair ? 1 : 0;
-    a.pair_part = reinterpret_cast<int *>(ws + p.part);
     XS_CUDA(launch_pdl(xs::w4_prepare_kernel, blocks, xs::kPrepThreads, 0, st, a));
     note_launch();
-    if (pair_parts)
-        *pair_parts = a.m[0].blocks;
     return 0;
 }
 
@@ -593,7 +579,7 @@ xs::TcOperands operands(const XsMoeW4 *w, const uint8_t *ws, const TcScratch &p,
 
 size_t linear_bytes(const XsMoeW4 *w, int T)
 {
-    return small_batch(T, w->cols) ? kStatusBytes : plan_scratch(w, nullptr, T, kStatusBytes).bytes;
+    return small_batch(T, w->cols) ? kStatusBytes : plan_scratch(w, nullptr, T).bytes;
 }
 
 int run_linear(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void *out, uint8_t *ws, cudaStream_t st)
@@ -601,19 +587,20 @@ int run_linear(const XsMoeW4 *w, bool gated, int act, const void *x, int T, void
     int32_t *status = reinterpret_cast<int32_t *>(ws);
     if (small_batch(T, w->cols))
         return run_small(w, gated, act, x, T, out, status, st);
-    const TcScratch p = plan_scratch(w, nullptr, T, kStatusBytes);
-    if (int rc = launch_prepare(w, gated, nullptr, nullptr, x, T, ws, p, st))
+    const TcScratch p = plan_scratch(w, nullptr, T);
+    if (int rc = launch_prepare(w, nullptr, nullptr, x, T, ws, p, st))
         return rc;
     const xs::TcOperands ops = operands(w, ws, p, 0);
-    return gated ? launch_tc<true>(w, ws + p.x16, T, out, ops, act, status, st) : launch_tc<false>(w, ws + p.x16, T, out, ops, 0, status, st);
+    __nv_bfloat16 *o = static_cast<__nv_bfloat16 *>(out);
+    return gated ? launch_tc<true>(w, ws + p.x16, T, o, ops, act, status, st) : launch_tc<false>(w, ws + p.x16, T, o, ops, 0, status, st);
 }
 
-// The gated product and the down product share one scratch: h behind the status block, then what the tensor-core kernel needs.
+// The gated product and the down product share one scratch: behind the status block h alone, or what the tensor-core kernel needs.
 size_t mlp_bytes(const XsMoeW4 *gu, const XsMoeW4 *dn, int T)
 {
     if (small_mlp(gu, dn, T))
         return kStatusBytes + static_cast<size_t>(T) * (gu->rows / 2) * 4;
-    return plan_scratch(gu, dn, T, kStatusBytes + bf16_bytes(T, gu->rows / 2)).bytes;
+    return plan_scratch(gu, dn, T).bytes;
 }
 
 // norm: the rows of x are normed on the way to the tensor core (null for small batches, and where there is no norm).
@@ -622,28 +609,21 @@ int run_mlp(const XsMoeW4 *gu, const XsMoeW4 *dn, int32_t act, const XsMoeBlockN
             bool after_norm = false)
 {
     int32_t *status = reinterpret_cast<int32_t *>(ws);
-    uint8_t *h = ws + kStatusBytes;
     if (small_mlp(gu, dn, T)) {
+        uint8_t *h = ws + kStatusBytes;
         if (int rc = launch_small<true, false>(gu, x, T, h, act, true, after_norm, status, st))
             return rc;
         return launch_small<false, true>(dn, h, T, out, 0, false, true, status, st);
     }
-    const TcScratch p = plan_scratch(gu, dn, T, kStatusBytes + bf16_bytes(T, gu->rows / 2));
-    int pair_parts = 0;
-    if (int rc = launch_prepare(gu, true, dn, norm, x, T, ws, p, st, &pair_parts))
+    const TcScratch p = plan_scratch(gu, dn, T);
+    if (int rc = launch_prepare(gu, dn, norm, x, T, ws, p, st))
         return rc;
-    xs::TcOperands up = operands(gu, ws, p, 0), down = operands(dn, ws, p, 1);
-    up.out_f16 = 1;
-    down.token = nullptr;
-    for (xs::TcOperands *o : {&up, &down}) {
-        o->l = reinterpret_cast<const int *>(ws + p.l);
-        o->pair_part = reinterpret_cast<const int *>(ws + p.part);
-        o->parts = pair_parts;
-        o->bound_add = bound_exponent(gu->cols);
-    }
-    if (int rc = launch_tc<true>(gu, ws + p.x16, T, h, up, act, status, st))
+    float *h = reinterpret_cast<float *>(ws + p.h), *token = reinterpret_cast<float *>(ws + p.token);
+    if (int rc = launch_tc<true>(gu, ws + p.x16, T, h, operands(gu, ws, p, 0), act, status, st))
         return rc;
-    return launch_tc<false>(dn, h, T, out, down, 0, status, st);
+    XS_CUDA(launch_pdl(xs::w4_rescale_kernel, T, xs::kRescaleThreads, 0, st, h, reinterpret_cast<__half *>(ws + p.x16), token, dn->cols));
+    note_launch();
+    return launch_tc<false>(dn, ws + p.x16, T, static_cast<__nv_bfloat16 *>(out), operands(dn, ws, p, 1), 0, status, st);
 }
 
 template <int GROUP, int ITER, bool ALIGNED>

@@ -91,6 +91,12 @@ __device__ __forceinline__ float finite_abs(float v)
     return a <= 3.4e38f ? a : 0.0f; // infinities and NaN do not count
 }
 
+// The power of two that brings a token whose largest element is `top` to 2^13 .. 2^14.
+__device__ __forceinline__ int token_exponent(float top)
+{
+    return max(kExpMin, min(kExpMax, log2_floor(top) - 13));
+}
+
 // silu: v / (1 + exp(-v)); gelu: v / 2 * (1 + tanh(c (v + 0.044715 v^3))), and (1 + tanh(a)) / 2 = 1 / (1 + exp(-2 a)).  The fast
 // exponential and division are off by a few f32 steps, far below the step of the result; far below zero, where the
 // exponential leaves f32, the division gives the zero that the result is.

@@ -8,9 +8,9 @@
 // alignment of the originals; a row whose scales differ by less than 2^4 is marked, and takes a shorter conversion there.  The powers of
 // two come back in the kernel's epilogue.
 //
-// The gated product's own result becomes the next product's token, and must be scaled before the largest of a row is known: by
-// a bound, |act(g) u| <= |g| |u| <= (|x| |w_g|) (|x| |w_u|) with |w| <= sqrt(K) 15 max s (2-norms).  The bound lies some 2^15 above
-// what occurs, of the 2^39 that f16 spans; the products of a row smaller than that again lose bits.
+// The gated product's own result becomes the next product's token.  It is handed on in f32 and scaled like a token, by its own
+// largest element (w4_rescale_kernel): a bound from the norms of token and weights, with which it could be written in f16 at
+// once, may lie any distance above what occurs, where the weights do not take a large element of the token or the gate closes.
 //
 // Bytes decide: tokens are read once and written once; the scales are a fiftieth of the weights.  With `norm_w` the tokens are
 // normed on the way (the first norm of a block): v / sqrt(mean v^2 + eps) * (offset + w), rounded once, to f16.  8192 tokens of
@@ -33,7 +33,7 @@ struct PrepareScales {
     uint8_t *zeros8;        // (rows, pitch)
     float *factor;          // 2^(c + 9) of a row: what its sums are multiplied by; negative for a row of wide range
     int rows, groups, pitch;
-    int per_block, blocks; // rows of a block (half gate, half up rows where they go together)
+    int per_block, blocks; // rows of a block
     int lanes;             // lanes on a row: a power of two; 8 groups each at a time if `vec`
     int vec;
 };
@@ -41,12 +41,9 @@ struct PrepareArgs {
     const __nv_bfloat16 *x, *norm_w;
     __half *x16;
     float *factor; // token = x16 * factor
-    int *l;        // 2-norm of the token <= 2^l
     int T, K;
     float eps, offset;
     PrepareScales m[2];   // the second may be empty (blocks = 0)
-    int pair;             // m[0] is gate and up: rows i and i + rows / 2 go together
-    int *pair_part;       // for each block of m[0]: its largest exponent(gate) + exponent(up)
 };
 
 constexpr int kPrepThreads = 128;
@@ -62,8 +59,7 @@ __device__ __forceinline__ float prep_get(const uint4 &v, int i)
 __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareArgs a)
 {
     constexpr int WARPS = kPrepThreads / 32;
-    __shared__ float part[3][WARPS];
-    __shared__ int ipart[WARPS], row_exp[kPrepRows];
+    __shared__ float part[2][WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
     pdl_launch_dependents();
@@ -98,12 +94,12 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
             for (int o = 16; o; o >>= 1)
                 ss += __shfl_xor_sync(0xffffffffu, ss, o);
             if (lane == 0)
-                part[2][warp] = ss;
+                part[1][warp] = ss;
             __syncthreads();
             ss = 0.0f;
 #pragma unroll
             for (int i = 0; i < WARPS; i++)
-                ss += part[2][i];
+                ss += part[1][i];
             inv = rsqrtf(ss / static_cast<float>(a.K) + a.eps);
         }
         // the eight columns of a piece, normed
@@ -118,34 +114,25 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
                     f[i] = f[i] * inv * (a.offset + __bfloat162float(w[i]));
             }
         };
-        float top = 0.0f, ss = 0.0f;
+        float top = 0.0f;
         each([&](int p, const uint4 &v) {
             float f[8];
             values(p, v, f);
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float c = finite_abs(f[i]);
-                top = fmaxf(top, c);
-                ss = fmaf(c, c, ss);
-            }
+            for (int i = 0; i < 8; i++)
+                top = fmaxf(top, finite_abs(f[i]));
         });
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
+        for (int o = 16; o; o >>= 1)
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        }
-        if (lane == 0) {
+        if (lane == 0)
             part[0][warp] = top;
-            part[1][warp] = ss;
-        }
         __syncthreads();
-        top = ss = 0.0f;
+        top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < WARPS; i++) {
+        for (int i = 0; i < WARPS; i++)
             top = fmaxf(top, part[0][i]);
-            ss += part[1][i];
-        }
-        const int top_exp = log2_floor(top), e = max(kExpMin, min(kExpMax, top_exp - 13));
+        const int e = token_exponent(top);
         const float down = pow2f(-e);
         uint4 *out = reinterpret_cast<uint4 *>(a.x16 + static_cast<size_t>(t) * a.K);
         each([&](int p, const uint4 &v) {
@@ -157,23 +144,14 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
                 o[i] = __floats2half2_rn(f[2 * i] * down, f[2 * i + 1] * down);
             out[p] = *reinterpret_cast<uint4 *>(o);
         });
-        if (threadIdx.x == 0) {
+        if (threadIdx.x == 0)
             a.factor[t] = pow2f(e);
-            // sqrt(ss) < 2^((k + 1) / 2) with k = floor(log2 ss), and one more for the roundings of the sum; where the squares leave
-            // the range of f32, sqrt(K) times the largest element
-            int l = (log2_floor(ss) + 3) >> 1;
-            if (top_exp > 50 || top_exp < -50)
-                l = top_exp + 1 + (32 - __clz(a.K) + 1) / 2;
-            a.l[t] = l;
-        }
     } else {
         int b = blockIdx.x - a.T;
         const int which = b >= a.m[0].blocks ? 1 : 0;
         if (which)
             b -= a.m[0].blocks;
         const PrepareScales m = which ? a.m[1] : a.m[0];
-        const bool pair = which == 0 && a.pair;
-        const int half_rows = m.rows / 2, half_block = m.per_block / 2;
         const int sub = lane & (m.lanes - 1);
         const int stride = kPrepThreads / m.lanes;
         struct Row {
@@ -206,10 +184,9 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
         };
         auto load = [&](int r) {
             Row w;
-            // a block's first rows are gate rows, its last the up rows of the same features
-            const int i = pair ? b * half_block + (r < half_block ? r : r - half_block) : b * m.per_block + r;
-            w.there = r < m.per_block && i < (pair ? half_rows : m.rows);
-            w.row = w.there ? static_cast<size_t>(i) + (pair && r >= half_block ? half_rows : 0) : 0;
+            const int i = b * m.per_block + r;
+            w.there = r < m.per_block && i < m.rows;
+            w.row = w.there ? static_cast<size_t>(i) : 0;
             w.s0 = make_uint4(0, 0, 0, 0);
             w.z0 = make_uint2(0, 0);
             if (w.there && sub * 8 < m.groups) {
@@ -219,7 +196,7 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
             }
             return w;
         };
-        auto finish = [&](const Row &w, int r) {
+        auto finish = [&](const Row &w) {
             float top = 0.0f, low = 3.4e38f;
             bool odd = false; // an infinity or NaN
             for (int g = sub * 8; g < m.groups; g += m.lanes * 8) {
@@ -257,8 +234,6 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
                 if (sub == 0)
                     m.factor[w.row] = narrow ? pow2f(c + kTcUnitExp) : -pow2f(c + kTcUnitExp);
             }
-            if (pair && sub == 0 && r < m.per_block)
-                row_exp[r] = w.there ? top_exp + 1 : -1000; // the row's scales are below 2^row_exp
         };
         // four rows' loads on their way before the first is worked on
         for (int r = static_cast<int>(threadIdx.x) / m.lanes; r - static_cast<int>(threadIdx.x) / m.lanes < m.per_block; r += 4 * stride) {
@@ -269,24 +244,62 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 if (i * stride + r - static_cast<int>(threadIdx.x) / m.lanes < m.per_block)
-                    finish(w[i], r + i * stride);
-        }
-        if (pair) {
-            __syncthreads();
-            int top = -4000;
-            for (int r = threadIdx.x; r < half_block; r += kPrepThreads)
-                top = max(top, row_exp[r] + row_exp[r + half_block]);
-            top = __reduce_max_sync(0xffffffffu, top);
-            if (lane == 0)
-                ipart[warp] = top;
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                for (int i = 0; i < WARPS; i++)
-                    top = max(top, ipart[i]);
-                a.pair_part[b] = top;
-            }
+                    finish(w[i]);
         }
     }
+}
+
+// f32 rows (T, K) to f16, each scaled by its own largest element like a token above.  One block a row, which it reads once: kept in
+// registers up to 12288 columns, the rest of a longer row from memory again.
+constexpr int kRescaleThreads = 256;
+constexpr int kRescaleKeep = 6;
+__global__ void __launch_bounds__(kRescaleThreads) w4_rescale_kernel(const float *__restrict__ h, __half *__restrict__ h16, float *__restrict__ factor, int K)
+{
+    __shared__ float part[kRescaleThreads / 32];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int pieces = K / 8;
+    const float4 *row = reinterpret_cast<const float4 *>(h + static_cast<size_t>(blockIdx.x) * K);
+    uint4 *out = reinterpret_cast<uint4 *>(h16 + static_cast<size_t>(blockIdx.x) * K);
+    float4 keep[kRescaleKeep][2];
+#pragma unroll
+    for (int i = 0; i < kRescaleKeep; i++) {
+        const int p = threadIdx.x + i * kRescaleThreads;
+        keep[i][0] = keep[i][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (p < pieces) {
+            keep[i][0] = row[2 * p];
+            keep[i][1] = row[2 * p + 1];
+        }
+    }
+    auto most = [](const float4 &v) { return fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w))); };
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kRescaleKeep; i++)
+        top = fmaxf(top, fmaxf(most(keep[i][0]), most(keep[i][1])));
+    for (int p = threadIdx.x + kRescaleKeep * kRescaleThreads; p < pieces; p += kRescaleThreads)
+        top = fmaxf(top, fmaxf(most(row[2 * p]), most(row[2 * p + 1])));
+    const uint32_t of_warp = __reduce_max_sync(0xffffffffu, __float_as_uint(top)); // floats that are not negative are ordered like their bits
+    if ((threadIdx.x & 31) == 0)
+        part[threadIdx.x >> 5] = __uint_as_float(of_warp);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kRescaleThreads / 32; i++)
+        top = fmaxf(top, part[i]);
+    const int e = token_exponent(top);
+    const float down = pow2f(-e);
+    auto store = [&](int p, const float4 &a, const float4 &b) {
+        const __half2 o[4] = {__floats2half2_rn(a.x * down, a.y * down), __floats2half2_rn(a.z * down, a.w * down),
+                              __floats2half2_rn(b.x * down, b.y * down), __floats2half2_rn(b.z * down, b.w * down)};
+        out[p] = *reinterpret_cast<const uint4 *>(o);
+    };
+#pragma unroll
+    for (int i = 0; i < kRescaleKeep; i++)
+        if (static_cast<int>(threadIdx.x) + i * kRescaleThreads < pieces)
+            store(threadIdx.x + i * kRescaleThreads, keep[i][0], keep[i][1]);
+    for (int p = threadIdx.x + kRescaleKeep * kRescaleThreads; p < pieces; p += kRescaleThreads)
+        store(p, row[2 * p], row[2 * p + 1]);
+    if (threadIdx.x == 0)
+        factor[blockIdx.x] = pow2f(e);
 }
 
 } // namespace xs

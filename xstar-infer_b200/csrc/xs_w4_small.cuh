@@ -223,7 +223,7 @@ w4_small_kernel(const __grid_constant__ CUtensorMap tmap, const W4Matrix w, cons
                 part[warp] = __uint_as_float(of_warp);
             __syncthreads();
             const uint32_t of_token = __reduce_max_sync(0xffffffffu, __float_as_uint(part[n * spread + (lane & (spread - 1))]));
-            const int e = max(kExpMin, min(kExpMax, log2_floor(__uint_as_float(of_token)) - 13));
+            const int e = token_exponent(__uint_as_float(of_token));
             const float down = pow2f(-e);
             if (lane == 0 && n < T)
                 factor[n] = pow2f(e);

@@ -57,7 +57,7 @@ __host__ __device__ constexpr int tc_raw_stages(int cg, int n_tile)
 }
 __host__ __device__ constexpr int tc_smem_bytes(int cg, int n_tile)
 {
-    return 1024 + tc_raw_stages(cg, n_tile) * kTcRawBytes + kTcStages * tc_x_bytes(cg, n_tile) + 512 + 4 * 256 * 4; // barriers; factors of two tiles' tokens
+    return 1024 + tc_raw_stages(cg, n_tile) * kTcRawBytes + kTcStages * tc_x_bytes(cg, n_tile) + 512 + 2 * 256 * 4; // barriers; factors of two tiles' tokens
 }
 
 __device__ __forceinline__ bool elect_one()
@@ -155,18 +155,9 @@ struct TcOperands {
     const uint16_t *scales; // f16 (rows, pitch)
     const uint8_t *zeros;   // (rows, pitch) or null: 8
     const float *row;       // factor of a weight row's sums; negative: its scales are of wide range
-    const float *token;     // factor of a token; or null: the tokens are a gated product, scaled by its bound
+    const float *token;     // factor of a token
     int pitch;
-    int out_f16;           // gated: write the product in f16, scaled by its bound
-    const int *l;          // 2-norm of the (gated product's) tokens <= 2^l
-    const int *pair_part;  // its largest is the largest exponent(gate) + exponent(up)
-    int parts, bound_add;  // what the number of columns adds to the bound
 };
-// Exponent of the scale of a token's gated product: the product is below 2^(exponent + 15).
-__device__ __forceinline__ int tc_bound(int l, int pair_and_columns)
-{
-    return max(kExpMin, min(kExpMax, 2 * l + pair_and_columns));
-}
 
 struct TcShape {
     int n_out, T, K, G_log; // G_log: log2 of the group
@@ -185,21 +176,21 @@ __device__ __forceinline__ void tc_tile(const TcShape &s, int item, int &wt, int
     tt = first + r - wt * width;
 }
 
-// One element of the result: v, or act(v) u; in bf16, or scaled by its bound in f16 for the product that follows.
-template <bool GATED>
-__device__ __forceinline__ uint16_t tc_result(const TcOperands &w, int act, float inverse, float v, float u)
+// One element of the result: v, or act(v) u; in bf16, or in f32 for the product that follows.
+template <bool GATED, typename Out>
+__device__ __forceinline__ Out tc_result(int act, float v, float u)
 {
-    if constexpr (GATED) {
+    if constexpr (GATED)
         v = w4_activation(v, act) * u;
-        if (w.out_f16)
-            return __half_as_ushort(__float2half_rn(v * inverse));
-    }
-    return __bfloat16_as_ushort(__float2bfloat16_rn(v));
+    if constexpr (sizeof(Out) == 4)
+        return v;
+    else
+        return __float2bfloat16_rn(v);
 }
 
-template <int CG, int N_TILE, bool GATED>
+template <int CG, int N_TILE, bool GATED, typename Out>
 __global__ void __launch_bounds__(kTcThreads, 1)
-w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const TcOperands w, void *__restrict__ out,
+w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const TcOperands w, Out *__restrict__ out,
              const TcShape s, int act, int32_t *__restrict__ status)
 {
     constexpr int RAW = tc_raw_stages(CG, N_TILE), X_BYTES = tc_x_bytes(CG, N_TILE);
@@ -216,8 +207,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
     uint64_t *acc_full = empty + kTcStages, *acc_empty = acc_full + NBUF;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + NBUF);
     volatile uint32_t *abort_flag = tmem_slot + 1;
-    int *epi_max = reinterpret_cast<int *>(tmem_slot + 2); // eight
-    float *token_smem = reinterpret_cast<float *>(bars) + 128; // [tile parity][factor, inverse of the product's factor][256]
+    float *token_smem = reinterpret_cast<float *>(bars) + 128; // [tile parity][256]
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31; // warp: known to be uniform
     const int rank = CG > 1 || s.split > 1 ? static_cast<int>(cluster_rank()) : 0;
@@ -467,36 +457,15 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
         const int q = warp & 3, part = (warp - kTcEpilogueWarp) >> 2;
         constexpr int COLS = N_TILE / 2; // of this warp
         const int lane_feature = GATED ? q * 16 + (lane & 15) : q * 32 + lane;
-        const bool by_bound = GATED ? w.out_f16 != 0 : w.token == nullptr;
-        int bound = 0;
-        if (by_bound) {
-            int top = -4000;
-            for (int i = threadIdx.x - 32 * kTcEpilogueWarp; i < w.parts; i += 256)
-                top = max(top, __ldg(w.pair_part + i));
-            top = __reduce_max_sync(0xffffffffu, top);
-            if (lane == 0)
-                epi_max[warp - kTcEpilogueWarp] = top;
-            named_barrier_and(true);
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                top = max(top, epi_max[i]);
-            bound = top + w.bound_add;
-        }
         uint32_t use = 0;
         for (int item = item0; item < items; item += item_step, use++) {
             int wt, tt;
             tc_tile(s, item, wt, tt);
             const uint32_t buf = use % NBUF;
             // the factors of this tile's tokens, into the place the tile before last has left
-            float *factor = token_smem + (use & 1) * 512, *inverse = factor + 256;
-            {
-                const int j = threadIdx.x - 32 * kTcEpilogueWarp, t = min(tt * N_TILE + j, s.T - 1);
-                if (j < N_TILE) {
-                    const int e = by_bound ? tc_bound(__ldg(w.l + t), bound) : 0;
-                    factor[j] = GATED || !by_bound ? __ldg(w.token + t) : pow2f(e);
-                    inverse[j] = pow2f(-e);
-                }
-            }
+            float *factor = token_smem + (use & 1) * 256;
+            if (const int j = threadIdx.x - 32 * kTcEpilogueWarp; j < N_TILE)
+                factor[j] = __ldg(w.token + min(tt * N_TILE + j, s.T - 1));
             // one warp asks, sleeping in between, and the others wait at a barrier that costs no issue slots
             if (warp == kTcEpilogueWarp)
                 ok = warp_sleep_wait(&acc_full[buf], (use / NBUF) & 1, abort_flag);
@@ -523,19 +492,15 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                 break; // one tile a block; summed below
             }
             const bool whole = token0 + COLS <= s.T && feature - lane_feature + FEATURES <= s.n_out;
-            uint16_t *o = static_cast<uint16_t *>(out) + static_cast<size_t>(token0 + (GATED && lane >= 16 ? 1 : 0)) * s.n_out + feature;
+            Out *o = out + static_cast<size_t>(token0 + (GATED && lane >= 16 ? 1 : 0)) * s.n_out + feature;
             for (int c = 0; c < COLS; c += 16) {
                 uint32_t v[16];
                 tmem_ld16(acc + c, v);
-                float tf[16], ti[GATED ? 16 : 1];
+                float tf[16];
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
                     const float4 f = *reinterpret_cast<const float4 *>(factor + part * COLS + c + i);
                     tf[i] = f.x, tf[i + 1] = f.y, tf[i + 2] = f.z, tf[i + 3] = f.w;
-                    if constexpr (GATED) {
-                        const float4 g = *reinterpret_cast<const float4 *>(inverse + part * COLS + c + i);
-                        ti[i] = g.x, ti[i + 1] = g.y, ti[i + 2] = g.z, ti[i + 3] = g.w;
-                    }
                 }
                 tmem_ld_wait_16(v);
                 if (c + 16 == COLS) {
@@ -554,14 +519,14 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                         const float got = __shfl_xor_sync(0xffffffffu, up ? even : uneven, 16), f = up ? tf[i + 1] : tf[i];
                         const int t = token0 + c + i + (up ? 1 : 0);
                         if (whole || (feature < s.n_out && t < s.T))
-                            *o = tc_result<true>(w, act, up ? ti[i + 1] : ti[i], (up ? got : even) * f * row_f, (up ? uneven : got) * f * row_u);
+                            *o = tc_result<true, Out>(act, (up ? got : even) * f * row_f, (up ? uneven : got) * f * row_u);
                         o += 2 * static_cast<size_t>(s.n_out);
                     }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
                         if (whole || (feature < s.n_out && token0 + c + i < s.T))
-                            *o = tc_result<false>(w, act, 1.0f, __uint_as_float(v[i]) * tf[i] * row_f, 0.0f);
+                            *o = tc_result<false, Out>(act, __uint_as_float(v[i]) * tf[i] * row_f, 0.0f);
                         o += s.n_out;
                     }
                 }
@@ -604,13 +569,13 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                     if constexpr (GATED)
                         su[0] += u[r].x, su[1] += u[r].y, su[2] += u[r].z, su[3] += u[r].w;
                 }
-            const float t = token_smem[c], inverse = token_smem[256 + c]; // the one tile's
-            uint16_t *o = static_cast<uint16_t *>(out) + static_cast<size_t>(token) * s.n_out + feature;
+            const float t = token_smem[c]; // the one tile's
+            Out *o = out + static_cast<size_t>(token) * s.n_out + feature;
 #pragma unroll
             for (int j = 0; j < 4; j++)
                 if (feature + j < s.n_out)
-                    o[j] = tc_result<GATED>(w, act, inverse, sv[j] * t * fabsf(__ldg(w.row + feature + j)),
-                                            GATED ? su[j] * t * fabsf(__ldg(w.row + s.n_out + feature + j)) : 0.0f);
+                    o[j] = tc_result<GATED, Out>(act, sv[j] * t * fabsf(__ldg(w.row + feature + j)),
+                                                 GATED ? su[j] * t * fabsf(__ldg(w.row + s.n_out + feature + j)) : 0.0f);
         }
     }
     if (*abort_flag)
