@@ -112,7 +112,9 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volati
     bool ok = true;
     if ((threadIdx.x & 31) == 0)
         ok = mbar_wait(bar, parity, abort_flag);
-    return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+    ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+    __syncwarp(); // what the polling lane has seen of memory, the others see behind this; the shuffle orders nothing
+    return ok;
 }
 // The same for waits that are long by nature: sleeps between polls, so that the warp takes no issue slots from those that work.
 // Gives up after about a quarter of a second.
