@@ -106,15 +106,12 @@ __device__ __forceinline__ float w4_activation(float v, int act)
     return __fdividef(v, 1.0f + __expf(-a));
 }
 
-// A bounded wait of a whole warp with one outcome; one lane polls for all.
+// A bounded wait of a whole warp with one outcome.  Every lane asks, since what one of them has seen of memory orders nothing for
+// the others.
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag)
 {
-    bool ok = true;
-    if ((threadIdx.x & 31) == 0)
-        ok = mbar_wait(bar, parity, abort_flag);
-    ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-    __syncwarp(); // what the polling lane has seen of memory, the others see behind this; the shuffle orders nothing
-    return ok;
+    const bool there = mbar_try_wait(bar, parity);
+    return __all_sync(0xffffffffu, there || mbar_wait(bar, parity, abort_flag));
 }
 // The same for waits that are long by nature: sleeps between polls, so that the warp takes no issue slots from those that work.
 // Gives up after about a quarter of a second.
