@@ -292,6 +292,10 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
             tc_tile(s, item, wt, tt);
             for (int r = raw0; r < raw1; r++, n++) {
                 const uint32_t st = n % RAW;
+                // The ring is full, and empties once the other warps begin, behind the kernel before this one: however long that takes, it is
+                // not for the bounded wait below to count.
+                if (n == RAW)
+                    pdl_wait();
                 if (!mbar_wait(&raw_empty[st], ((n / RAW) & 1) ^ 1, abort_flag)) {
                     ok = false;
                     break;
