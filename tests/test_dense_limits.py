@@ -2,8 +2,11 @@
 import ctypes as C
 
 import pytest
+import torch
 
 from xstar_moe import capi
+
+import dense_util as du
 
 
 def _w4(rows, cols, group=128):
@@ -26,3 +29,28 @@ def test_rows_that_no_shared_memory_holds_ask_for_the_scratch_of_larger_batches(
         gate_up, down = _w4(2 * w.cols, 128), _w4(128, w.cols)
         assert L.xs_moe_mlp_w4_workspace_bytes(C.byref(gate_up), C.byref(down), tokens, C.byref(n)) == 0
         assert n.value > 2 * tokens * w.cols + 2 * gate_up.rows
+
+
+# ---- long rows --------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("T, K", [(1, 2**30), (9, 480_000_000)])
+def test_the_longest_rows(T, K):
+    # a tile of the first takes 0.4 s, in one wait of its epilogue
+    N, group = 5, 128
+    q = torch.full((N, K // 2), 0x88, dtype=torch.uint8, device="cuda")
+    s = torch.ones(N, K // group, dtype=torch.bfloat16, device="cuda")
+    x = torch.zeros(T, K, dtype=torch.bfloat16, device="cuda")
+    want = torch.zeros(T, N, dtype=torch.float64)
+    columns = [0, 255, 256, 100_001, K // 8 - 1, K // 8, K // 2 - 1, K // 2 + 77, K - 257, K - 1]
+    for i, k in enumerate(columns):
+        for n in range(N):
+            code = (3 * i + 5 * n) % 16
+            byte = int(q[n, k // 2])
+            q[n, k // 2] = (byte & 0x0F) | code << 4 if k % 2 else (byte & 0xF0) | code
+            for t in range(T):
+                want[t, n] += (code - 8) * 2.0 ** ((i + t) % 3)
+        for t in range(T):
+            x[t, k] = 2.0 ** ((i + t) % 3)
+    out, ws = du.linear(dict(q=q, s=s, z=None), x)
+    du.flags(ws)
+    assert torch.equal(out.cpu().to(torch.float64), want)  # small whole numbers: exact in every step

@@ -114,13 +114,13 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volati
     return __all_sync(0xffffffffu, there || mbar_wait(bar, parity, abort_flag));
 }
 // The same for waits that are long by nature: sleeps between polls, so that the warp takes no issue slots from those that work.
-// Gives up after about a quarter of a second.
-__device__ __forceinline__ bool warp_sleep_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag)
+// Gives up after about a quarter of a second and 8 us more for each of the `steps` that the wait is for.
+__device__ __forceinline__ bool warp_sleep_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag, uint32_t steps)
 {
     bool ok = true;
     if ((threadIdx.x & 31) == 0) {
         ok = false;
-        for (uint32_t i = 0; i < (1u << 21); i++) {
+        for (uint32_t i = 0; i < (1u << 21) + 64 * steps; i++) {
             if (mbar_test_wait(bar, parity)) {
                 ok = true;
                 break;

@@ -472,7 +472,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                 factor[j] = __ldg(w.token + min(tt * N_TILE + j, s.T - 1));
             // one warp asks, sleeping in between, and the others wait at a barrier that costs no issue slots
             if (warp == kTcEpilogueWarp)
-                ok = warp_sleep_wait(&acc_full[buf], (use / NBUF) & 1, abort_flag);
+                ok = warp_sleep_wait(&acc_full[buf], (use / NBUF) & 1, abort_flag, n_kb);
             if (!named_barrier_and(ok)) {
                 ok = false;
                 break;
