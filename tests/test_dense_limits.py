@@ -54,3 +54,22 @@ def test_the_longest_rows(T, K):
     out, ws = du.linear(dict(q=q, s=s, z=None), x)
     du.flags(ws)
     assert torch.equal(out.cpu().to(torch.float64), want)  # small whole numbers: exact in every step
+
+
+# ---- the range of f32 -------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [4, 17, 40, 130, 300])
+@pytest.mark.parametrize("x_power, s_power", [(122, -70), (-100, 90), (60, -60), (-60, 50), (118, -6)])
+def test_tokens_and_scales_at_opposite_ends_of_the_range(T, x_power, s_power):
+    # the result is within f32, whatever the order of its factors would give (the last pair: up to 1e38)
+    g = du.gen(T)
+    N, K = 200, 512
+    w, x = du.weight(g, N, K, 32, True), du.bf16(g, (T, K))
+    x = (x.float().clamp(-3.9, 3.9) * 2.0**x_power).to(torch.bfloat16)
+    # every other row of even scales, and of scales 2^14 apart: both kinds that the conversion knows
+    spread = torch.randint(0, 15, w["s"].shape, generator=g, device="cuda") * (torch.arange(N, device="cuda") % 2).view(N, 1)
+    w["s"] = (w["s"].float() * 2.0 ** (spread + s_power)).to(torch.bfloat16)
+    out, ws = du.linear(w, x)
+    du.flags(ws)
+    ref, tol = du.linear_reference(w, x)
+    du.assert_close(out, ref, tol)

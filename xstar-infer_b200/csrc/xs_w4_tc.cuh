@@ -176,6 +176,16 @@ __device__ __forceinline__ void tc_tile(const TcShape &s, int item, int &wt, int
     tt = first + r - wt * width;
 }
 
+// The factor of a weight row in two: a sum is multiplied by what shrinks it, then by its token's factor, then by what makes it grow, so that
+// neither a token near the largest number against a row of small scales nor the reverse leaves the range of f32 on the way.
+struct RowFactor {
+    float shrink, grow;
+    __device__ __forceinline__ explicit RowFactor(float f) : shrink(fminf(fabsf(f), 1.0f)), grow(fmaxf(fabsf(f), 1.0f)) {}
+    __device__ __forceinline__ float of(float v, float token) const
+    {
+        return v * shrink * token * grow;
+    }
+};
 // One element of the result: v, or act(v) u; in bf16, or in f32 for the product that follows.
 template <bool GATED, typename Out>
 __device__ __forceinline__ Out tc_result(int act, float v, float u)
@@ -481,7 +491,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
             const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16) + kTcAccCol + buf * N_TILE + part * COLS;
             const int feature = s.f0 + wt * FEATURES * CG + block_feature + lane_feature, token0 = tt * N_TILE + part * COLS;
             const int f0 = min(feature, s.n_out - 1);
-            const float row_f = fabsf(__ldg(w.row + f0)), row_u = GATED ? fabsf(__ldg(w.row + s.n_out + f0)) : 0.0f;
+            const RowFactor row_f(__ldg(w.row + f0)), row_u(GATED ? __ldg(w.row + s.n_out + f0) : 0.0f);
             if (CG == 1 && s.split > 1) {
                 // the sums of this block's slice of K, [token][lane], over the operand ring, which nothing reads or fills any more
                 float *red = reinterpret_cast<float *>(smem);
@@ -523,14 +533,14 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
                         const float got = __shfl_xor_sync(0xffffffffu, up ? even : uneven, 16), f = up ? tf[i + 1] : tf[i];
                         const int t = token0 + c + i + (up ? 1 : 0);
                         if (whole || (feature < s.n_out && t < s.T))
-                            *o = tc_result<true, Out>(act, (up ? got : even) * f * row_f, (up ? uneven : got) * f * row_u);
+                            *o = tc_result<true, Out>(act, row_f.of(up ? got : even, f), row_u.of(up ? uneven : got, f));
                         o += 2 * static_cast<size_t>(s.n_out);
                     }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
                         if (whole || (feature < s.n_out && token0 + c + i < s.T))
-                            *o = tc_result<false, Out>(act, __uint_as_float(v[i]) * tf[i] * row_f, 0.0f);
+                            *o = tc_result<false, Out>(act, row_f.of(__uint_as_float(v[i]), tf[i]), 0.0f);
                         o += s.n_out;
                     }
                 }
@@ -578,8 +588,8 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__
 #pragma unroll
             for (int j = 0; j < 4; j++)
                 if (feature + j < s.n_out)
-                    o[j] = tc_result<GATED, Out>(act, sv[j] * t * fabsf(__ldg(w.row + feature + j)),
-                                                 GATED ? su[j] * t * fabsf(__ldg(w.row + s.n_out + feature + j)) : 0.0f);
+                    o[j] = tc_result<GATED, Out>(act, RowFactor(__ldg(w.row + feature + j)).of(sv[j], t),
+                                                 GATED ? RowFactor(__ldg(w.row + s.n_out + feature + j)).of(su[j], t) : 0.0f);
         }
     }
     if (*abort_flag)
