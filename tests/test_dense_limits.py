@@ -73,3 +73,22 @@ def test_tokens_and_scales_at_opposite_ends_of_the_range(T, x_power, s_power):
     du.flags(ws)
     ref, tol = du.linear_reference(w, x)
     du.assert_close(out, ref, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 3, 17, 130])
+def test_a_gated_product_just_below_the_largest_number(T):
+    # 2 a a = 3.4021e38, between 3.4e38 and the largest f32: a number like any other
+    H = I = 32
+    a = 181 / 128 * 2.0**63
+    gu = dict(q=torch.full((2 * I, H // 2), 0x88, dtype=torch.uint8, device="cuda"), s=torch.ones(2 * I, 1, dtype=torch.bfloat16, device="cuda"), z=None)
+    dn = dict(q=torch.full((H, I // 2), 0x88, dtype=torch.uint8, device="cuda"), s=torch.full((H, 1), 2.0**-64, dtype=torch.bfloat16, device="cuda"), z=None)
+    gu["q"][0, 0] = gu["q"][I, 0] = 0x89  # gate and up of the first feature: 1 times their scale
+    gu["s"][0] = 2.0
+    dn["q"][:, 0] = 0x89
+    x = torch.zeros(T, H, dtype=torch.bfloat16, device="cuda")
+    x[:, 0] = a
+    out, ws = du.mlp(gu, dn, x, "silu")
+    du.flags(ws)
+    want = 2 * a * a * 2.0**-64
+    assert ((out.to(du.F) - want).abs() <= (du.HALF + 2.0**-11) * want).all()

@@ -3,6 +3,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <stdint.h>
 
 #include "xs_ptx.cuh"
@@ -88,7 +89,7 @@ __device__ __forceinline__ int log2_floor(float v)
 __device__ __forceinline__ float finite_abs(float v)
 {
     const float a = fabsf(v);
-    return a <= 3.4e38f ? a : 0.0f; // infinities and NaN do not count
+    return a <= FLT_MAX ? a : 0.0f; // infinities and NaN do not count
 }
 
 // The power of two that brings a token whose largest element is `top` to 2^13 .. 2^14.

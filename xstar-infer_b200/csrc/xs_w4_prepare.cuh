@@ -197,14 +197,14 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const PrepareA
             return w;
         };
         auto finish = [&](const Row &w) {
-            float top = 0.0f, low = 3.4e38f;
+            float top = 0.0f, low = FLT_MAX;
             bool odd = false; // an infinity or NaN
             for (int g = sub * 8; g < m.groups; g += m.lanes * 8) {
                 const uint4 v = g == sub * 8 ? w.s0 : scales(w, g);
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const float f = fabsf(prep_get(v, j)), c = finite_abs(f);
-                    odd |= !(f <= 3.4e38f);
+                    odd |= !(f <= FLT_MAX);
                     top = fmaxf(top, c);
                     low = c > 0.0f ? fminf(low, c) : low;
                 }
