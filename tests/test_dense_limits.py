@@ -7,6 +7,7 @@ import torch
 from xstar_moe import capi
 
 import dense_util as du
+from bridge import xstar_cpp as xs
 
 
 def _w4(rows, cols, group=128):
@@ -29,6 +30,44 @@ def test_rows_that_no_shared_memory_holds_ask_for_the_scratch_of_larger_batches(
         gate_up, down = _w4(2 * w.cols, 128), _w4(128, w.cols)
         assert L.xs_moe_mlp_w4_workspace_bytes(C.byref(gate_up), C.byref(down), tokens, C.byref(n)) == 0
         assert n.value > 2 * tokens * w.cols + 2 * gate_up.rows
+
+
+# ---- no tokens --------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["none", "channel", "row", "full"])
+def test_empty_batches_do_nothing_and_need_no_addresses(kind):
+    """a tensor without elements has no address: the gate of an empty batch, its rows and its result"""
+    L = capi.lib()
+    gate = 4096 if kind == "channel" else None
+    a = capi.XsMoeNormResidual()
+    a.gate_dev, a.gate_kind, a.rows, a.hidden, a.eps = gate, du.GATE[kind], 0, 64, 1e-6
+    a.post_weight_dev = a.next_weight_dev = 4096
+    assert L.xs_moe_norm_residual(C.byref(a), None) == 0
+    n = capi.XsMoeBlockNorms()
+    n.pre_weight_dev, n.gate_dev, n.gate_kind, n.eps = 4096, gate, du.GATE[kind], 1e-6
+    assert L.xs_moe_mlp_w4_block(C.byref(_w4(256, 64, 64)), C.byref(_w4(64, 128, 64)), 0, C.byref(n), None, 0, None, None, 0, None) == 0
+    cfg = capi.make_config(T=0, H=512, E=16, K=4, I=256, S=0)
+    assert L.xs_moe_normed_block_forward(C.byref(cfg), C.byref(capi.XsMoeWeights()), C.byref(n), None, None, None, 0, None) == 0
+    # what is wrong without tokens is wrong all the same
+    n.gate_kind = 4
+    assert L.xs_moe_mlp_w4_block(C.byref(_w4(256, 64, 64)), C.byref(_w4(64, 128, 64)), 0, C.byref(n), None, 0, None, None, 0, None) == -1
+    if kind != "none":
+        n.gate_dev, n.gate_kind = None, du.GATE[kind]
+        assert L.xs_moe_mlp_w4_block(C.byref(_w4(256, 64, 64)), C.byref(_w4(64, 128, 64)), 0, C.byref(n), 4096, 3, 4096, None, 0, None) == -1
+
+
+@pytest.mark.gpu
+def test_host_ops_take_empty_tensors_without_an_address():
+    g = du.gen(1)
+    gu_, dn, w = du.weight(g, 256, 512, 64, False), du.weight(g, 512, 128, 64, False), du.bf16(g, (512,))
+    view = lambda t, kind=xs.DType.BFloat16: xs.from_device_ptr(t.data_ptr(), list(t.shape), kind)
+    none = lambda *shape: xs.from_device_ptr(0, list(shape), xs.DType.BFloat16)
+    mats = [view(gu_["q"], xs.DType.UInt4x2), view(gu_["s"]), view(dn["q"], xs.DType.UInt4x2), view(dn["s"])]
+    for gate in (None, view(w), none(0, 1), none(0, 512)):
+        assert xs.mlp_w4_block(none(0, 512), view(w), *mats, gate=gate).shape() == [0, 512]
+        r, n = xs.norm_residual(none(0, 512), none(0, 512), gate=gate, next_norm_weight=view(w))
+        assert r.shape() == n.shape() == [0, 512]
+    assert xs.linear_w4(none(2, 0, 512), *mats[:2]).shape() == [2, 0, 256]
+    assert xs.mlp_w4(none(0, 512), *mats).shape() == [0, 512]
 
 
 # ---- long rows --------------------------------------------------------------------------------------------------------

@@ -697,24 +697,25 @@ int launch_norm_residual(const xs::NormResidualArgs &a, cudaStream_t st)
     return 0;
 }
 
+size_t gate_elems(int kind, size_t rows, size_t hidden)
+{
+    return kind == XS_MOE_GATE_CHANNEL ? hidden : kind == XS_MOE_GATE_ROW ? rows : kind == XS_MOE_GATE_FULL ? rows * hidden : 0;
+}
+
 int check_norm_shape(int gate_kind, const void *gate, int32_t rows, int32_t hidden)
 {
     if (gate_kind < XS_MOE_GATE_NONE || gate_kind > XS_MOE_GATE_FULL)
         return fail(XS_MOE_ERR_INVALID_ARG, "unknown gate kind");
-    if ((gate != nullptr) != (gate_kind != XS_MOE_GATE_NONE))
-        return fail(XS_MOE_ERR_INVALID_ARG, "gate and gate kind disagree");
     if (rows < 0 || hidden <= 0)
         return fail(XS_MOE_ERR_INVALID_ARG, "shape mismatch: non-positive dimension");
+    // a gate without elements (no rows) has no address
+    if (gate ? gate_kind == XS_MOE_GATE_NONE : gate_elems(gate_kind, rows, hidden) != 0)
+        return fail(XS_MOE_ERR_INVALID_ARG, "gate and gate kind disagree");
     if (rows > kMaxDim)
         return fail(XS_MOE_ERR_UNSUPPORTED, "rows must be at most 2^30");
     if (hidden > kNormMaxHidden)
         return fail(XS_MOE_ERR_UNSUPPORTED, "hidden must be at most %d", kNormMaxHidden);
     return 0;
-}
-
-size_t gate_elems(int kind, size_t rows, size_t hidden)
-{
-    return kind == XS_MOE_GATE_CHANNEL ? hidden : kind == XS_MOE_GATE_ROW ? rows : kind == XS_MOE_GATE_FULL ? rows * hidden : 0;
 }
 
 int check_norm(const XsMoeNormResidual *a)
@@ -725,14 +726,14 @@ int check_norm(const XsMoeNormResidual *a)
         return fail(XS_MOE_ERR_INVALID_ARG, "reserved fields must be zero");
     if (int rc = check_norm_shape(a->gate_kind, a->gate_dev, a->rows, a->hidden))
         return rc;
+    if (a->rows == 0)
+        return 0;
     if (!a->residual_dev)
         return fail(XS_MOE_ERR_INVALID_ARG, "null tensor pointer");
     if ((a->next_weight_dev != nullptr) != (a->next_out_dev != nullptr))
         return fail(XS_MOE_ERR_INVALID_ARG, "next weight and next output go together");
     if (a->y_dev ? !a->residual_out_dev : (a->residual_out_dev || a->post_weight_dev || a->gate_dev || !a->next_out_dev))
         return fail(XS_MOE_ERR_INVALID_ARG, "y and residual_out go together; without y there is only the next norm");
-    if (a->rows == 0)
-        return 0;
     const void *ptr[] = {a->y_dev, a->residual_dev, a->post_weight_dev, a->gate_dev, a->next_weight_dev, a->residual_out_dev, a->next_out_dev};
     const char *name[] = {"y", "residual", "post weight", "gate", "next weight", "residual_out", "next_out"};
     const size_t full = static_cast<size_t>(a->rows) * a->hidden, h = a->hidden;
@@ -779,7 +780,7 @@ int run_norm(const XsMoeNormResidual *a, cudaStream_t st)
     return launch_norm_residual(k, st);
 }
 
-int check_block_norms(const XsMoeBlockNorms *n, int32_t rows, int32_t hidden, int dev)
+int check_block_norms(const XsMoeBlockNorms *n, int32_t rows, int32_t hidden)
 {
     if (!n)
         return fail(XS_MOE_ERR_INVALID_ARG, "norms are null");
@@ -789,6 +790,11 @@ int check_block_norms(const XsMoeBlockNorms *n, int32_t rows, int32_t hidden, in
         return rc;
     if (!n->pre_weight_dev)
         return fail(XS_MOE_ERR_INVALID_ARG, "null tensor pointer");
+    return 0;
+}
+
+int check_block_norms_data(const XsMoeBlockNorms *n, int dev)
+{
     const void *ptr[] = {n->pre_weight_dev, n->post_weight_dev, n->gate_dev};
     const char *name[] = {"pre weight", "post weight", "gate"};
     for (int i = 0; i < 3; i++) {
@@ -975,14 +981,16 @@ int xs_moe_mlp_w4_block(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t act
     return guarded([&]() -> int {
         if (int rc = check_mlp_shape(gate_up, down, activation, tokens))
             return rc;
-        int dev = 0;
-        if (int rc = current_device(&dev))
-            return rc;
         const int32_t H = gate_up->cols;
-        if (int rc = check_block_norms(norms, tokens, H, dev))
+        if (int rc = check_block_norms(norms, tokens, H))
             return rc;
         if (tokens == 0)
             return 0;
+        int dev = 0;
+        if (int rc = current_device(&dev))
+            return rc;
+        if (int rc = check_block_norms_data(norms, dev))
+            return rc;
         const size_t inner = mlp_bytes(gate_up, down, tokens), row_bytes = bf16_bytes(tokens, H), need = inner + 2 * row_bytes;
         if (int rc = check_workspace(ws, ws_bytes, need))
             return rc;
@@ -1028,13 +1036,15 @@ int xs_moe_normed_block_forward(const XsMoeConfig *cfg, const XsMoeWeights *w, c
         if (int rc = xs_moe_workspace_bytes(cfg, &fwd))
             return rc;
         const int32_t T = cfg->num_tokens, H = cfg->hidden;
-        int dev = 0;
-        if (int rc = current_device(&dev))
-            return rc;
-        if (int rc = check_block_norms(norms, T, H, dev))
+        if (int rc = check_block_norms(norms, T, H))
             return rc;
         if (T == 0)
             return 0;
+        int dev = 0;
+        if (int rc = current_device(&dev))
+            return rc;
+        if (int rc = check_block_norms_data(norms, dev))
+            return rc;
         const size_t row_bytes = bf16_bytes(T, H), inner = align_up(fwd, 256), need = inner + 2 * row_bytes;
         if (int rc = check_workspace(ws, ws_bytes, need))
             return rc;
