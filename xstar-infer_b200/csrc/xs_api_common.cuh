@@ -189,7 +189,6 @@ inline int make_tmap_bytes(CUtensorMap *m, const void *base, uint64_t rows, uint
 }
 
 struct DeviceInfo {
-    int ok = 0;
     int sms = 0;
     int max_smem = 0;
 };
@@ -198,8 +197,11 @@ inline int device_info(DeviceInfo *out)
 {
     int dev = 0;
     XS_CUDA(cudaGetDevice(&dev));
+    // written before `known` says so: a second thread's first call must not see half of it
     static DeviceInfo cache[64];
-    if (dev < 64 && cache[dev].ok) {
+    static std::atomic<bool> known[64];
+    static std::mutex mu;
+    if (dev < 64 && known[dev].load(std::memory_order_acquire)) {
         *out = cache[dev];
         return 0;
     }
@@ -210,11 +212,15 @@ inline int device_info(DeviceInfo *out)
     if (major != 10)
         return fail(XS_MOE_ERR_DEVICE, "this library holds sm_100a kernels only; device %d has compute capability %d.x", dev, major);
     DeviceInfo d;
-    d.ok = 1;
     d.sms = sms;
     d.max_smem = smem;
-    if (dev < 64)
-        cache[dev] = d;
+    if (dev < 64) {
+        std::lock_guard<std::mutex> lock(mu);
+        if (!known[dev].load(std::memory_order_relaxed)) {
+            cache[dev] = d;
+            known[dev].store(true, std::memory_order_release);
+        }
+    }
     *out = d;
     return 0;
 }
