@@ -41,9 +41,10 @@ typedef enum XsMoeActivation {
 } XsMoeActivation;
 
 /* out (tokens, rows) bf16 = x (tokens, cols) bf16 times W^T; f32 sums, one rounding at the end.  Small
- * batches (up to 8 tokens of 32768 columns, up to 16 of 8192) multiply with the exact weights; larger ones go to the tensor core
- * in f16, tokens and weight rows scaled by powers of two: a weight is rounded once to 11 bits, tokens are exact down to 2^-27 of
- * their largest element.
+ * batches (up to 8 tokens of 32768 columns, up to 16 of 8192) multiply with the exact weights; their tokens are below 2^123, so that a
+ * group's sum of (q - z) x is within f32.  Larger ones go to the tensor core in f16, tokens and weight rows scaled by powers of
+ * two: a weight is rounded once to 11 bits, fewer where its scale is below 2^-20 of the largest of its row, and tokens are exact
+ * down to 2^-27 of their largest element (smaller elements are off by 2^-39 of it at most).
  * x is 16-byte aligned; what a call writes may not overlap what it reads.  Takes the role of gemm_launch behind linear
  * (xstar_cpp/include/ops/gemm.h:165-176). */
 int xs_moe_linear_w4_workspace_bytes(const XsMoeW4 *w, int32_t tokens, size_t *bytes);
@@ -58,7 +59,8 @@ int xs_moe_gated_w4(const XsMoeW4 *gate_up, int32_t activation, const void *x_de
 
 /* out (tokens, H) bf16 = (act(x Wg^T) * (x Wu^T)) Wd^T, gate_up (2I, H), down (H, I): the reference's
  * mlp(x, gate_up_weight, down_weight) (xstar_cpp/include/ops/mlp.h:51) with 4-bit weights.  The product of the first half is
- * rounded once, to f16, scaled by a power of two for each token. */
+ * held in f32 and rounded once, to f16, after a power of two has brought each token's largest element of it (up to 16 tokens: each
+ * part of a token that is summed together) to 2^13 .. 2^14: 11 bits down to 2^-27 of that element. */
 int xs_moe_mlp_w4_workspace_bytes(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t tokens, size_t *bytes);
 int xs_moe_mlp_w4(const XsMoeW4 *gate_up, const XsMoeW4 *down, int32_t activation, const void *x_dev, int32_t tokens,
                   void *out_dev, void *workspace_dev, size_t workspace_bytes, void *stream);

@@ -5,8 +5,8 @@
 // first sum, several rows are in work on an SM and hide one another's sums, and a sum costs one barrier of the row's warps (the
 // partial sums alternate between two places).  The weights stay in L1 rather than in registers: more rows fit an SM.
 //
-// Measured: 8192 x 4096 with a full gate 53.5 us, 6.27 TB/s (97 % of a copy); 777 x 2885 at odd addresses 8.2 us (2.2 TB/s: pieces
-// overlap their neighbours); one row 2.1 us.
+// Measured: 8192 x 4096 with a full gate 54 us, 6.2 TB/s (96 % of a copy); 777 x 2885 at odd addresses 8.1 us (2.2 TB/s: one wave of rows,
+// whose two sums and the loads of weights behind each follow one another); one row 2.2 us.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>

@@ -16,13 +16,13 @@
 // word t of row g to lane (g, t), which is the fragment layout.  The MMA sums (q - z) x in f32; the scale multiplies the f32 sum of
 // a group, so the weights are never rounded.
 //
-// Measured: 1 x 4096 x 4096 5.5 us, of which some 4 are launch, first load and sums; 7 x 4096 x 32003 with zero points 24 us, 3.0
+// Measured: 1 x 4096 x 4096 5.4 us, of which some 4 are launch, first load and sums; 7 x 4096 x 32003 with zero points 24 us, 3.0
 // TB/s, half of the issue slots used: registers hold sixteen warps an SM, with chains of conversion and MMA between their loads.
 //
 // An MLP hands its gated product on in f32 (HALF): rounded to bf16 it would add as much error as the result's own rounding.  The
 // second product brings each token, or its slice of one, to a largest element of 2^13 .. 2^14 by a power of two, rounds it once to
 // the eleven bits of f16, and multiplies with f16 codes, which are as exact as those in bf16.  Against bf16 rows that costs 0.3 to 0.5 us
-// (one token of 4096 x 2048: 10.2 us for 9.7, with an error of 0.0017 for 0.0025); as a second bf16 row of what the first leaves it
+// (one token of 4096 x 2048: 10.0 us in all, with an error of 0.0017 for 0.0025); as a second bf16 row of what the first leaves it
 // cost 0.7, and half as much K fits.
 #pragma once
 #include <cuda_bf16.h>

@@ -20,10 +20,10 @@
 // parked wait about 300, an expect or a load 100 each): with 64 columns one loading thread took 600 cycles a block, whatever the
 // tile, and everybody else waited for it.
 //
-// Measured: 4096 x 4096 x 8192 190 to 197 us with the preparation, 1.40 to 1.45 PFLOP/s of the 1.66 that the library reaches on this part; 8192 x
-// 8192 x 8192 770 us (1.43).  With few tokens the conversion of the codes is the work, 0.42 to 0.46 us for a block of 128 x
+// Measured: 4096 x 4096 x 8192 194 us with the preparation at 1965 MHz, 1.42 PFLOP/s of the 1.66 that the library reaches there, and 226 us
+// in a long run under the power cap (about 1480 MHz), 1.22 of 1.37; 8192 x 8192 x 8192 739 us (1.49).  With few tokens the conversion of the codes is the work, 0.42 to 0.46 us for a block of 128 x
 // 128 weights: the sixteen warps use half of the issue slots, the tensor pipe is active 19 % of the time, and six stages instead of four gain 1 %.
-// 45 x 4096 x 20480 takes 39 us, 83 x 11264 x 4096 27 us, where the bytes would take 8 and 5.
+// 45 x 4096 x 20480 takes 38 us, 83 x 11264 x 4096 25 us, where the bytes would take 8 and 5.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
