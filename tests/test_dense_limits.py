@@ -32,6 +32,18 @@ def test_rows_that_no_shared_memory_holds_ask_for_the_scratch_of_larger_batches(
         assert n.value > 2 * tokens * w.cols + 2 * gate_up.rows
 
 
+def test_the_workspace_of_an_mlp_grows_by_what_its_tokens_need():
+    """tokens and gated product in 16 bits, and no more than half a gigabyte of that product in 32"""
+    L, n, h, i = capi.lib(), C.c_size_t(0), 4096, 12288
+    last = 0
+    for tokens in (1, 16, 17, 512, 8192, 10752, 10753, 16384, 65536, 2**20):
+        assert L.xs_moe_mlp_w4_workspace_bytes(C.byref(_w4(2 * i, h)), C.byref(_w4(h, i)), tokens, C.byref(n)) == 0
+        assert last <= n.value, "a workspace for more tokens serves fewer"
+        last = n.value
+        weights = 3 * h * i // 128 * 3 + 4 * (2 * i + h)
+        assert n.value <= tokens * (2 * h + 2 * i + 4) + min(4 * tokens * i, 2**29) + weights + 2**14
+
+
 # ---- no tokens --------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("kind", ["none", "channel", "row", "full"])
 def test_empty_batches_do_nothing_and_need_no_addresses(kind):

@@ -166,6 +166,23 @@ def test_mlp_with_a_long_gated_product(T, H, I):
 
 
 @pytest.mark.gpu
+def test_mlp_whose_gated_product_goes_through_memory_in_parts():
+    # 2^19 columns: 256 tokens at a time; the second part has 44
+    T, H, I = 300, 32, 2**19
+    g = du.gen(19)
+    gu, dn = du.weight(g, 2 * I, H, 32, False, std=H**-0.5), du.weight(g, H, I, 128, False, std=I**-0.5)
+    x = (du.bf16(g, (T, H)).float() * 2.0 ** torch.randint(-3, 4, (T, 1), generator=g, device="cuda")).to(torch.bfloat16)
+    out, ws = du.mlp(gu, dn, x, "gelu")
+    du.flags(ws)
+    ref = mlp_exact(gu, dn, x, "gelu")
+    for rows in (slice(0, 256), slice(256, T)):  # a tensor of rows of its own size, each brought to its norm
+        unit = ref[rows].norm(dim=-1, keepdim=True)
+        assert du.rel_l2(out[rows].to(du.F) / unit, ref[rows] / unit) < allowed(ref[rows].reshape(1, -1), D_MLP + I**0.5 * 2.0**-23).item()
+    few = du.mlp(gu, dn, x[256:].contiguous(), "gelu")[0]  # a tile of another shape sums in another order
+    assert du.rel_l2(few, out[256:].to(du.F)) < du.HALF
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [1, 16, 17, 300])
 def test_mlp_gives_the_same_bits_each_time_and_for_each_token(T):
     gu, dn, g = _mlp(300 + T, True)

@@ -481,12 +481,20 @@ bool small_mlp(const XsMoeW4 *gu, const XsMoeW4 *dn, int T)
 
 // Scratch of the tensor-core kernel: tokens and scales in f16, zero points, factors; of an MLP also its gated product.
 struct TcScratch {
-    size_t x16 = 0, token = 0, h = 0, scales[2] = {}, zeros[2] = {}, row[2] = {}, bytes = 0;
+    size_t x16 = 0, h16 = 0, token = 0, h = 0, scales[2] = {}, zeros[2] = {}, row[2] = {}, bytes = 0;
 };
 
 int groups_pitch(const XsMoeW4 *w)
 {
     return (w->cols / w->group + 7) / 8 * 8;
+}
+
+// Tokens whose gated product is in memory as f32 at one time: 512 MB of it, and all tokens up to there (8192 of 12288 columns are 403).
+int gated_part(const XsMoeW4 *down, int T)
+{
+    constexpr size_t kBytes = size_t(512) << 20, kTile = 256;
+    const size_t tokens = kBytes / (static_cast<size_t>(down->cols) * 4) / kTile * kTile, part = tokens < kTile ? kTile : tokens;
+    return part < static_cast<size_t>(T) ? static_cast<int>(part) : T;
 }
 
 TcScratch plan_scratch(const XsMoeW4 *first, const XsMoeW4 *second, int T)
@@ -498,11 +506,15 @@ TcScratch plan_scratch(const XsMoeW4 *first, const XsMoeW4 *second, int T)
         at = align_up(at + bytes, 256);
         return o;
     };
-    // the second product's tokens take the place of the first one's
-    p.x16 = take(static_cast<size_t>(T) * (second && second->cols > first->cols ? second->cols : first->cols) * 2);
+    const size_t x_bytes = static_cast<size_t>(T) * first->cols * 2, h16_bytes = second ? static_cast<size_t>(T) * second->cols * 2 : 0;
+    const int part = second ? gated_part(second, T) : T;
+    // the second product's tokens take the place of the first one's where those are done with
+    p.x16 = p.h16 = take(part == T && h16_bytes > x_bytes ? h16_bytes : x_bytes);
+    if (part < T)
+        p.h16 = take(h16_bytes);
     p.token = take(static_cast<size_t>(T) * 4);
     if (second)
-        p.h = take(static_cast<size_t>(T) * second->cols * 4);
+        p.h = take(static_cast<size_t>(part) * second->cols * 4);
     const XsMoeW4 *w[2] = {first, second};
     for (int i = 0; i < 2; i++) {
         if (!w[i])
@@ -619,11 +631,17 @@ int run_mlp(const XsMoeW4 *gu, const XsMoeW4 *dn, int32_t act, const XsMoeBlockN
     if (int rc = launch_prepare(gu, dn, norm, x, T, ws, p, st))
         return rc;
     float *h = reinterpret_cast<float *>(ws + p.h), *token = reinterpret_cast<float *>(ws + p.token);
-    if (int rc = launch_tc<true>(gu, ws + p.x16, T, h, operands(gu, ws, p, 0), act, status, st))
-        return rc;
-    XS_CUDA(launch_pdl(xs::w4_rescale_kernel, T, xs::kRescaleThreads, 0, st, h, reinterpret_cast<__half *>(ws + p.x16), token, dn->cols));
-    note_launch();
-    return launch_tc<false>(dn, ws + p.x16, T, static_cast<__nv_bfloat16 *>(out), operands(dn, ws, p, 1), 0, status, st);
+    for (int t = 0, part = gated_part(dn, T); t < T; t += part) {
+        const int n = part < T - t ? part : T - t;
+        xs::TcOperands up = operands(gu, ws, p, 0);
+        up.token += t;
+        if (int rc = launch_tc<true>(gu, ws + p.x16 + static_cast<size_t>(t) * gu->cols * 2, n, h, up, act, status, st))
+            return rc;
+        __half *h16 = reinterpret_cast<__half *>(ws + p.h16) + static_cast<size_t>(t) * dn->cols;
+        XS_CUDA(launch_pdl(xs::w4_rescale_kernel, n, xs::kRescaleThreads, 0, st, h, h16, token + t, dn->cols));
+        note_launch();
+    }
+    return launch_tc<false>(dn, ws + p.h16, T, static_cast<__nv_bfloat16 *>(out), operands(dn, ws, p, 1), 0, status, st);
 }
 
 template <int GROUP, int ITER, bool ALIGNED>
